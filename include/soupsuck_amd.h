@@ -35,7 +35,8 @@ enum ss_status {
   SS_ERR_UNSUPPORTED = -3
 };
 
-enum ss_dtype { SS_F16 = 0, SS_F32 = 1 };
+/* SS_BF16 (bfloat16 bits) only where an entry point says so. */
+enum ss_dtype { SS_F16 = 0, SS_F32 = 1, SS_BF16 = 2 };
 
 /* Library identity and the last error message of the calling thread. */
 int ss_abi_version(void);
@@ -534,6 +535,119 @@ int ss_attn_varlen_bwd(const void* q, int64_t q_tok, int64_t q_head, const void*
                        int64_t dq_head, void* dk, int64_t dk_tok, int64_t dk_head, void* dv,
                        int64_t dv_tok, int64_t dv_head, void* workspace, size_t workspace_bytes,
                        void* stream);
+
+/* ------------------------------------------------ paged key-value cache ---
+ * No counterpart in the reference (it trains only): what generation with the
+ * tuned projections needs.
+ *
+ * Keys and values lie in pages of page_size rows.  A sequence's rows are named by
+ * its line of a block table (int32 [rows, row_pages] with a stride between lines,
+ * unit between entries): row j of the sequence is row j % page_size of page
+ * table[j / page_size].  A table entry outside [0, pages) is a page that the
+ * sequence does not hold: its rows are never read or written, and no query sees
+ * them.  lengths (int32 [rows], on the device like the table) counts a sequence's
+ * rows, the tokens of the call included; what exceeds row_pages * page_size or is
+ * negative is cut off.
+ *
+ * New tokens of all sequences are packed back to back; cu_seqlens (int32
+ * [rows + 1], nondecreasing from 0) gives each sequence's own, and its last n
+ * cache rows, lengths - n .., are theirs in order.
+ *
+ * k / v: base of [pages, kv_heads, page_size, head_dim] tensors with any page,
+ * head and row strides (elements, multiples of 8) and a unit last stride, 16-byte
+ * aligned, fp16 or bf16; head_dim 128, page_size a multiple of 16. */
+typedef struct ss_paged_cache {
+  void* k;
+  int64_t k_page, k_head, k_row;
+  void* v;
+  int64_t v_page, v_head, v_row;
+  int pages, page_size, kv_heads, head_dim;
+  int dtype; /* SS_F16 or SS_BF16 */
+} ss_paged_cache;
+
+/* Writes k (rotated if cos is given) and v [tokens, kv_heads, 128] of the new
+ * tokens into the cache and, if q is given, the rotated q [tokens, q_heads, 128] to
+ * q_out.  Rotation (fp32 products and sum, one rounding): y[c] = x[c] cos[c] -
+ * x[c + 64] sin[c], y[c + 64] = x[c + 64] cos[c + 64] + x[c] sin[c + 64] with the
+ * token's rows of cos / sin [tokens, 128] (cs_dtype the cache's or SS_F32).  Inputs
+ * are (base, token stride, head stride) in elements, of the cache's type, with a
+ * unit last stride, 16-byte aligned bases and strides that are multiples of 8 (of
+ * 4 for fp32 cos / sin).  A token whose row the sequence does not hold is skipped. */
+int ss_kv_append(const ss_paged_cache* cache, const void* k, int64_t k_tok, int64_t k_head,
+                 const void* v, int64_t v_tok, int64_t v_head, const void* q, int64_t q_tok,
+                 int64_t q_head, int q_heads, const void* cos, int64_t cos_tok, const void* sin,
+                 int64_t sin_tok, int cs_dtype, const int32_t* table, int64_t table_stride,
+                 int row_pages, const int32_t* lengths, const int32_t* cu_seqlens, int rows,
+                 int64_t tokens, void* q_out, int64_t qo_tok, int64_t qo_head, void* stream);
+
+/* Scratch bytes of ss_cached_attention (weights: 1 if weights_out is given). */
+size_t ss_cached_attention_workspace_size(int rows, int64_t tokens, int q_heads, int kv_heads,
+                                          int max_new, int64_t max_length, int weights);
+
+/* o = softmax(scale q . k) v of the new tokens over the cache, GQA (kv head = q head
+ * / (q_heads / kv_heads)).  The token at row p of its sequence sees row j if j <= p
+ * and (window == 0 or j > p - window or j < sinks); one that sees nothing gives 0.
+ * What is not seen has no part in the result, infinities and NaN included.  q / o
+ * [tokens, q_heads, 128] of the cache's type, (base, token stride, head stride) as
+ * above.  max_new >= the most tokens of a sequence, max_length >= the greatest
+ * length (rows beyond it are not read).  weights_out (NULL: none) fp32 [rows,
+ * kv_heads, row_pages * page_size] receives weights_in (NULL: 0; may be weights_out
+ * itself) plus each cache row's probabilities, summed over the tokens and the q heads
+ * of its kv head.  workspace: at least ss_cached_attention_workspace_size() bytes,
+ * 16-byte aligned, fully written before it is read. */
+int ss_cached_attention(const ss_paged_cache* cache, const void* q, int64_t q_tok, int64_t q_head,
+                        int q_heads, const int32_t* table, int64_t table_stride, int row_pages,
+                        const int32_t* lengths, const int32_t* cu_seqlens, int rows,
+                        int64_t tokens, int max_new, int64_t max_length, float scale,
+                        int64_t window, int64_t sinks, const float* weights_in,
+                        float* weights_out, void* o, int64_t o_tok, int64_t o_head,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+/* Scratch bytes of ss_kv_evict. */
+size_t ss_kv_evict_workspace_size(int rows, int kv_heads, int64_t budget);
+
+/* Per sequence and kv head, keeps min(length, budget) rows: the first `sinks`, the
+ * last `recent` and the heaviest of the others by weights (fp32 [rows, kv_heads,
+ * row_pages * page_size]; equal ones from the lowest row up, NaN heaviest), sinks +
+ * recent <= budget.  The kept rows go in their order to rows 0 .. of the pages that
+ * out_table (out_pages entries a line, out_pages * page_size >= budget) names, which
+ * must not be pages that `table` names; out_lengths (int32 [rows]) receives their
+ * count and out_weights (fp32 [rows, kv_heads, out_pages * page_size], not
+ * overlapping weights) their weights, 0 behind them.  Rows on pages that the sequence does not hold are
+ * kept like others, as zeros.  max_length >= the greatest length (what exceeds it is
+ * cut off).  workspace: at least ss_kv_evict_workspace_size() bytes, 16-byte aligned. */
+int ss_kv_evict(const ss_paged_cache* cache, const int32_t* table, int64_t table_stride,
+                int row_pages, const int32_t* lengths, int rows, int64_t max_length,
+                const float* weights, const int32_t* out_table, int64_t out_stride, int out_pages,
+                int64_t budget, int64_t sinks, int64_t recent, int32_t* out_lengths,
+                float* out_weights, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------- drafted tokens ---
+ * Scratch bytes of ss_verify_drafts (drafted: 1 with draft logits). */
+size_t ss_verify_drafts_workspace_size(int rows, int drafts, int64_t vocab, int drafted);
+
+/* Checks up to `drafts` drafted tokens (int64 [rows, drafts], contiguous; counts int32 [rows]
+ * of them or NULL for all; a count is cut to 0 .. drafts) of each sequence against
+ * the target's logits [rows, drafts + 1, vocab] from uniform numbers in [0, 1) (fp32
+ * [rows, drafts + 1], contiguous).  With p = softmax(target / temperature) and q =
+ * softmax(draft / temperature) (draft [rows, drafts, vocab]; NULL: q is 1 on the drafted
+ * token), draft i is accepted while u_i q_i(x_i) < p_i(x_i); at the first refusal the
+ * next token is drawn from max(p_i - q_i, 0) (from p_i where that is 0 everywhere), after none
+ * from p at `count`: the first token at which the running sum in token order exceeds
+ * u_drafts times the whole.  Sums and probabilities are fp64.  temperature 0 accepts the
+ * target's largest logit (the lowest token of equal ones) and ends with that of
+ * the next row; uniform and draft may then be NULL.  A NaN logit counts as
+ * -inf, and +inf logits share the whole; a drafted token outside the vocabulary has
+ * p = 0 and is refused; a row with no logit above -inf draws token -1.
+ * Logits are fp16, bf16 or fp32 (both `dtype`), (base, sequence stride, row stride)
+ * in elements with a unit last stride.  accepted int32 [rows]; out int64 [rows,
+ * drafts + 1]: the accepted drafts, the next token, then -1.  workspace: at least
+ * ss_verify_drafts_workspace_size() bytes, 16-byte aligned. */
+int ss_verify_drafts(const void* target, int64_t t_seq, int64_t t_row, const void* draft,
+                     int64_t d_seq, int64_t d_row, int dtype, const int64_t* tokens,
+                     const int32_t* counts, const float* uniform, int rows, int drafts,
+                     int64_t vocab, double temperature, int32_t* accepted, int64_t* out,
+                     void* workspace, size_t workspace_bytes, void* stream);
 
 /* --------------------------------------- lossless fp16 table storage (f4) ---
  * dst[i] = fp16_rne(src[i]) for i < n, and *flag = 1 if any element does not

@@ -15,6 +15,7 @@ LIBRARY = Path(__file__).resolve().parent / "libsoupsuck_amd.so"
 
 F16 = 0
 F32 = 1
+BF16 = 2
 
 OK = 0
 ERR_INVALID_ARGUMENT = -1
@@ -26,7 +27,18 @@ _i64 = ctypes.c_int64
 _u64 = ctypes.c_uint64
 _int = ctypes.c_int
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 _size = ctypes.c_size_t
+
+
+class PagedCacheStruct(ctypes.Structure):
+    """ss_paged_cache of include/soupsuck_amd.h."""
+
+    _fields_ = [("k", _c_void_p), ("k_page", _i64), ("k_head", _i64), ("k_row", _i64),
+                ("v", _c_void_p), ("v_page", _i64), ("v_head", _i64), ("v_row", _i64),
+                ("pages", _int), ("page_size", _int), ("kv_heads", _int), ("head_dim", _int),
+                ("dtype", _int)]
+
 
 # name -> argument types (restype is int unless listed in _RESTYPES)
 SIGNATURES = {
@@ -128,6 +140,21 @@ SIGNATURES = {
                                                            _int, _int, _int, _f32]
                           + [_c_void_p, _i64, _i64] * 3 + [_c_void_p, _size, _c_void_p],
     "ss_attn_varlen_bwd_workspace_size": [_int, _int, _i64],
+    "ss_kv_append": [_c_void_p] + [_c_void_p, _i64, _i64] * 3 + [_int]
+                    + [_c_void_p, _i64] * 2 + [_int, _c_void_p, _i64, _int, _c_void_p, _c_void_p,
+                                               _int, _i64, _c_void_p, _i64, _i64, _c_void_p],
+    "ss_cached_attention_workspace_size": [_int, _i64, _int, _int, _int, _i64, _int],
+    "ss_cached_attention": [_c_void_p, _c_void_p, _i64, _i64, _int, _c_void_p, _i64, _int,
+                            _c_void_p, _c_void_p, _int, _i64, _int, _i64, _f32, _i64, _i64,
+                            _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _c_void_p, _size,
+                            _c_void_p],
+    "ss_kv_evict_workspace_size": [_int, _int, _i64],
+    "ss_kv_evict": [_c_void_p, _c_void_p, _i64, _int, _c_void_p, _int, _i64, _c_void_p,
+                    _c_void_p, _i64, _int, _i64, _i64, _i64, _c_void_p, _c_void_p, _c_void_p,
+                    _size, _c_void_p],
+    "ss_verify_drafts_workspace_size": [_int, _int, _i64, _int],
+    "ss_verify_drafts": [_c_void_p, _i64, _i64] * 2 + [_int] + [_c_void_p] * 3
+                        + [_int, _int, _i64, _f64] + [_c_void_p] * 3 + [_size, _c_void_p],
     "ss_f32_to_f16_exact": [_c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p],
     "ss_hbm_read_probe": [_c_void_p, _i64, _i64, _c_void_p, _c_void_p],
     "ss_ce_finalize_dx": [_c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p, _int, _i64, _i64,
@@ -136,7 +163,9 @@ SIGNATURES = {
 _RESTYPES = {"ss_last_error": ctypes.c_char_p, "ss_nf4_gemm_workspace_size": _size,
              "ss_lora_workspace_size": _size, "ss_qlora_rank_workspace_size": _size,
              "ss_gemm_f16_workspace_size": _size, "ss_add_rmsnorm_dgamma_waves": _i64,
-             "ss_attn_varlen_bwd_workspace_size": _size}
+             "ss_attn_varlen_bwd_workspace_size": _size,
+             "ss_cached_attention_workspace_size": _size, "ss_kv_evict_workspace_size": _size,
+             "ss_verify_drafts_workspace_size": _size}
 
 _lock = threading.Lock()
 _lib = None
