@@ -4,9 +4,41 @@
 // (j <= p, and inside the window or among the sinks), with a running maximum and sum in
 // fp32: m' = max(m, s), l' = l 2^(m - m') + 2^(s - m'), o' likewise, in base-2 scores.
 //
-// One workgroup per (token, q head): its four waves take every fourth visible row, a
-// lane holds two of the 128 columns; the waves' (m, l, o) are joined at the end.  The
-// weights are a second pass over the keys with the joined statistics.
+// A unit of work is one kv head over one block of a sequence's query rows (token-major, the
+// q heads of the group side by side: all of them share the cache's rows, which are read
+// once for the block).  Its keys go in tiles of 32, dealt to the waves of a workgroup in
+// turn; each wave keeps its own (m, l, o) in registers and meets the others only at the
+// end, so no barrier stands between two loads.
+//
+// Products (v_mfma_f32_16x16x32): S^T = K Q^T, keys down, one query row per lane and
+// column; the accumulator of two 16-key halves is the operand P^T of O^T += V^T P^T as it
+// stands, slots 8 h .. + 7 of lane group h being keys 4 h + i and 16 + 4 h + i.  V is read
+// as whole rows (lane c of a group takes columns 8 c .. + 7 of a key) and turned in
+// registers: tile e of O^T holds the columns 8 c + e.  K rows are the MFMA operand as they
+// lie.  Neither passes through LDS: at HBM's rate a CU gets 13 bytes a clock, against
+// which the 32 permutes and 16 MFMAs of a 16 KiB tile are small, and what counts is the
+// loads in flight: 16 KiB a wave, the next tile's keys issued before this one's softmax
+// and its values before the next scores.
+//
+// Split over the keys (cached_attention_kernel<.., true>): the tiles of all units form one
+// line that is cut into equal ranges, one a workgroup, from the lengths on the device, so
+// that one long sequence and a batch of ragged ones load every CU alike whatever the
+// bounds that the host knows.  A unit inside a range is finished there; of one that
+// crosses ranges each part leaves (o, m, l), and cached_join_kernel adds them up.
+// Bounds on the length up to kWhole give one workgroup a unit and no second launch.
+//
+// Masked rows: a tile that every query row sees whole takes no mask.  In the others scores
+// are replaced (never multiplied) by -inf and the values of rows that no query row sees by
+// 0, so that nothing stored there counts.  A row that some tokens of the block see and
+// others do not keeps its value, and an infinity or NaN in it would reach the others as 0
+// times it: a wave that ends with one such in o repeats its tiles token by token.
+//
+// Weights: the scores (fp32, base 2) are left in the workspace, 4 bytes a query row and
+// key against 256 for the key again, and added up once the statistics are known; where
+// they would be many (more than 32 query rows a kv head, or more than kScoreBytes in all)
+// the keys are multiplied again.
+#include <type_traits>
+
 #include "paged.h"
 #include "elementwise.h"
 
@@ -14,6 +46,13 @@ namespace ss {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kKeys = 32;       // of a tile
+constexpr int kPadDim = kCacheDim + 4;  // fp32 row of the waves' results in LDS
+constexpr int64_t kWhole = 512;
+constexpr size_t kScoreBytes = (size_t)512 << 20;
+constexpr int kSteps = 31;      // tiles of a wave whose pages are looked up at once
+constexpr int kMinTiles = 8;    // of a range
+constexpr int64_t kMaxGrid = (int64_t)1 << 23;  // workgroups of a launch
 
 struct CachedAttnArgs {
   CacheView cache;
@@ -28,113 +67,730 @@ struct CachedAttnArgs {
   int64_t window, sinks;
   const float* w_in;
   float* w_out;
-  float* lse2;  // [tokens][hq], base 2
+  float* lse2;  // [tokens][hq], base 2; +inf where a row sees nothing
+  int max_new, blocks;      // new tokens of a sequence at most; row blocks of as many
+  int workers;              // ranges
+  int4* units;              // [sequences][blocks][kv heads]: first, last worker, slot of the first
+  float* part_ml;           // [workers][2][block rows][2]
+  float* part_o;            // [workers][2][block rows][128]
+  float* scores;            // [sequences][kv heads][score_rows][score_keys]
+  int score_rows;
+  int64_t score_keys;
 };
 
-__device__ __forceinline__ bool visible(const CachedAttnArgs& a, int64_t j, int64_t at) {
-  return j <= at && (a.window == 0 || j > at - a.window || j < a.sinks);
+template <class T>
+using Vec8 = T __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ float4v mfma(Vec8<half_t> a, Vec8<half_t> b, float4v c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ float4v mfma(Vec8<bhalf_t> a, Vec8<bhalf_t> b, float4v c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
+// Powers of two that P is raised by: fp16 holds 2^-14 .. 2^15 in full, and the many small
+// weights beside a large one count together.
 template <class T>
-__device__ __forceinline__ float dot_row(const char* row, int lane, float q0, float q1) {
-  const T* p = reinterpret_cast<const T*>(row) + 2 * lane;
-  return wave_sum((float)p[0] * q0 + (float)p[1] * q1);
+constexpr float kLift = std::is_same<T, half_t>::value ? 15.f : 0.f;
+
+// Over the four lane groups: each swap leaves a pair of rows (halves) of lanes side by side.
+template <class F>
+__device__ __forceinline__ float over_groups(float v, F f) {
+  uint32_t u = __builtin_bit_cast(uint32_t, v);
+  const auto rows = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  u = __builtin_bit_cast(uint32_t, f(__builtin_bit_cast(float, (uint32_t)rows[0]),
+                                     __builtin_bit_cast(float, (uint32_t)rows[1])));
+  const auto halves = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return f(__builtin_bit_cast(float, (uint32_t)halves[0]),
+           __builtin_bit_cast(float, (uint32_t)halves[1]));
+}
+__device__ __forceinline__ float group_max(float v) {
+  return over_groups(v, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ float group_sum(float v) {
+  return over_groups(v, [](float a, float b) { return a + b; });
+}
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+  return (int64_t)((uint64_t)(uint32_t)uniform((int)v) |
+                   (uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32);
 }
 
-template <class T>
-__global__ __launch_bounds__(256) void cached_attention_kernel(CachedAttnArgs a) {
-  __shared__ float part[4][130];
-  const int64_t t = blockIdx.x / a.hq;
-  const int head = (int)(blockIdx.x - t * a.hq);
-  const int kv = head / a.group;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int b = sequence_of(a.cu, a.sequences, t);
-  const int64_t len = b < 0 ? 0 : a.rows.length(b, a.cache.page_size, a.max_length);
-  const int64_t at = b < 0 ? -1 : (int64_t)a.rows.lengths[b] - a.cu[b + 1] + t;
-  const T* q = reinterpret_cast<const T*>(a.q + t * a.q_tok + head * a.q_head) + 2 * lane;
-  const float q0 = (float)q[0], q1 = (float)q[1];
-  float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-  for (int64_t j = wave; j < len; j += 4) {
-    if (!visible(a, j, at)) continue;
-    const int64_t entry = j / a.cache.page_size;
-    const int page = a.rows.page(b, entry, a.cache.pages);
-    if (page < 0) continue;
-    const int64_t r = j - entry * a.cache.page_size;
-    const float s = a.scale_log2 * dot_row<T>(a.cache.k + page * a.cache.k_page +
-                                                  kv * a.cache.k_head + r * a.cache.k_row,
-                                              lane, q0, q1);
-    const T* v = reinterpret_cast<const T*>(a.cache.v + page * a.cache.v_page +
-                                            kv * a.cache.v_head + r * a.cache.v_row) + 2 * lane;
-    const float top = fmaxf(m, s);
-    const float keep = m == -INFINITY ? 0.f : exp2f(m - top);
-    const float p = s == -INFINITY ? 0.f : exp2f(s - top);
-    o0 = o0 * keep + p * (float)v[0];
-    o1 = o1 * keep + p * (float)v[1];
-    l = l * keep + p;
-    m = top;
+__device__ __forceinline__ int clamp_to(int64_t v, int64_t lo, int64_t hi) {
+  return (int)(v < lo ? lo : v > hi ? hi : v);
+}
+
+// The new tokens of sequence b, and the cache rows they see.
+struct Sequence {
+  int start, n, len;  // first packed token, tokens, cache rows
+  int64_t at;         // cache row of the first token
+  __device__ __forceinline__ Sequence(const CachedAttnArgs& a, int b) {
+    const int64_t c0 = clamp_to(a.cu[b], 0, a.tokens), c1 = clamp_to(a.cu[b + 1], 0, a.tokens);
+    start = (int)c0;
+    n = (int)(c1 > c0 ? c1 - c0 : 0);
+    len = (int)a.rows.length(b, a.cache.page_size, a.max_length);
+    at = (int64_t)a.rows.lengths[b] - a.cu[b + 1] + c0;
   }
-  part[wave][2 * lane] = o0;
-  part[wave][2 * lane + 1] = o1;
-  if (lane == 0) part[wave][128] = m, part[wave][129] = l;
+  __device__ __forceinline__ void settle() {  // into scalar registers
+    start = uniform(start);
+    n = uniform(n);
+    len = uniform(len);
+    at = uniform(at);
+  }
+  // Token i sees [low(i), last(i)] and below last(i) the sinks.
+  __device__ __forceinline__ int last(int i) const { return clamp_to(at + i, -1, len - 1); }
+  __device__ __forceinline__ int low(const CachedAttnArgs& a, int i) const {
+    return a.window ? clamp_to(at + i - a.window + 1, 0, len) : 0;
+  }
+};
+
+// The tiles that a block of query rows has to visit: those of the sinks, then from the
+// first token's window to the last token's row.
+struct Span {
+  int i0, i1;     // tokens of the block
+  int low, high;  // rows [low, high) and the sinks below low
+  int sink_tiles, first, tiles;
+  __device__ __forceinline__ Span(const CachedAttnArgs& a, const Sequence& s, int block,
+                                  int block_rows) {
+    const int rows = min(s.n, a.max_new) * a.group;
+    const int r0 = block * block_rows;
+    i0 = r0 / a.group;
+    i1 = (min(rows, r0 + block_rows) - 1) / a.group;
+    tiles = low = high = sink_tiles = first = 0;
+    if (r0 >= rows) return;
+    high = s.last(i1) + 1;
+    low = min(s.low(a, i0), high);
+    sink_tiles = (clamp_to(a.sinks, 0, low) + kKeys - 1) / kKeys;
+    first = max(low / kKeys, sink_tiles);
+    // a block that sees nothing still has its zeros to write
+    tiles = max(sink_tiles + max((high + kKeys - 1) / kKeys - first, 0), 1);
+  }
+  __device__ __forceinline__ int tile(int x) const {
+    return x < sink_tiles ? x : x - sink_tiles + first;
+  }
+};
+
+template <class T, int QT, int W>
+struct Shared {
+  float o[W][16 * QT][kPadDim];
+  float m[W][16 * QT], l[W][16 * QT];
+  int64_t upto[64];
+  int tiles[64];
+};
+
+typedef __amdgpu_buffer_rsrc_t Rsrc;
+
+// The 16 cache rows of half tile h of a wave, whose page and row in it lane h holds.
+__device__ __forceinline__ Rsrc half_tile(int page, int row, int h, const char* base,
+                                          int64_t page_bytes, int64_t row_bytes) {
+  const int p = __builtin_amdgcn_readlane(page, h);
+  const int r = __builtin_amdgcn_readlane(row, h);
+  const char* at = base + (int64_t)max(p, 0) * page_bytes + (int64_t)r * row_bytes;
+  return __builtin_amdgcn_make_buffer_rsrc((void*)at, 0, p < 0 ? 0 : -1, 0x00027000);
+}
+__device__ __forceinline__ u32x4 load16(Rsrc r, uint32_t lane, uint32_t all) {
+  return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, lane, all, 0));
+}
+
+// The tiles [x0, x1) of a unit by the waves of the workgroup, and their join: the result
+// where the range is the whole unit, a partial one in the workspace elsewhere.
+template <class T, int QT, int W, bool SCORES>
+__device__ __forceinline__ void attend(const CachedAttnArgs& a, Shared<T, QT, W>& lds, int b,
+                                       int block, int kv, const Sequence& seq, const Span& span,
+                                       int x0, int x1, bool whole, int slot) {
+  // Opaque, or all that follows from them is computed ahead of the segments' loop and kept
+  // in registers through it (45 more).
+  int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6));
+  asm volatile("" : "+v"(lane), "+s"(wave));
+  const int thread = 64 * wave + lane;
+  const int col = lane & 15, grp = lane >> 4;
+  const int size = a.cache.page_size;
+  const int rows = min(seq.n, a.max_new) * a.group;
+  const int r0 = block * 16 * QT;
+
+  Vec8<T> q[QT][4];  // Q[row][32 ks + 8 grp ..]
+  int last[QT], low[QT];
+  auto token_of = [&](int t) { return min(r0 + 16 * t + col, rows - 1) / a.group; };
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int r = min(r0 + 16 * t + col, rows - 1);
+    const int token = r / a.group;
+    const char* p = a.q + (int64_t)(seq.start + token) * a.q_tok +
+                    (int64_t)(kv * a.group + r - token * a.group) * a.q_head + grp * 16;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) q[t][ks] = *reinterpret_cast<const Vec8<T>*>(p + ks * 64);
+    last[t] = seq.last(token);
+    low[t] = seq.low(a, token);
+  }
+  const int sinks = clamp_to(a.sinks, 0, seq.len);
+  // Tiles that every row of the block sees whole.
+  const int clear_end = seq.last(span.i0) + 1, clear_low = seq.low(a, span.i1);
+  const uint32_t k_lane = (uint32_t)col * (uint32_t)a.cache.k_row + grp * 16;
+  const uint32_t v_lane = (uint32_t)(4 * grp) * (uint32_t)a.cache.v_row + col * 16;
+  const char* k_base = a.cache.k + (int64_t)kv * a.cache.k_head;
+  const char* v_base = a.cache.v + (int64_t)kv * a.cache.v_head;
+  float* scores = SCORES ? a.scores + ((int64_t)b * a.cache.kv_heads + kv) * a.score_rows *
+                                          a.score_keys
+                         : nullptr;
+
+  int only = -1;  // the token whose rows alone count, or all
+  for (;;) {
+    const int see_low = only < 0 ? span.low : seq.low(a, only);
+    const int see_high = only < 0 ? span.high : seq.last(only) + 1;
+    float4v acc[QT][8];
+    float m[QT], l[QT];
+    bool partly = false;
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[t][e] = float4v{0.f, 0.f, 0.f, 0.f};
+      m[t] = -INFINITY;
+      l[t] = 0.f;
+    }
+    // Some of this wave's tiles at a time: their halves' pages in one load, the last two
+    // lanes' none.
+#pragma unroll 1
+    for (int x = x0 + wave; x < x1; x += kSteps * W) {
+      const int steps = uniform(min((x1 - x + W - 1) / W, kSteps));
+      int page = -1, row = 0;
+      {
+        const int j = span.tile(x + (lane >> 1) * W) * kKeys + (lane & 1) * 16;
+        if ((lane >> 1) < steps && j < seq.len) {
+          const int entry = j / size;
+          page = a.rows.page(b, entry, a.cache.pages);
+          row = j - entry * size;
+        }
+      }
+      Vec8<T> kf[2][4];
+      u32x4 vf[8];
+      // Of a half that no page holds, or behind the last tile, nothing is fetched.
+      auto load_k = [&](int s) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const auto half = half_tile(page, row, 2 * s + u, k_base, a.cache.k_page, a.cache.k_row);
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks)
+            kf[u][ks] = __builtin_bit_cast(Vec8<T>, load16(half, k_lane + ks * 64, 0));
+        }
+      };
+      auto load_v = [&](int s) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const auto half = half_tile(page, row, 2 * s + u, v_base, a.cache.v_page, a.cache.v_row);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            vf[4 * u + i] = load16(half, v_lane, i * (uint32_t)a.cache.v_row);
+        }
+      };
+      load_k(0);
+      __builtin_amdgcn_sched_barrier(0);  // in the order of the loop's, for its waits
+      load_v(0);
+#pragma unroll 1
+      for (int s = 0; s < steps; ++s) {
+        const int j0 = span.tile(x + s * W) * kKeys;
+        const bool held0 = __builtin_amdgcn_readlane(page, 2 * s) >= 0;
+        const bool held1 = __builtin_amdgcn_readlane(page, 2 * s + 1) >= 0;
+        float sc[QT][8];
+#pragma unroll
+        for (int t = 0; t < QT; ++t)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            float4v c{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) c = mfma(kf[u][ks], q[t][ks], c);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[t][4 * u + i] = c[i] * a.scale_log2;
+          }
+        // Not before the products: their operands' registers take the next keys.
+        __builtin_amdgcn_sched_barrier(0);
+        load_k(s + 1);
+        const bool clear = j0 + kKeys <= clear_end && held0 && held1 &&
+                           (j0 >= clear_low || j0 + kKeys <= sinks);
+        if (!clear) {
+          partly = true;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int j = j0 + 4 * grp + (i & 3) + 16 * (i >> 2);
+            const bool held = i < 4 ? held0 : held1;
+#pragma unroll
+            for (int t = 0; t < QT; ++t)
+              sc[t][i] = held & (j <= last[t]) & ((j >= low[t]) | (j < sinks)) ? sc[t][i] : -INFINITY;
+            const bool seen = held & (j < see_high) & ((j >= see_low) | (j < sinks));
+#pragma unroll
+            for (int w = 0; w < 4; ++w) vf[i][w] = seen ? vf[i][w] : 0u;
+          }
+        }
+        if constexpr (SCORES) {
+#pragma unroll
+          for (int t = 0; t < QT; ++t)
+            if (16 * t + col < rows) {
+              float* out = scores + (int64_t)(16 * t + col) * a.score_keys + j0 + 4 * grp;
+#pragma unroll
+              for (int u = 0; u < 2; ++u)
+                *reinterpret_cast<float4v*>(out + 16 * u) =
+                    float4v{sc[t][4 * u], sc[t][4 * u + 1], sc[t][4 * u + 2], sc[t][4 * u + 3]};
+            }
+        }
+        Vec8<T> p[QT];
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+          float top = sc[t][0];
+#pragma unroll
+          for (int i = 1; i < 8; ++i) top = fmaxf(top, sc[t][i]);
+          top = fmaxf(m[t], group_max(top));
+          const float base = top == -INFINITY ? 0.f : top;
+          if (__any(top > m[t])) {
+            const float keep = __builtin_amdgcn_exp2f(m[t] - base);
+            l[t] *= keep;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[t][e] *= keep;
+            m[t] = top;
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float w = __builtin_amdgcn_exp2f(sc[t][i] - base + kLift<T>);
+            l[t] += w;
+            p[t][i] = (T)w;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          u32x4 v;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            v[i] = __builtin_amdgcn_perm(vf[2 * i + 1][e >> 1], vf[2 * i][e >> 1],
+                                         e & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+          for (int t = 0; t < QT; ++t)
+            acc[t][e] = mfma(__builtin_bit_cast(Vec8<T>, v), p[t], acc[t][e]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        load_v(s + 1);
+      }
+    }
+    bool odd = false;
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      const float sum = group_sum(l[t]);
+      if (only < 0 || token_of(t) == only) {
+        const int r = 16 * t + col;
+        if (grp == 0) lds.m[wave][r] = m[t], lds.l[wave][r] = sum;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+            *reinterpret_cast<float4v*>(&lds.o[wave][r][32 * grp + 8 * i + 4 * u]) =
+                float4v{acc[t][4 * u][i], acc[t][4 * u + 1][i], acc[t][4 * u + 2][i],
+                        acc[t][4 * u + 3][i]};
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) odd |= !(fabsf(acc[t][e][i]) < INFINITY);
+    }
+    if (only < 0) {
+      if (span.i0 == span.i1 || !partly || !__any(odd)) break;
+      only = span.i0;
+    } else if (only++ == span.i1) {
+      break;
+    }
+  }
   __syncthreads();
-  if (wave) return;
-  float top = -INFINITY;
-  for (int w = 0; w < 4; ++w) top = fmaxf(top, part[w][128]);
-  float sum = 0.f, x0 = 0.f, x1 = 0.f;
-  for (int w = 0; w < 4; ++w) {
-    const float f = part[w][128] == -INFINITY ? 0.f : exp2f(part[w][128] - top);
-    sum += f * part[w][129];
-    x0 += f * part[w][2 * lane];
-    x1 += f * part[w][2 * lane + 1];
+
+  for (int item = thread; item < 16 * QT * 16; item += 64 * W) {
+    const int r = item >> 4, c = (item & 15) * 8;
+    if (r0 + r >= rows) continue;
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < W; ++w) top = fmaxf(top, lds.m[w][r]);
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, o[8] = {};
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float f = __builtin_amdgcn_exp2f(lds.m[w][r] - base);
+      sum += f * lds.l[w][r];
+      const float4v x = *reinterpret_cast<const float4v*>(&lds.o[w][r][c]);
+      const float4v y = *reinterpret_cast<const float4v*>(&lds.o[w][r][c + 4]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        o[i] += f * x[i];
+        o[4 + i] += f * y[i];
+      }
+    }
+    if (whole) {
+      const int i = (r0 + r) / a.group;
+      const int head = kv * a.group + r0 + r - i * a.group;
+      const float inverse = sum == 0.f ? 0.f : 1.f / sum;
+      Vec8<T> out;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) out[e] = (T)(sum == 0.f ? 0.f : o[e] * inverse);
+      *reinterpret_cast<Vec8<T>*>(a.o + (int64_t)(seq.start + i) * a.o_tok + head * a.o_head +
+                                  c * 2) = out;
+      if (a.lse2 && c == 0)
+        a.lse2[(int64_t)(seq.start + i) * a.hq + head] =
+            sum == 0.f ? INFINITY : base - kLift<T> + log2f(sum);
+    } else {
+      const int64_t part = (int64_t)slot * 16 * QT + r;
+      float* out = a.part_o + part * kCacheDim + c;
+      *reinterpret_cast<float4v*>(out) = float4v{o[0], o[1], o[2], o[3]};
+      *reinterpret_cast<float4v*>(out + 4) = float4v{o[4], o[5], o[6], o[7]};
+      if (c == 0) *reinterpret_cast<float2v*>(a.part_ml + part * 2) = float2v{top, sum};
+    }
   }
-  T* o = reinterpret_cast<T*>(a.o + t * a.o_tok + head * a.o_head) + 2 * lane;
-  o[0] = (T)(sum > 0.f || sum != sum ? x0 / sum : 0.f);
-  o[1] = (T)(sum > 0.f || sum != sum ? x1 / sum : 0.f);
-  if (lane == 0 && a.lse2) a.lse2[t * a.hq + head] = top + log2f(sum);
+  // Tokens behind the bound on a sequence's new ones have no part in the call.
+  if (whole || x1 == span.tiles)
+    if (seq.n > a.max_new && block == a.blocks - 1)
+      for (int64_t i = thread; i < (int64_t)(seq.n - a.max_new) * a.group * 16; i += 64 * W) {
+        const int64_t r = i / 16 + (int64_t)a.max_new * a.group;
+        const int64_t t = r / a.group;
+        const int64_t at = (seq.start + t) * a.o_tok + (kv * a.group + r - t * a.group) * a.o_head;
+        *reinterpret_cast<u32x4*>(a.o + at + (i & 15) * 16) = u32x4{0, 0, 0, 0};
+      }
 }
 
-template <class T>
+// Zeros for packed tokens that no sequence has.
+template <int W>
+__device__ __forceinline__ void clear_outside(const CachedAttnArgs& a) {
+  const int64_t head = clamp_to(a.cu[0], 0, a.tokens);
+  const int64_t tail = clamp_to(a.cu[a.sequences], 0, a.tokens);
+  const int64_t per = (int64_t)a.hq * 16;
+  for (int64_t i = threadIdx.x; i < (head + a.tokens - tail) * per; i += 64 * W) {
+    int64_t t = i / per;
+    const int64_t c = i - t * per;
+    if (t >= head) t += tail - head;
+    *reinterpret_cast<u32x4*>(a.o + t * a.o_tok + c / 16 * a.o_head + (c & 15) * 16) =
+        u32x4{0, 0, 0, 0};
+  }
+}
+
+template <class T, int QT, int W, bool SPLIT, bool SCORES>
+__global__ __launch_bounds__(64 * W) void cached_attention_kernel(CachedAttnArgs a) {
+  __shared__ Shared<T, QT, W> lds;
+  const int hk = a.cache.kv_heads;
+  if (blockIdx.x == 0) clear_outside<W>(a);
+  if constexpr (!SPLIT) {
+    const int line = uniform((int)(blockIdx.x / hk)), kv = (int)(blockIdx.x - line * hk);
+    const int b = uniform(line / a.blocks), block = line - b * a.blocks;
+    Sequence seq(a, b);
+    seq.settle();
+    const Span span(a, seq, block, 16 * QT);
+    if (span.tiles)
+      attend<T, QT, W, SCORES>(a, lds, b, block, kv, seq, span, 0, span.tiles, true, 0);
+  } else {
+    // Lines (sequence, block), 64 at a time: the tiles of each, and up to and with it.
+    const int lane = threadIdx.x & 63;
+    const int lines = a.sequences * a.blocks;
+    auto scan = [&](int first) {
+      __syncthreads();
+      if (threadIdx.x < 64) {
+        int mine = 0;
+        if (first + lane < lines) {
+          const int b = (first + lane) / a.blocks;
+          const Sequence seq(a, b);
+          mine = Span(a, seq, first + lane - b * a.blocks, 16 * QT).tiles;
+        }
+        int64_t sum = mine;
+        int me = lane;
+        asm volatile("" : "+v"(me));  // its neighbours' numbers are not kept in registers
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+          const uint32_t low = __builtin_amdgcn_ds_bpermute((me - d) * 4, (int)sum);
+          const uint32_t high = __builtin_amdgcn_ds_bpermute((me - d) * 4, (int)(sum >> 32));
+          if (me >= d) sum += (int64_t)((uint64_t)high << 32 | low);
+        }
+        lds.tiles[lane] = mine;
+        lds.upto[lane] = sum;
+      }
+      __syncthreads();
+    };
+    int64_t total = 0;
+#pragma unroll 1
+    for (int first = (lines - 1) / 64 * 64; first >= 0; first -= 64) {
+      scan(first);
+      total += lds.upto[63];
+    }
+    total = uniform(total) * hk;
+    int64_t range = uniform((total + a.workers - 1) / a.workers);
+    if (range < kMinTiles) range = kMinTiles;
+    const int64_t end = min((blockIdx.x + 1) * range, total);
+    const int64_t begin = uniform((int64_t)(blockIdx.x * range));
+    int base = 0;
+    int64_t before = 0;  // tiles (of one kv head) of the lines before these 64
+    for (int64_t pos = begin; pos < end;) {
+      while (pos >= (before + uniform(lds.upto[63])) * hk) {
+        before += uniform(lds.upto[63]);
+        base += 64;
+        scan(base);
+      }
+      const int at = uniform(__ffsll((long long)__ballot((before + lds.upto[lane]) * hk > pos)) - 1);
+      const int tiles = uniform(lds.tiles[at]);
+      const int64_t line_start = (before + uniform(lds.upto[at]) - tiles) * hk;
+      const int kv = uniform((int)((pos - line_start) / tiles));
+      const int64_t unit = line_start + (int64_t)kv * tiles;
+      const int x0 = uniform((int)(pos - unit));
+      const int x1 = uniform((int)min((int64_t)tiles, end - unit));
+      const bool whole = x0 == 0 && x1 == tiles;
+      const int line = base + at;
+      const int b = uniform(line / a.blocks), block = line - b * a.blocks;
+      if (x0 == 0 && threadIdx.x == 0)
+        a.units[(int64_t)line * hk + kv] =
+            int4{(int)blockIdx.x, (int)((unit + tiles - 1) / range), unit > begin, 0};
+      Sequence seq(a, b);
+      seq.settle();
+      Span span(a, seq, block, 16 * QT);
+      attend<T, QT, W, SCORES>(a, lds, b, block, kv, seq, span, x0, x1, whole,
+                               2 * blockIdx.x + (unit > begin));
+      pos = unit + x1;
+      if (pos < end) __syncthreads();  // the waves' results are read before the next ones come
+    }
+  }
+}
+
+// Parts of units that cross ranges: one workgroup a query row, 32 lanes of 4 columns, every
+// eighth part in turn, added in the order of the ranges.
+template <class T, int QT>
+__global__ __launch_bounds__(256) void cached_join_kernel(CachedAttnArgs a) {
+  __shared__ float4v sums[8][32];
+  const int hk = a.cache.kv_heads;
+  const int line = (int)(blockIdx.x / hk), kv = (int)(blockIdx.x - line * hk);
+  const int b = line / a.blocks, block = line - b * a.blocks;
+  const Sequence seq(a, b);
+  const int row = block * 16 * QT + blockIdx.y;
+  if (row >= min(seq.n, a.max_new) * a.group) return;
+  const int4 unit = a.units[blockIdx.x];
+  if (unit.x == unit.y) return;
+  const int lane = threadIdx.x & 63;
+  auto part = [&](int w) {
+    return (int64_t)(2 * w + (w == unit.x ? unit.z : 0)) * 16 * QT + blockIdx.y;
+  };
+  float top = -INFINITY;
+  for (int w = unit.x + lane; w <= unit.y; w += 64) top = fmaxf(top, a.part_ml[part(w) * 2]);
+  top = wave_max(top);
+  const float base = top == -INFINITY ? 0.f : top;
+  float sum = 0.f;
+  for (int w = unit.x + lane; w <= unit.y; w += 64) {
+    const float* ml = a.part_ml + part(w) * 2;
+    sum += __builtin_amdgcn_exp2f(ml[0] - base) * ml[1];
+  }
+  sum = wave_sum(sum);
+  const int c = threadIdx.x & 31, g = threadIdx.x >> 5;
+  float4v o{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int w = unit.x + g; w <= unit.y; w += 8) {
+    const int64_t p = part(w);
+    const float f = __builtin_amdgcn_exp2f(a.part_ml[p * 2] - base);
+    o += f * *reinterpret_cast<const float4v*>(a.part_o + p * kCacheDim + 4 * c);
+  }
+  sums[g][c] = o;
+  __syncthreads();
+  if (g) return;
+#pragma unroll
+  for (int i = 1; i < 8; ++i) o += sums[i][c];
+  const int i = row / a.group;
+  const int head = kv * a.group + row - i * a.group;
+  T* out = reinterpret_cast<T*>(a.o + (int64_t)(seq.start + i) * a.o_tok + head * a.o_head) + 4 * c;
+  const float inverse = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) out[e] = (T)(sum == 0.f ? 0.f : o[e] * inverse);
+  if (a.lse2 && c == 0)
+    a.lse2[(int64_t)(seq.start + i) * a.hq + head] =
+        sum == 0.f ? INFINITY : base - kLift<T> + log2f(sum);
+}
+
+// Weights of 1024 cache rows of one kv head from the scores, a thread to every 256th.
 __global__ __launch_bounds__(256) void cached_weights_kernel(CachedAttnArgs a) {
   const int64_t cap = (int64_t)a.rows.row_pages * a.cache.page_size;
-  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  if (item >= cap * a.sequences * a.cache.kv_heads) return;
-  const int64_t j = item % cap;
-  const int kv = (int)(item / cap % a.cache.kv_heads);
-  const int b = (int)(item / cap / a.cache.kv_heads);
-  float sum = 0.f;
-  const int64_t entry = j / a.cache.page_size;
-  const int page = a.rows.page(b, entry, a.cache.pages);
-  if (j < a.rows.length(b, a.cache.page_size, a.max_length) && page >= 0) {
-    const char* k = a.cache.k + page * a.cache.k_page + kv * a.cache.k_head +
-                    (j - entry * a.cache.page_size) * a.cache.k_row;
-    const int64_t last = min((int64_t)a.cu[b + 1], a.tokens);
-    for (int64_t t = max(a.cu[b], 0); t < last; ++t) {
-      if (!visible(a, j, (int64_t)a.rows.lengths[b] - a.cu[b + 1] + t)) continue;
-      for (int h = kv * a.group; h < (kv + 1) * a.group; ++h) {
-        const T* q = reinterpret_cast<const T*>(a.q + t * a.q_tok + h * a.q_head) + 2 * lane;
-        sum += exp2f(a.scale_log2 * dot_row<T>(k, lane, (float)q[0], (float)q[1]) -
-                     a.lse2[t * a.hq + h]);
+  const int64_t pieces = cdiv(cap, 1024), unit = blockIdx.x / pieces;
+  const int64_t piece = blockIdx.x - unit * pieces;
+  const int b = (int)(unit / a.cache.kv_heads), kv = (int)(unit - (int64_t)b * a.cache.kv_heads);
+  const Sequence seq(a, b);
+  const int n = min(seq.n, a.max_new);
+  const int64_t line = ((int64_t)b * a.cache.kv_heads + kv) * cap;
+  const float* scores = a.scores + ((int64_t)b * a.cache.kv_heads + kv) * a.score_rows *
+                                       a.score_keys;
+  const int64_t j0 = piece * 1024 + threadIdx.x;
+  float sum[4] = {};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int64_t j = j0 + 256 * e;
+    if (a.w_in && j < cap) sum[e] = a.w_in[line + j];
+  }
+  if (piece * 1024 < seq.len) {
+    for (int i = 0; i < n; ++i) {
+      const int last = seq.last(i), low = seq.low(a, i);
+      bool seen[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int64_t j = j0 + 256 * e;
+        seen[e] = j <= last && (j >= low || j < a.sinks);
+      }
+      for (int g = 0; g < a.group; ++g) {
+        const float lse = a.lse2[(int64_t)(seq.start + i) * a.hq + kv * a.group + g];
+        const float* s = scores + (int64_t)(i * a.group + g) * a.score_keys + j0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (seen[e]) sum[e] += __builtin_amdgcn_exp2f(s[256 * e] - lse);
       }
     }
   }
-  if (lane == 0) a.w_out[item] = (a.w_in ? a.w_in[item] : 0.f) + sum;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int64_t j = j0 + 256 * e;
+    if (j < cap) a.w_out[line + j] = sum[e];
+  }
+}
+
+// Weights by multiplying the keys again: one wave to 32 cache rows of one kv head, all the
+// sequence's query rows in tiles of 16.
+template <class T>
+__global__ __launch_bounds__(256) void cached_weights_again_kernel(CachedAttnArgs a) {
+  const int64_t cap = (int64_t)a.rows.row_pages * a.cache.page_size;
+  const int64_t pieces = cdiv(cap, 4 * kKeys), unit = blockIdx.x / pieces;
+  const int64_t piece = blockIdx.x - unit * pieces;
+  const int b = (int)(unit / a.cache.kv_heads), kv = (int)(unit - (int64_t)b * a.cache.kv_heads);
+  const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6));
+  const int col = lane & 15, grp = lane >> 4;
+  const int64_t first = (piece * 4 + wave) * kKeys;
+  if (first >= cap) return;
+  const Sequence seq(a, b);
+  const int rows = min(seq.n, a.max_new) * a.group;
+  float sum[8] = {};
+  if (first < seq.len && rows > 0) {
+    const int j0 = (int)first, size = a.cache.page_size;
+    Vec8<T> kf[2][4];
+    bool held[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int j = j0 + 16 * u, entry = j / size;
+      const int page = j < seq.len ? a.rows.page(b, entry, a.cache.pages) : -1;
+      held[u] = page >= 0;
+      const char* base = a.cache.k + (int64_t)max(page, 0) * a.cache.k_page +
+                         (int64_t)kv * a.cache.k_head + (int64_t)(j - entry * size) * a.cache.k_row +
+                         (uint32_t)col * (uint32_t)a.cache.k_row + grp * 16;
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks)
+        kf[u][ks] = *reinterpret_cast<const Vec8<T>*>(base + ks * 64);
+    }
+    for (int r0 = 0; r0 < rows; r0 += 16) {
+      const int r = min(r0 + col, rows - 1), i = r / a.group;
+      const int head = kv * a.group + r - i * a.group;
+      const char* p = a.q + (int64_t)(seq.start + i) * a.q_tok + head * a.q_head + grp * 16;
+      const float lse = a.lse2[(int64_t)(seq.start + i) * a.hq + head];
+      const int last = r0 + col < rows ? seq.last(i) : -1, low = seq.low(a, i);
+      Vec8<T> q[4];
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) q[ks] = *reinterpret_cast<const Vec8<T>*>(p + ks * 64);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        float4v c{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) c = mfma(kf[u][ks], q[ks], c);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int j = j0 + 16 * u + 4 * grp + e;
+          const float w = __builtin_amdgcn_exp2f(c[e] * a.scale_log2 - lse);
+          if (held[u] && j <= last && (j >= low || j < a.sinks)) sum[4 * u + e] += w;
+        }
+      }
+    }
+  }
+  // Over the 16 query rows of a lane group; lane col keeps key col / 8, col % 8 of it.
+#pragma unroll
+  for (int d = 1; d < 16; d <<= 1)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum[e] += __shfl_xor(sum[e], d, kWave);
+  if (col < 8) {
+    float mine = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) mine = col == e ? sum[e] : mine;
+    const int64_t j = first + 16 * (col >> 2) + 4 * grp + (col & 3);
+    const int64_t at = ((int64_t)b * a.cache.kv_heads + kv) * cap + j;
+    if (j < cap) a.w_out[at] = (a.w_in ? a.w_in[at] : 0.f) + mine;
+  }
+}
+
+// How a call is laid out, from what the host knows.
+struct Layout {
+  int max_new, qt, blocks, workers;  // workers 0: one workgroup a unit
+  int64_t units;
+  int score_rows;           // 0: no scores kept
+  int64_t score_keys;
+  size_t lse, list, ml, o, scores, bytes;  // workspace offsets
+  Layout(int rows, int64_t tokens, int q_heads, int kv_heads, int new_bound, int64_t max_length,
+         bool weights) {
+    max_new = (int)(new_bound < tokens ? new_bound : tokens);
+    const int64_t block_rows = (int64_t)(max_new > 0 ? max_new : 1) * (q_heads / kv_heads);
+    // 16 query rows a wave as long as a sequence has no more; 64 read the cache a fourth as
+    // often as 16.
+    qt = block_rows <= 16 ? 1 : block_rows <= 32 ? 2 : 4;
+    blocks = (int)cdiv(block_rows, 16 * qt);
+    units = (int64_t)rows * blocks * kv_heads;
+    workers = max_length <= kWhole ? 0 : device_cu_count();
+    score_keys = cdiv(max_length > 0 ? max_length : 1, kKeys) * kKeys;
+    score_rows = 0;
+    if (weights && block_rows <= 32 &&
+        (size_t)rows * kv_heads * block_rows * score_keys * 4 <= kScoreBytes)
+      score_rows = (int)block_rows;
+    bytes = 0;
+    auto take = [&](size_t n) {
+      const size_t at = bytes;
+      bytes += (n + 255) / 256 * 256;
+      return at;
+    };
+    lse = take(weights ? (size_t)tokens * q_heads * 4 : 0);
+    list = take(workers ? (size_t)units * sizeof(int4) : 0);
+    ml = take((size_t)workers * 2 * 16 * qt * 2 * 4);
+    o = take((size_t)workers * 2 * 16 * qt * kCacheDim * 4);
+    scores = take((size_t)rows * kv_heads * score_rows * score_keys * 4);
+  }
+};
+
+constexpr int waves_of(int qt) { return qt == 4 ? 4 : 8; }
+
+template <class T, int QT, bool SCORES>
+int launch_attention(const CachedAttnArgs& a, const Layout& p, hipStream_t st) {
+  constexpr int W = waves_of(QT);
+  if (!p.workers) {
+    hipLaunchKernelGGL((cached_attention_kernel<T, QT, W, false, SCORES>), dim3((unsigned)p.units),
+                       dim3(64 * W), 0, st, a);
+    SS_CHECK_LAUNCH("cached_attention_kernel");
+    return SS_OK;
+  }
+  hipLaunchKernelGGL((cached_attention_kernel<T, QT, W, true, SCORES>), dim3((unsigned)p.workers),
+                     dim3(64 * W), 0, st, a);
+  SS_CHECK_LAUNCH("cached_attention_kernel");
+  const int64_t rows = (int64_t)a.max_new * a.group;
+  hipLaunchKernelGGL((cached_join_kernel<T, QT>),
+                     dim3((unsigned)p.units, (unsigned)(rows < 16 * QT ? rows : 16 * QT)),
+                     dim3(256), 0, st, a);
+  SS_CHECK_LAUNCH("cached_join_kernel");
+  return SS_OK;
 }
 
 template <class T>
-int launch(const CachedAttnArgs& a, hipStream_t st) {
+int launch(const CachedAttnArgs& a, const Layout& p, hipStream_t st) {
   if (a.tokens > 0) {
-    hipLaunchKernelGGL(cached_attention_kernel<T>, dim3((unsigned)(a.tokens * a.hq)), dim3(256), 0,
-                       st, a);
-    SS_CHECK_LAUNCH("cached_attention_kernel");
+    int rc;
+    if (p.qt == 1)
+      rc = p.score_rows ? launch_attention<T, 1, true>(a, p, st)
+                        : launch_attention<T, 1, false>(a, p, st);
+    else if (p.qt == 2)
+      rc = p.score_rows ? launch_attention<T, 2, true>(a, p, st)
+                        : launch_attention<T, 2, false>(a, p, st);
+    else
+      rc = launch_attention<T, 4, false>(a, p, st);
+    if (rc) return rc;
   }
-  if (a.w_out) {
-    const int64_t items =
-        (int64_t)a.rows.row_pages * a.cache.page_size * a.sequences * a.cache.kv_heads;
-    hipLaunchKernelGGL(cached_weights_kernel<T>, dim3((unsigned)cdiv(items, 4)), dim3(256), 0, st,
-                       a);
-    SS_CHECK_LAUNCH("cached_weights_kernel");
-  }
+  if (!a.w_out) return SS_OK;
+  const int64_t cap = (int64_t)a.rows.row_pages * a.cache.page_size;
+  const int64_t units = (int64_t)a.sequences * a.cache.kv_heads;
+  if (p.score_rows || a.tokens == 0)
+    hipLaunchKernelGGL(cached_weights_kernel, dim3((unsigned)(units * cdiv(cap, 1024))),
+                       dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL(cached_weights_again_kernel<T>,
+                       dim3((unsigned)(units * cdiv(cap, 4 * kKeys))), dim3(256), 0, st, a);
+  SS_CHECK_LAUNCH("cached_weights_kernel");
   return SS_OK;
 }
 
@@ -144,8 +800,10 @@ int launch(const CachedAttnArgs& a, hipStream_t st) {
 extern "C" size_t ss_cached_attention_workspace_size(int rows, int64_t tokens, int q_heads,
                                                      int kv_heads, int max_new,
                                                      int64_t max_length, int weights) {
-  if (rows <= 0 || tokens <= 0 || q_heads <= 0 || kv_heads <= 0 || !weights) return 0;
-  return (size_t)tokens * q_heads * sizeof(float);
+  if (rows <= 0 || tokens <= 0 || q_heads <= 0 || kv_heads <= 0 || max_new < 0 ||
+      max_length < 0 || q_heads % kv_heads)
+    return 0;
+  return ss::Layout(rows, tokens, q_heads, kv_heads, max_new, max_length, weights != 0).bytes;
 }
 
 extern "C" int ss_cached_attention(const ss_paged_cache* cache, const void* q, int64_t q_tok,
@@ -169,16 +827,27 @@ extern "C" int ss_cached_attention(const ss_paged_cache* cache, const void* q, i
   SS_CHECK_ARG(cu_seqlens && (tokens == 0 || (q && o)), "%s: null pointer", who);
   SS_CHECK_ARG(aligned16(q) && aligned16(o) && ((q_tok | q_head | o_tok | o_head) & 7) == 0,
                "%s: needs 16-byte aligned bases and strides that are multiples of 8", who);
-  SS_CHECK_ARG(tokens <= (int64_t)INT32_MAX / q_heads, "%s: too many tokens in one call", who);
+  SS_CHECK_ARG(max_new > 0 || tokens == 0, "%s: tokens, but max_new is 0", who);
+  SS_CHECK_ARG(cache->k_row >= 0 && cache->k_row < (1 << 26) && cache->v_row >= 0 &&
+                   cache->v_row < (1 << 26),
+               "%s: cache rows must lie less than 2^26 elements apart", who);
+  const Layout p(rows, tokens, q_heads, cache->kv_heads, max_new, max_length, weights_out != 0);
+  const int64_t cap = (int64_t)row_pages * cache->page_size;
+  SS_CHECK_ARG(tokens <= (int64_t)INT32_MAX / q_heads && p.units <= kMaxGrid / 4 &&
+                   (!weights_out || rows * (int64_t)cache->kv_heads * cdiv(cap, 4 * kKeys) <= kMaxGrid),
+               "%s: too many tokens in one call", who);
   const size_t need = ss_cached_attention_workspace_size(rows, tokens, q_heads, cache->kv_heads,
                                                          max_new, max_length, weights_out != 0);
   SS_CHECK_ARG(need <= workspace_bytes && (need == 0 || (workspace && aligned16(workspace))),
                "%s: workspace of %zu bytes, needs %zu", who, workspace_bytes, need);
+  char* ws = (char*)workspace;
   CachedAttnArgs a{cache_view(cache), TableView{table, table_stride, row_pages, lengths},
                    cu_seqlens, rows, tokens, max_length, (const char*)q, q_tok * 2, q_head * 2,
                    (char*)o, o_tok * 2, o_head * 2, q_heads, q_heads / cache->kv_heads,
                    scale * kLog2e, window, sinks, weights_in, weights_out,
-                   need ? (float*)workspace : nullptr};
+                   weights_out ? (float*)(ws + p.lse) : nullptr, p.max_new, p.blocks, p.workers,
+                   (int4*)(ws + p.list), (float*)(ws + p.ml), (float*)(ws + p.o),
+                   (float*)(ws + p.scores), p.score_rows, p.score_keys};
   const hipStream_t st = (hipStream_t)stream;
-  return cache->dtype == SS_F16 ? launch<half_t>(a, st) : launch<bhalf_t>(a, st);
+  return cache->dtype == SS_F16 ? launch<half_t>(a, p, st) : launch<bhalf_t>(a, p, st);
 }
