@@ -25,7 +25,8 @@
 // that one long sequence and a batch of ragged ones load every CU alike whatever the
 // bounds that the host knows.  A unit inside a range is finished there; of one that
 // crosses ranges each part leaves (o, m, l), and cached_join_kernel adds them up.
-// Bounds on the length up to kWhole give one workgroup a unit and no second launch.
+// Bounds on the length that give a wave at most four tiles take one workgroup a unit and no
+// second launch.
 //
 // Masked rows: a tile that every query row sees whole takes no mask.  In the others scores
 // are replaced (never multiplied) by -inf and the values of rows that no query row sees by
@@ -48,10 +49,11 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kKeys = 32;       // of a tile
 constexpr int kPadDim = kCacheDim + 4;  // fp32 row of the waves' results in LDS
-constexpr int64_t kWhole = 512;
+constexpr int kWholeTiles = 4;  // of a wave
 constexpr size_t kScoreBytes = (size_t)512 << 20;
 constexpr int kSteps = 31;      // tiles of a wave whose pages are looked up at once
 constexpr int kMinTiles = 8;    // of a range
+constexpr int kStart = 8;       // tiles that a unit's start and join take the time of
 constexpr int64_t kMaxGrid = (int64_t)1 << 23;  // workgroups of a launch
 
 struct CachedAttnArgs {
@@ -110,6 +112,25 @@ __device__ __forceinline__ float group_max(float v) {
 __device__ __forceinline__ float group_sum(float v) {
   return over_groups(v, [](float a, float b) { return a + b; });
 }
+// Sums over the lanes up to and with each.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int64_t add_moved(int64_t v) {
+  const uint32_t low = __builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+  const uint32_t high = __builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, ROWS, 0xf, false);
+  return v + (int64_t)((uint64_t)high << 32 | low);
+}
+__device__ __forceinline__ int64_t lanes_upto(int64_t v) {
+  v = add_moved<0x111, 0xf>(v);  // lanes 1, 2, 4, 8 below in the row
+  v = add_moved<0x112, 0xf>(v);
+  v = add_moved<0x114, 0xf>(v);
+  v = add_moved<0x118, 0xf>(v);
+  v = add_moved<0x142, 0xa>(v);  // the last lane of rows 0 and 2 to rows 1 and 3
+  return add_moved<0x143, 0xc>(v);  // and of row 1 to rows 2 and 3
+}
+// a / b of numbers from 0 and 1 up: seldom more than 32 bits.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ int64_t uniform(int64_t v) {
   return (int64_t)((uint64_t)(uint32_t)uniform((int)v) |
@@ -124,6 +145,7 @@ __device__ __forceinline__ int clamp_to(int64_t v, int64_t lo, int64_t hi) {
 struct Sequence {
   int start, n, len;  // first packed token, tokens, cache rows
   int64_t at;         // cache row of the first token
+  Sequence() = default;
   __device__ __forceinline__ Sequence(const CachedAttnArgs& a, int b) {
     const int64_t c0 = clamp_to(a.cu[b], 0, a.tokens), c1 = clamp_to(a.cu[b + 1], 0, a.tokens);
     start = (int)c0;
@@ -176,6 +198,7 @@ struct Shared {
   float m[W][16 * QT], l[W][16 * QT];
   int64_t upto[64];
   int tiles[64];
+  Sequence seq[64];
 };
 
 typedef __amdgpu_buffer_rsrc_t Rsrc;
@@ -467,7 +490,6 @@ template <class T, int QT, int W, bool SPLIT, bool SCORES>
 __global__ __launch_bounds__(64 * W) void cached_attention_kernel(CachedAttnArgs a) {
   __shared__ Shared<T, QT, W> lds;
   const int hk = a.cache.kv_heads;
-  if (blockIdx.x == 0) clear_outside<W>(a);
   if constexpr (!SPLIT) {
     const int line = uniform((int)(blockIdx.x / hk)), kv = (int)(blockIdx.x - line * hk);
     const int b = uniform(line / a.blocks), block = line - b * a.blocks;
@@ -477,29 +499,22 @@ __global__ __launch_bounds__(64 * W) void cached_attention_kernel(CachedAttnArgs
     if (span.tiles)
       attend<T, QT, W, SCORES>(a, lds, b, block, kv, seq, span, 0, span.tiles, true, 0);
   } else {
-    // Lines (sequence, block), 64 at a time: the tiles of each, and up to and with it.
+    // Lines (sequence, block), 64 at a time: the places of each, and up to and with it.
     const int lane = threadIdx.x & 63;
     const int lines = a.sequences * a.blocks;
     auto scan = [&](int first) {
       __syncthreads();
       if (threadIdx.x < 64) {
-        int mine = 0;
+        uint32_t mine = 0;
         if (first + lane < lines) {
           const int b = (first + lane) / a.blocks;
           const Sequence seq(a, b);
           mine = Span(a, seq, first + lane - b * a.blocks, 16 * QT).tiles;
+          lds.seq[lane] = seq;
+          lds.tiles[lane] = mine;
+          if (mine) mine += kStart;
         }
-        int64_t sum = mine;
-        int me = lane;
-        asm volatile("" : "+v"(me));  // its neighbours' numbers are not kept in registers
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-          const uint32_t low = __builtin_amdgcn_ds_bpermute((me - d) * 4, (int)sum);
-          const uint32_t high = __builtin_amdgcn_ds_bpermute((me - d) * 4, (int)(sum >> 32));
-          if (me >= d) sum += (int64_t)((uint64_t)high << 32 | low);
-        }
-        lds.tiles[lane] = mine;
-        lds.upto[lane] = sum;
+        lds.upto[lane] = lanes_upto(mine);
       }
       __syncthreads();
     };
@@ -510,12 +525,12 @@ __global__ __launch_bounds__(64 * W) void cached_attention_kernel(CachedAttnArgs
       total += lds.upto[63];
     }
     total = uniform(total) * hk;
-    int64_t range = uniform((total + a.workers - 1) / a.workers);
-    if (range < kMinTiles) range = kMinTiles;
-    const int64_t end = min((blockIdx.x + 1) * range, total);
+    const int64_t range = max(uniform(quotient(total + a.workers - 1, a.workers)),
+                              (int64_t)(kMinTiles + kStart));
     const int64_t begin = uniform((int64_t)(blockIdx.x * range));
+    const int64_t end = min(begin + range, total);
     int base = 0;
-    int64_t before = 0;  // tiles (of one kv head) of the lines before these 64
+    int64_t before = 0;  // places (of one kv head) of the lines before these 64
     for (int64_t pos = begin; pos < end;) {
       while (pos >= (before + uniform(lds.upto[63])) * hk) {
         before += uniform(lds.upto[63]);
@@ -524,68 +539,72 @@ __global__ __launch_bounds__(64 * W) void cached_attention_kernel(CachedAttnArgs
       }
       const int at = uniform(__ffsll((long long)__ballot((before + lds.upto[lane]) * hk > pos)) - 1);
       const int tiles = uniform(lds.tiles[at]);
-      const int64_t line_start = (before + uniform(lds.upto[at]) - tiles) * hk;
-      const int kv = uniform((int)((pos - line_start) / tiles));
-      const int64_t unit = line_start + (int64_t)kv * tiles;
-      const int x0 = uniform((int)(pos - unit));
-      const int x1 = uniform((int)min((int64_t)tiles, end - unit));
-      const bool whole = x0 == 0 && x1 == tiles;
+      const int64_t line_start = (before + uniform(lds.upto[at]) - tiles - kStart) * hk;
+      const int kv = uniform((int)quotient(pos - line_start, tiles + kStart));
+      const int64_t unit = line_start + (int64_t)kv * (tiles + kStart);
+      const int x0 = max((int)(pos - unit) - kStart, 0);
+      const int x1 = (int)min((int64_t)tiles, end - unit - kStart);
       const int line = base + at;
       const int b = uniform(line / a.blocks), block = line - b * a.blocks;
+      pos = unit + kStart + x1;
+      if (x1 <= x0) break;  // the range ends before the unit's first tile
+      const bool whole = x0 == 0 && x1 == tiles;
       if (x0 == 0 && threadIdx.x == 0)
         a.units[(int64_t)line * hk + kv] =
-            int4{(int)blockIdx.x, (int)((unit + tiles - 1) / range), unit > begin, 0};
-      Sequence seq(a, b);
+            int4{(int)blockIdx.x, (int)quotient(unit + kStart + tiles - 1, range), unit > begin, 0};
+      Sequence seq = lds.seq[at];
       seq.settle();
       Span span(a, seq, block, 16 * QT);
       attend<T, QT, W, SCORES>(a, lds, b, block, kv, seq, span, x0, x1, whole,
                                2 * blockIdx.x + (unit > begin));
-      pos = unit + x1;
       if (pos < end) __syncthreads();  // the waves' results are read before the next ones come
     }
   }
+  if (blockIdx.x == 0) clear_outside<W>(a);
 }
 
-// Parts of units that cross ranges: one workgroup a query row, 32 lanes of 4 columns, every
-// eighth part in turn, added in the order of the ranges.
+// Parts of units that cross ranges: one workgroup a query row, 32 lanes of 4 columns for every
+// eighth part, joined in the order of the ranges.
 template <class T, int QT>
 __global__ __launch_bounds__(256) void cached_join_kernel(CachedAttnArgs a) {
   __shared__ float4v sums[8][32];
+  __shared__ float ml[8][2];
   const int hk = a.cache.kv_heads;
   const int line = (int)(blockIdx.x / hk), kv = (int)(blockIdx.x - line * hk);
   const int b = line / a.blocks, block = line - b * a.blocks;
-  const Sequence seq(a, b);
   const int row = block * 16 * QT + blockIdx.y;
-  if (row >= min(seq.n, a.max_new) * a.group) return;
   const int4 unit = a.units[blockIdx.x];
-  if (unit.x == unit.y) return;
-  const int lane = threadIdx.x & 63;
-  auto part = [&](int w) {
-    return (int64_t)(2 * w + (w == unit.x ? unit.z : 0)) * 16 * QT + blockIdx.y;
-  };
-  float top = -INFINITY;
-  for (int w = unit.x + lane; w <= unit.y; w += 64) top = fmaxf(top, a.part_ml[part(w) * 2]);
-  top = wave_max(top);
-  const float base = top == -INFINITY ? 0.f : top;
-  float sum = 0.f;
-  for (int w = unit.x + lane; w <= unit.y; w += 64) {
-    const float* ml = a.part_ml + part(w) * 2;
-    sum += __builtin_amdgcn_exp2f(ml[0] - base) * ml[1];
-  }
-  sum = wave_sum(sum);
+  const Sequence seq(a, b);
+  if (row >= min(seq.n, a.max_new) * a.group || unit.x == unit.y) return;
   const int c = threadIdx.x & 31, g = threadIdx.x >> 5;
   float4v o{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
 #pragma unroll 4
   for (int w = unit.x + g; w <= unit.y; w += 8) {
-    const int64_t p = part(w);
-    const float f = __builtin_amdgcn_exp2f(a.part_ml[p * 2] - base);
-    o += f * *reinterpret_cast<const float4v*>(a.part_o + p * kCacheDim + 4 * c);
+    const int64_t p = (int64_t)(2 * w + (w == unit.x ? unit.z : 0)) * 16 * QT + blockIdx.y;
+    const float2v s = *reinterpret_cast<const float2v*>(a.part_ml + p * 2);
+    const float4v x = *reinterpret_cast<const float4v*>(a.part_o + p * kCacheDim + 4 * c);
+    const float top = fmaxf(m, s[0]), base = top == -INFINITY ? 0.f : top;
+    const float f = __builtin_amdgcn_exp2f(m - base), h = __builtin_amdgcn_exp2f(s[0] - base);
+    o = o * f + x * h;
+    l = l * f + s[1] * h;
+    m = top;
   }
   sums[g][c] = o;
+  if (c == 0) ml[g][0] = m, ml[g][1] = l;
   __syncthreads();
   if (g) return;
 #pragma unroll
-  for (int i = 1; i < 8; ++i) o += sums[i][c];
+  for (int i = 1; i < 8; ++i) m = fmaxf(m, ml[i][0]);
+  const float base = m == -INFINITY ? 0.f : m;
+  float sum = 0.f;
+  o = float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float f = __builtin_amdgcn_exp2f(ml[i][0] - base);
+    sum += f * ml[i][1];
+    o += f * sums[i][c];
+  }
   const int i = row / a.group;
   const int head = kv * a.group + row - i * a.group;
   T* out = reinterpret_cast<T*>(a.o + (int64_t)(seq.start + i) * a.o_tok + head * a.o_head) + 4 * c;
@@ -709,6 +728,8 @@ __global__ __launch_bounds__(256) void cached_weights_again_kernel(CachedAttnArg
   }
 }
 
+constexpr int waves_of(int qt) { return qt == 4 ? 4 : 8; }
+
 // How a call is laid out, from what the host knows.
 struct Layout {
   int max_new, qt, blocks, workers;  // workers 0: one workgroup a unit
@@ -725,7 +746,7 @@ struct Layout {
     qt = block_rows <= 16 ? 1 : block_rows <= 32 ? 2 : 4;
     blocks = (int)cdiv(block_rows, 16 * qt);
     units = (int64_t)rows * blocks * kv_heads;
-    workers = max_length <= kWhole ? 0 : device_cu_count();
+    workers = max_length <= kWholeTiles * kKeys * waves_of(qt) ? 0 : device_cu_count();
     score_keys = cdiv(max_length > 0 ? max_length : 1, kKeys) * kKeys;
     score_rows = 0;
     if (weights && block_rows <= 32 &&
@@ -744,8 +765,6 @@ struct Layout {
     scores = take((size_t)rows * kv_heads * score_rows * score_keys * 4);
   }
 };
-
-constexpr int waves_of(int qt) { return qt == 4 ? 4 : 8; }
 
 template <class T, int QT, bool SCORES>
 int launch_attention(const CachedAttnArgs& a, const Layout& p, hipStream_t st) {
