@@ -19,7 +19,7 @@ from pathlib import Path
 PACKAGE = Path(__file__).resolve().parent
 CSRC = PACKAGE / "csrc"
 LIBRARY = PACKAGE / "libsoupsuck_amd.so"
-NODES = CSRC / "torch" / "nodes.cpp"    # autograd nodes over the C ABI (host code only)
+NODES = sorted((CSRC / "torch").glob("*.cpp"))  # entry points over the C ABI (host code only)
 NATIVE = PACKAGE / "_native.so"
 ARCH = "gfx950"
 
@@ -46,7 +46,7 @@ def _nodes_command(target):
     for path in [*cpp_extension.include_paths(), "/opt/rocm/include",
                  sysconfig.get_paths()["include"]]:
         command += ["-isystem", path]
-    command += [str(NODES), "-o", str(target)]
+    command += [*map(str, NODES), "-o", str(target)]
     for path in cpp_extension.library_paths():
         command += ["-L" + path]
     return command + ["-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_hip",
@@ -123,7 +123,8 @@ def built_library(address_sanitizer=False):
     if not target.exists() or target.stat().st_mtime < max(p.stat().st_mtime for p in inputs):
         return build(address_sanitizer=address_sanitizer)
     if not address_sanitizer and (not NATIVE.exists()
-                                  or NATIVE.stat().st_mtime < NODES.stat().st_mtime):
+                                  or NATIVE.stat().st_mtime < max(
+                                      p.stat().st_mtime for p in (CSRC / "torch").iterdir())):
         build_nodes()
     return target
 

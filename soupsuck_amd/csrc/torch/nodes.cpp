@@ -12,37 +12,22 @@
 //
 // Everything a node keeps is a tensor (no raw pointer outlives a call); the streams are
 // torch's current ones at the call, which for a backward is its forward's.
-#include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_cpp_function.h>
-#include <torch/extension.h>
 
-#include "soupsuck_amd.h"
+#include "calls.h"
+
+// serving.cpp
+void define_serving(pybind11::module_& m);
 
 namespace {
 
-using at::Tensor;
 // An absent tensor argument of a node (apply() takes no undefined Tensor).
 using OptionalTensor = std::optional<at::Tensor>;
 using torch::autograd::AutogradContext;
 using torch::autograd::Function;
 using torch::autograd::variable_list;
 
-void* stream_of(const Tensor& t) {
-  return c10::hip::getCurrentHIPStream(t.device().index()).stream();
-}
-
-void check(int rc, const char* name) {
-  if (rc == SS_OK) return;
-  const std::string text = ss_last_error();
-  if (rc == SS_ERR_INVALID_ARGUMENT) TORCH_CHECK_VALUE(false, name, ": ", text);
-  TORCH_CHECK(false, name, " failed (", rc, "): ", text);
-}
-
-template <class T>
-T* ptr(const Tensor& t) {
-  return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr;
-}
 uint16_t* half_ptr(const Tensor& t) { return ptr<uint16_t>(t); }
 
 int code_of(at::ScalarType t) {
@@ -51,14 +36,6 @@ int code_of(at::ScalarType t) {
   return t == at::kHalf ? SS_F16 : SS_F32;
 }
 int code_of(const Tensor& t) { return t.defined() ? code_of(t.scalar_type()) : SS_F16; }
-
-Tensor empty(at::IntArrayRef sizes, const Tensor& like, at::ScalarType dtype) {
-  return at::empty(sizes, like.options().dtype(dtype));
-}
-
-Tensor workspace(size_t bytes, const Tensor& like) {
-  return bytes ? empty({(int64_t)bytes}, like, at::kByte) : Tensor();
-}
 
 // Gradients of a node that cannot be differentiated again: as Python's
 // once_differentiable, they fail when a graph through them is used.
@@ -403,4 +380,5 @@ PYBIND11_MODULE(_native, m) {
   m.def("nf4_linear", &nf4_linear, Unlocked());
   m.def("row_norm", &row_norm, Unlocked());
   m.def("qlora", &qlora, Unlocked());
+  define_serving(m);
 }

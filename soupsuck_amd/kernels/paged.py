@@ -25,7 +25,7 @@ import ctypes
 
 import torch
 
-from .. import _lib
+from .. import _lib, native
 from ..contract import Rule, enforce, finite_real
 
 HEAD_DIM = 128
@@ -166,6 +166,12 @@ def append_kv(cache, k, v, block_table, lengths, cu_seqlens, q=None, cos=None, s
     them) k is rotated on its way and ``q`` [T, q_heads, 128] is rotated too: returns the
     rotated q (None without q).  A token whose row the sequence does not hold is skipped.
     """
+    nodes = native.nodes() if _is_cache(cache) else None
+    if nodes is not None:
+        got = nodes.append_kv(cache._pointer, cache._k, k, v, block_table, lengths, cu_seqlens, q,
+                              cos, sin)
+        if got is not None:
+            return got if q is not None else None
     enforce(APPEND_RULES, cache=cache, k=k, v=v, block_table=block_table, lengths=lengths,
             cu_seqlens=cu_seqlens, q=q, cos=cos, sin=sin,
             tensors=(k, v, block_table, lengths, cu_seqlens, q, cos, sin))
@@ -232,6 +238,13 @@ def cached_attention(q, cache, block_table, lengths, cu_seqlens, max_new, max_le
     zeros; may be the same tensor) plus every cache row's attention weight, summed over the new tokens
     and the q heads of its kv head: what ``evict_kv`` ranks by.
     """
+    nodes = native.nodes() if _is_cache(cache) else None
+    if nodes is not None:
+        got = nodes.cached_attention(cache._pointer, cache._k, q, block_table, lengths, cu_seqlens,
+                                     max_new, max_length, scale, window, sinks, weights,
+                                     weights_out)
+        if got is not None:
+            return got
     enforce(ATTENTION_RULES, q=q, cache=cache, block_table=block_table, lengths=lengths,
             cu_seqlens=cu_seqlens, max_new=max_new, max_length=max_length, scale=scale,
             window=window, sinks=sinks, weights=weights, weights_out=weights_out,
@@ -282,6 +295,12 @@ def evict_kv(cache, block_table, lengths, weights, out_table, budget, max_length
     were, so that a shared start serves its other sequences.  Returns the new lengths (int32 [rows]) and weights
     (fp32 [rows, kv_heads, out pages a row * page_size], 0 behind the kept rows).
     """
+    nodes = native.nodes() if _is_cache(cache) else None
+    if nodes is not None:
+        got = nodes.evict_kv(cache._pointer, cache._k, block_table, lengths, weights, out_table,
+                             budget, max_length, sinks, recent)
+        if got is not None:
+            return got
     enforce(EVICT_RULES, cache=cache, block_table=block_table, lengths=lengths, weights=weights,
             out_table=out_table, budget=budget, sinks=sinks, recent=recent, max_length=max_length,
             tensors=(block_table, lengths, weights, out_table))

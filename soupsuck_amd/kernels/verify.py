@@ -7,7 +7,7 @@ call is a function of its arguments; probabilities and running sums are fp64
 
 import torch
 
-from .. import _lib
+from .. import _lib, native
 from ..contract import Rule, enforce, finite_real
 
 _CODES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
@@ -65,6 +65,12 @@ def verify_drafts(target_logits, draft_tokens, uniform=None, draft_logits=None, 
     the first refusal, else from p behind the last draft.  ``temperature`` divides both logits;
     0 compares with the target's largest logit (the lowest token of equal ones).
     """
+    nodes = native.nodes()
+    if nodes is not None:
+        got = nodes.verify_drafts(target_logits, draft_tokens, uniform, draft_logits, draft_counts,
+                                  temperature)
+        if got is not None:
+            return got
     enforce(VERIFY_RULES, target=target_logits, tokens=draft_tokens, uniform=uniform,
             draft=draft_logits, counts=draft_counts, temperature=temperature)
     rows, length, vocab = target_logits.shape
