@@ -7,21 +7,27 @@
 //
 // Probabilities and sums are fp64: a drawn token is the place of one number among up to
 // 151936 running sums, and sums that are off by 1e-7 would name another token once in a
-// hundred draws from a flat distribution.
+// hundred draws from a flat distribution.  The exponential is 2^t = 2^n 2^f, n = rint(t), with
+// a polynomial of degree 8 for 2^f on [-1/2, 1/2] that interpolates at the Chebyshev nodes:
+// off by 1.1e-12 at most, 18 fp64 operations (full rate here) for each logit.
 //
-// Three launches, each logit read once but for the chosen rows:
-//   1. per (row, chunk of 8192 logits): maximum and sum of exp((l - max) / T) (or the
-//      place of the maximum at T = 0);
-//   2. per (sequence, chunk): the decisions, then the chunk's part of the chosen row's
-//      max(p - q, 0) and p;
+// Three launches, each logit read once but for the chosen rows of refused drafts:
+//   1. per (row, chunk of 8192 logits): maximum and sum of 2^((l - max) c), c = log2(e) / T (or
+//      the place of the maximum at T = 0);
+//   2. per (sequence, chunk): the decisions, then the chunk's part of the chosen row's mass;
 //   3. per sequence: the chunk in which the drawn number lies, and the token in it.
+#include <algorithm>
+
 #include "paged.h"
 #include "elementwise.h"
 
 namespace ss {
 namespace {
 
-constexpr int kChunk = 8192;  // logits of a workgroup: 256 threads x 4 groups of 8
+constexpr int kThreads = 512;
+constexpr int kWaves = kThreads / 64;
+constexpr int kGroups = 2;                        // of 8 logits a thread
+constexpr int kChunk = kThreads * 8 * kGroups;    // 8192 logits of a workgroup
 
 struct Stat {  // of a chunk, or of a row
   double sum;  // of weight(l, max)
@@ -30,7 +36,7 @@ struct Stat {  // of a chunk, or of a row
 };
 
 struct Choice {  // of a sequence
-  double p_sum, q_sum;
+  double p_inv, q_inv;    // 1 / sum, 0 where a row has no mass
   float p_max, q_max;
   int accepted, refused;  // refused: a draft was, and q applies
   int drafted;            // the refused token, or -1
@@ -45,12 +51,12 @@ struct VerifyArgs {
   int rows, drafts, chunks;
   int per;  // logit rows of a sequence: drafts + 1 of the target, then the draft's if given
   int64_t vocab;
-  double inv_t;
+  double c;  // log2(e) / T
   int32_t* accepted;
   int64_t* out;
   Stat* stats;      // target [rows][drafts + 1][chunks], then draft [rows][drafts][chunks]
   Choice* choices;  // [rows]
-  double* parts;    // [2][rows][chunks]: max(p - q, 0), p
+  double* parts;    // [rows][chunks]: mass to draw from
 
   __device__ __forceinline__ int count(int b) const {
     return counts ? min(max(counts[b], 0), drafts) : drafts;
@@ -63,11 +69,38 @@ struct VerifyArgs {
   }
 };
 
-// exp((l - top) / T): 1 at the maximum (an infinite one included), 0 where there is none.
-__device__ __forceinline__ double weight(float l, float top, double inv_t) {
-  if (top == -INFINITY) return 0.0;
-  if (l == top) return 1.0;
-  return exp(((double)l - (double)top) * inv_t);
+// 2^t, 0 for t below -1074 and NaN.
+__device__ __forceinline__ double power(double t) {
+  t = __builtin_fmax(t, -1100.0);
+  const double n = __builtin_rint(t), f = t - n;
+  double p = 0x1.63d1363930791p-20;
+  p = __builtin_fma(p, f, 0x1.00dc4a53395d3p-16);
+  p = __builtin_fma(p, f, 0x1.4308ac85a7718p-13);
+  p = __builtin_fma(p, f, 0x1.5d8745a72831bp-10);
+  p = __builtin_fma(p, f, 0x1.3b2ab7181b778p-7);
+  p = __builtin_fma(p, f, 0x1.c6b08dd6fd236p-5);
+  p = __builtin_fma(p, f, 0x1.ebfbdff823cedp-3);
+  p = __builtin_fma(p, f, 0x1.62e42fef84cf0p-1);
+  p = __builtin_fma(p, f, 0x1.0000000000000p+0);
+  return __builtin_ldexp(p, (int)n);
+}
+
+// exp((l - top) / T): 1 at an infinite maximum and 0 below it, 0 where there is none.
+__device__ __forceinline__ double weight(float l, float top, double c) {
+  if (top == INFINITY) return l == top ? 1.0 : 0.0;
+  return power(((double)l - (double)top) * c);
+}
+// The same of several logits; the branch on an infinite maximum is uniform.
+template <int N>
+__device__ __forceinline__ void weights(const float (&l)[N], float top, double c, double (&w)[N]) {
+  const bool infinite = top == INFINITY;
+  const double base = infinite ? 0.0 : (double)top;
+#pragma unroll
+  for (int e = 0; e < N; ++e) w[e] = power(((double)l[e] - base) * c);
+  if (infinite) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) w[e] = l[e] == top ? 1.0 : 0.0;
+  }
 }
 
 template <class T>
@@ -94,21 +127,29 @@ __device__ __forceinline__ double wave_sum_f64(double v) {
   for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, kWave);
   return v;
 }
-
-__device__ __forceinline__ double block_sum(double v, double* lds) {
-  v = wave_sum_f64(v);
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = lds[0] + lds[1] + lds[2] + lds[3];
-  __syncthreads();
+// Sums over the lanes up to and with each.
+__device__ __forceinline__ double wave_upto(double v) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const double other = __shfl_up(v, d, kWave);
+    if (lane >= d) v += other;
+  }
   return v;
 }
 
+// One statistic from the lanes' (those without a part: {0, -inf, INT32_MAX}).
+__device__ __forceinline__ Stat join(Stat s, double c) {
+  const float top = wave_max(s.max);
+  if (s.max != top) s.at = INT32_MAX;
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) s.at = min(s.at, __shfl_xor(s.at, m, kWave));
+  return Stat{wave_sum_f64(s.sum * weight(s.max, top, c)), top, s.at};
+}
+
 template <class T, bool VEC, bool GREEDY>
-__global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs a) {
-  __shared__ float tops[4];
-  __shared__ double sums[4];
-  __shared__ int places[4];
+__global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyArgs a) {
+  __shared__ Stat waves[kWaves];
   const int chunk = blockIdx.x;
   const int b = blockIdx.y / a.per;
   const int i = blockIdx.y - b * a.per;
@@ -117,60 +158,60 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs a) {
   if (is_draft ? i - a.drafts - 1 >= n : i > n) return;
   const char* row = is_draft ? a.draft + b * a.d_seq + (i - a.drafts - 1) * a.d_row
                              : a.target + b * a.t_seq + i * a.t_row;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t j0 = (int64_t)chunk * kChunk + threadIdx.x * 8;
-  float x[4][8];
+  float x[kGroups][8];
 #pragma unroll
-  for (int g = 0; g < 4; ++g) load8<T, VEC>(row, j0 + g * 2048, a.vocab, x[g]);
+  for (int g = 0; g < kGroups; ++g) load8<T, VEC>(row, j0 + g * kThreads * 8, a.vocab, x[g]);
   float top = -INFINITY;
 #pragma unroll
-  for (int g = 0; g < 4; ++g)
+  for (int g = 0; g < kGroups; ++g)
 #pragma unroll
     for (int e = 0; e < 8; ++e) top = fmaxf(top, x[g][e]);
   top = wave_max(top);
-  if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-  Stat s{0.0, top, 0};
+  Stat s{0.0, top, INT32_MAX};
   if (GREEDY) {
-    int at = INT32_MAX;
 #pragma unroll
-    for (int g = 3; g >= 0; --g)
+    for (int g = kGroups - 1; g >= 0; --g)
 #pragma unroll
       for (int e = 7; e >= 0; --e)
-        if (x[g][e] == top) at = (int)(j0 + g * 2048 + e);
+        if (x[g][e] == top) s.at = (int)(j0 + g * kThreads * 8 + e);
 #pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) at = min(at, __shfl_xor(at, m, kWave));
-    if ((threadIdx.x & 63) == 0) places[threadIdx.x >> 6] = at;
-    __syncthreads();
-    s.at = min(min(places[0], places[1]), min(places[2], places[3]));
+    for (int m = 32; m >= 1; m >>= 1) s.at = min(s.at, __shfl_xor(s.at, m, kWave));
   } else {
-    double sum = 0.0;
 #pragma unroll
-    for (int g = 0; g < 4; ++g)
+    for (int g = 0; g < kGroups; ++g) {
+      double w[8];
+      weights(x[g], top, a.c, w);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum += weight(x[g][e], top, a.inv_t);
-    s.sum = block_sum(sum, sums);
+      for (int e = 0; e < 8; ++e) s.sum += w[e];
+    }
+    s.sum = wave_sum_f64(s.sum);
   }
-  if (threadIdx.x == 0)
+  if (lane == 0) waves[wave] = s;
+  __syncthreads();
+  if (wave) return;
+  s = join(lane < kWaves ? waves[lane] : Stat{0.0, -INFINITY, INT32_MAX}, a.c);
+  if (lane == 0)
     (is_draft ? a.draft_stats(b, i - a.drafts - 1) : a.target_stats(b, i))[chunk] = s;
 }
 
 // Statistics of a whole row from its chunks', by one wave.
-__device__ __forceinline__ Stat row_stat(const Stat* chunk, int chunks, double inv_t) {
+__device__ __forceinline__ Stat row_stat(const Stat* chunk, int chunks, double c) {
   const int lane = threadIdx.x & 63;
-  float top = -INFINITY;
-  for (int c = lane; c < chunks; c += 64) top = fmaxf(top, chunk[c].max);
-  top = wave_max(top);
-  double sum = 0.0;
-  int at = INT32_MAX;
-  for (int c = lane; c < chunks; c += 64) {
-    const Stat s = chunk[c];
-    sum += s.sum * weight(s.max, top, inv_t);
-    if (s.max == top) at = min(at, s.at);
+  Stat mine{0.0, -INFINITY, INT32_MAX};
+  for (int i = lane; i < chunks; i += 64) {
+    const Stat s = chunk[i];
+    if (chunks <= 64) {
+      mine = s;
+    } else {
+      const float top = fmaxf(mine.max, s.max);
+      if (s.max > mine.max || (s.max == mine.max && s.at < mine.at)) mine.at = s.at;
+      mine.sum = mine.sum * weight(mine.max, top, c) + s.sum * weight(s.max, top, c);
+      mine.max = top;
+    }
   }
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) at = min(at, __shfl_xor(at, m, kWave));
-  return Stat{wave_sum_f64(sum), top, at};
+  return join(mine, c);
 }
 
 template <class T>
@@ -179,177 +220,201 @@ __device__ __forceinline__ float logit(const char* row, int64_t j) {
   return l == l ? l : -INFINITY;
 }
 
+// Row i of sequence b as the one to draw from, and whether it is: a refused draft, or the
+// row behind the last one.
 template <class T>
-__device__ __forceinline__ bool accepts(const VerifyArgs& a, int b, int i) {
-  const int64_t x = a.tokens[(int64_t)b * a.drafts + i];
-  if (x < 0 || x >= a.vocab) return false;
-  const Stat p = row_stat(a.target_stats(b, i), a.chunks, a.inv_t);
-  const double px = weight(logit<T>(a.target + b * a.t_seq + i * a.t_row, x), p.max, a.inv_t);
-  double qx = 1.0, q_sum = 1.0;
-  if (a.draft) {
-    const Stat q = row_stat(a.draft_stats(b, i), a.chunks, a.inv_t);
-    qx = weight(logit<T>(a.draft + b * a.d_seq + i * a.d_row, x), q.max, a.inv_t);
-    q_sum = q.sum;
+__device__ __forceinline__ bool choose(const VerifyArgs& a, int b, int i, int n, Choice* c) {
+  const int64_t x = i < n ? a.tokens[(int64_t)b * a.drafts + i] : -1;
+  const bool known = x >= 0 && x < a.vocab;
+  const bool drafted = i < n && a.draft;
+  const float pl = known ? logit<T>(a.target + b * a.t_seq + i * a.t_row, x) : -INFINITY;
+  const float ql = known && drafted ? logit<T>(a.draft + b * a.d_seq + i * a.d_row, x) : -INFINITY;
+  const Stat p = row_stat(a.target_stats(b, i), a.chunks, a.c);
+  c->p_inv = p.sum > 0.0 ? 1.0 / p.sum : 0.0;
+  c->p_max = p.max;
+  c->q_inv = 0.0;
+  c->q_max = -INFINITY;
+  c->accepted = i;
+  c->refused = i < n;
+  c->drafted = known ? (int)x : -1;
+  if (drafted) {
+    const Stat q = row_stat(a.draft_stats(b, i), a.chunks, a.c);
+    c->q_inv = q.sum > 0.0 ? 1.0 / q.sum : 0.0;
+    c->q_max = q.max;
   }
-  const double u = a.uniform[(int64_t)b * (a.drafts + 1) + i];
-  return u * (q_sum > 0.0 ? qx / q_sum : 0.0) < (p.sum > 0.0 ? px / p.sum : 0.0);
+  if (i >= n || !known) return true;
+  const double px = weight(pl, c->p_max, a.c) * c->p_inv;
+  const double qx = drafted ? weight(ql, c->q_max, a.c) * c->q_inv : 1.0;
+  return !(a.uniform[(int64_t)b * (a.drafts + 1) + i] * qx < px);
 }
 
-// max(p - q, 0) and p of eight logits of the chosen row.
-struct Mass {
-  double rest[8], p[8];
-};
+// The mass of eight logits of the chosen row: max(p - q, 0) of a refused draft, else (and
+// where that is nothing) p.
 template <class T, bool VEC>
-__device__ __forceinline__ Mass masses(const VerifyArgs& a, const Choice& c, int b, int64_t j) {
-  Mass m;
-  float x[8];
+__device__ __forceinline__ void masses(const VerifyArgs& a, const Choice& c, int b, int64_t j,
+                                       bool plain, double (&m)[8]) {
+  float x[8], y[8];
+  const bool drafted = !plain && a.draft;
   load8<T, VEC>(a.target + b * a.t_seq + c.accepted * a.t_row, j, a.vocab, x);
+  if (drafted) load8<T, VEC>(a.draft + b * a.d_seq + c.accepted * a.d_row, j, a.vocab, y);
+  weights(x, c.p_max, a.c, m);
 #pragma unroll
-  for (int e = 0; e < 8; ++e)
-    m.rest[e] = m.p[e] = c.p_sum > 0.0 ? weight(x[e], c.p_max, a.inv_t) / c.p_sum : 0.0;
-  if (c.refused) {
-    if (a.draft) {
-      load8<T, VEC>(a.draft + b * a.d_seq + c.accepted * a.d_row, j, a.vocab, x);
+  for (int e = 0; e < 8; ++e) m[e] *= c.p_inv;
+  if (drafted) {
+    double q[8];
+    weights(y, c.q_max, a.c, q);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const double q = c.q_sum > 0.0 ? weight(x[e], c.q_max, a.inv_t) / c.q_sum : 0.0;
-        m.rest[e] = fmax(m.p[e] - q, 0.0);
-      }
-    } else {
+    for (int e = 0; e < 8; ++e) m[e] = fmax(m[e] - q[e] * c.q_inv, 0.0);
+  } else if (!plain) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (j + e == c.drafted) m.rest[e] = 0.0;
-    }
+    for (int e = 0; e < 8; ++e)
+      if (j + e == c.drafted) m[e] = 0.0;
   }
-  return m;
+}
+
+// A chunk's part of p, from its statistics.
+__device__ __forceinline__ double plain_part(const VerifyArgs& a, const Choice& c, int b,
+                                             int chunk) {
+  const Stat s = a.target_stats(b, c.accepted)[chunk];
+  return s.sum * weight(s.max, c.p_max, a.c) * c.p_inv;
 }
 
 template <class T, bool VEC>
-__global__ __launch_bounds__(256) void verify_rest_kernel(VerifyArgs a) {
-  __shared__ int first;
-  __shared__ Choice choice;
-  __shared__ double sums[4];
+__global__ __launch_bounds__(kThreads) void verify_rest_kernel(VerifyArgs a) {
+  __shared__ Choice choices[kWaves];
+  __shared__ double sums[kWaves];
   const int chunk = blockIdx.x, b = blockIdx.y;
-  const int wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int n = a.count(b);
-  if (threadIdx.x == 0) first = n;
-  __syncthreads();
-  for (int i = wave; i < n; i += 4) {
-    if (!accepts<T>(a, b, i)) {
-      if ((threadIdx.x & 63) == 0) atomicMin(&first, i);
+  // Every wave looks at its rows up to its first choice; the lowest of theirs is the one.
+  Choice mine{};
+  mine.accepted = INT32_MAX;
+  for (int i = wave; i <= n; i += kWaves) {
+    Choice c;
+    if (choose<T>(a, b, i, n, &c)) {
+      mine = c;
       break;
     }
   }
+  if (lane == 0) choices[wave] = mine;
   __syncthreads();
-  if (wave == 0) {
-    Choice c;
-    c.accepted = first;
-    c.refused = first < n;
-    const Stat p = row_stat(a.target_stats(b, first), a.chunks, a.inv_t);
-    c.p_sum = p.sum;
-    c.p_max = p.max;
-    c.q_sum = 0.0;
-    c.q_max = -INFINITY;
-    c.drafted = -1;
-    if (c.refused) {
-      const int64_t x = a.tokens[(int64_t)b * a.drafts + first];
-      if (x >= 0 && x < a.vocab) c.drafted = (int)x;
-      if (a.draft) {
-        const Stat q = row_stat(a.draft_stats(b, first), a.chunks, a.inv_t);
-        c.q_sum = q.sum;
-        c.q_max = q.max;
-      }
-    }
-    if (threadIdx.x == 0) {
-      choice = c;
-      if (chunk == 0) a.choices[b] = c;
-    }
-  }
-  __syncthreads();
-  const Choice c = choice;
-  double rest = 0.0, p = 0.0;
-  const int64_t j0 = (int64_t)chunk * kChunk + threadIdx.x * 8;
-  for (int g = 0; g < 4; ++g) {
-    const Mass m = masses<T, VEC>(a, c, b, j0 + g * 2048);
+  int first = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      rest += m.rest[e];
-      p += m.p[e];
-    }
+  for (int w = 1; w < kWaves; ++w)
+    if (choices[w].accepted < choices[first].accepted) first = w;
+  const Choice c = choices[first];
+  if (chunk == 0 && threadIdx.x == 0) a.choices[b] = c;
+  double* part = a.parts + (int64_t)b * a.chunks + chunk;
+  if (!c.refused) {
+    if (threadIdx.x == 0) *part = plain_part(a, c, b, chunk);
+    return;
   }
-  rest = block_sum(rest, sums);
-  p = block_sum(p, sums);
-  if (threadIdx.x == 0) {
-    a.parts[(int64_t)b * a.chunks + chunk] = rest;
-    a.parts[(int64_t)(a.rows + b) * a.chunks + chunk] = p;
+  double sum = 0.0;
+  const int64_t j0 = (int64_t)chunk * kChunk + threadIdx.x * 8;
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) {
+    double m[8];
+    masses<T, VEC>(a, c, b, j0 + g * kThreads * 8, false, m);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum += m[e];
   }
+  sum = wave_sum_f64(sum);
+  if (lane == 0) sums[wave] = sum;
+  __syncthreads();
+  if (threadIdx.x) return;
+  sum = 0.0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) sum += sums[w];
+  *part = sum;
 }
 
 template <class T, bool VEC>
-__global__ __launch_bounds__(256) void verify_pick_kernel(VerifyArgs a) {
-  __shared__ double scan[256];
-  __shared__ int64_t drawn, last;
+__global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a) {
+  __shared__ double sums[kWaves];
+  __shared__ int hits[kWaves], lasts[kWaves];
   const int b = blockIdx.x;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const Choice c = a.choices[b];
-  const double* rest = a.parts + (int64_t)b * a.chunks;
-  const double* whole = a.parts + (int64_t)(a.rows + b) * a.chunks;
-  double total = 0.0;
-  for (int i = 0; i < a.chunks; ++i) total += rest[i];
-  const bool use_p = !(total > 0.0);
-  if (use_p) {
-    total = 0.0;
-    for (int i = 0; i < a.chunks; ++i) total += whole[i];
+  const double* parts = a.parts + (int64_t)b * a.chunks;
+  bool plain = !c.refused;
+  auto part = [&](int i) {
+    return i >= a.chunks ? 0.0 : plain && c.refused ? plain_part(a, c, b, i) : parts[i];
+  };
+  auto whole = [&] {
+    double v = 0.0;
+    for (int i = lane; i < a.chunks; i += 64) v += part(i);
+    return wave_sum_f64(v);
+  };
+  double total = whole();
+  if (!(total > 0.0) && c.refused) {
+    plain = true;
+    total = whole();
   }
-  const double* part = use_p ? whole : rest;
   const double goal = (double)a.uniform[(int64_t)b * (a.drafts + 1) + a.drafts] * total;
   // The first chunk whose running sum exceeds the goal, or the last one that holds any.
   int chunk = -1;
-  double sum = 0.0, ahead = 0.0;
-  for (int i = 0; i < a.chunks; ++i) {
-    if (part[i] > 0.0) {
-      chunk = i;
-      ahead = sum;
-      if (sum + part[i] > goal) break;
+  double ahead = 0.0, sum = 0.0;
+  bool found = false;
+  for (int i = 0; i < a.chunks && !found; i += 64) {
+    const double v = part(i + lane);
+    const double upto = sum + wave_upto(v);
+    double below = __shfl_up(upto, 1, kWave);
+    if (lane == 0) below = sum;
+    const uint64_t over = __ballot(v > 0.0 && upto > goal), any = __ballot(v > 0.0);
+    found = over != 0;
+    if (any) {
+      const int at = found ? __ffsll((long long)over) - 1 : 63 - __clzll((long long)any);
+      chunk = i + at;
+      ahead = __shfl(below, at, kWave);
     }
-    sum += part[i];
+    sum = __shfl(upto, 63, kWave);
   }
-  if (threadIdx.x == 0) drawn = INT64_MAX, last = -1;
   int64_t token = -1;
   if (chunk >= 0) {
-    const int64_t j0 = (int64_t)chunk * kChunk + threadIdx.x * 32;
-    double mine = 0.0;
-    double m[32];
+    const int64_t j0 = (int64_t)chunk * kChunk + threadIdx.x * 8 * kGroups;
+    double m[kGroups][8], mine = 0.0;
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const Mass q = masses<T, VEC>(a, c, b, j0 + g * 8);
+    for (int g = 0; g < kGroups; ++g) {
+      masses<T, VEC>(a, c, b, j0 + g * 8, plain, m[g]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        m[g * 8 + e] = use_p ? q.p[e] : q.rest[e];
-        mine += m[g * 8 + e];
-      }
+      for (int e = 0; e < 8; ++e) mine += m[g][e];
     }
-    scan[threadIdx.x] = mine;
+    double upto = wave_upto(mine);
+    double start = __shfl_up(upto, 1, kWave);
+    if (lane == 0) start = 0.0;
+    if (lane == 63) sums[wave] = upto;
     __syncthreads();
-    double start = ahead;
-    for (int i = 0; i < (int)threadIdx.x; ++i) start += scan[i];
+    for (int w = 0; w < wave; ++w) ahead += sums[w];
+    start += ahead;
     // Place of the first running sum above the goal, and of the last logit with any mass
     // (taken where rounding leaves the chunk's own sum at or below the goal).
-    int64_t hit = INT64_MAX, any = -1;
+    int hit = INT32_MAX, any = -1;
 #pragma unroll
-    for (int e = 0; e < 32; ++e) {
-      start += m[e];
-      if (m[e] > 0.0) {
-        any = j0 + e;
-        if (start > goal && hit == INT64_MAX) hit = j0 + e;
+    for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        start += m[g][e];
+        if (m[g][e] > 0.0) {
+          any = (int)(j0 + g * 8 + e);
+          if (start > goal) hit = min(hit, any);
+        }
       }
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) {
+      hit = min(hit, __shfl_xor(hit, d, kWave));
+      any = max(any, __shfl_xor(any, d, kWave));
     }
-    atomicMin((long long*)&drawn, (long long)hit);
-    atomicMax((long long*)&last, (long long)any);
+    if (lane == 0) hits[wave] = hit, lasts[wave] = any;
     __syncthreads();
-    token = drawn != INT64_MAX ? drawn : last;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      hit = min(hit, hits[w]);
+      any = max(any, lasts[w]);
+    }
+    token = hit != INT32_MAX ? hit : any;
   }
   int64_t* out = a.out + (int64_t)b * (a.drafts + 1);
-  for (int i = threadIdx.x; i <= a.drafts; i += 256)
+  for (int i = threadIdx.x; i <= a.drafts; i += kThreads)
     out[i] = i < c.accepted ? a.tokens[(int64_t)b * a.drafts + i] : i == c.accepted ? token : -1;
   if (threadIdx.x == 0) a.accepted[b] = c.accepted;
 }
@@ -372,7 +437,7 @@ __global__ __launch_bounds__(64) void verify_greedy_kernel(VerifyArgs a) {
 
 template <class T, bool VEC>
 int launch(const VerifyArgs& a, bool greedy, hipStream_t st) {
-  const dim3 block(256);
+  const dim3 block(kThreads);
   const dim3 grid((unsigned)a.chunks, (unsigned)a.rows * a.per);
   if (greedy) {
     hipLaunchKernelGGL((verify_stats_kernel<T, VEC, true>), grid, block, 0, st, a);
@@ -408,7 +473,7 @@ extern "C" size_t ss_verify_drafts_workspace_size(int rows, int drafts, int64_t 
   if (rows <= 0 || drafts < 0 || vocab <= 0) return 0;
   const size_t chunks = (size_t)cdiv(vocab, kChunk);
   return (size_t)rows * ((2 * (size_t)drafts + 1) * chunks * sizeof(Stat) + sizeof(Choice) +
-                         2 * chunks * sizeof(double));
+                         chunks * sizeof(double));
 }
 
 extern "C" int ss_verify_drafts(const void* target, int64_t t_seq, int64_t t_row,
@@ -439,12 +504,14 @@ extern "C" int ss_verify_drafts(const void* target, int64_t t_seq, int64_t t_row
   const int chunks = (int)cdiv(vocab, kChunk);
   VerifyArgs a{(const char*)target, t_seq * size, t_row * size,
                greedy ? nullptr : (const char*)draft, d_seq * size, d_row * size, tokens, counts,
-               uniform, rows, drafts, chunks, drafts + 1, vocab, greedy ? 1.0 : 1.0 / temperature, accepted,
+               uniform, rows, drafts, chunks, drafts + 1, vocab,
+               // a finite number, or the maximum's own 0 times it is none
+               greedy ? 1.0 : std::min(1.4426950408889634 / temperature, 1e300), accepted,
                out, (Stat*)workspace, nullptr, nullptr};
   if (a.draft) a.per += drafts;
   else a.d_seq = a.d_row = 0;
   a.parts = (double*)(a.stats + (int64_t)rows * (2 * drafts + 1) * chunks);
-  a.choices = (Choice*)(a.parts + 2 * (int64_t)rows * chunks);
+  a.choices = (Choice*)(a.parts + (int64_t)rows * chunks);
   const hipStream_t st = (hipStream_t)stream;
   if (dtype == SS_F16) return launch<half_t>(a, greedy, st);
   if (dtype == SS_BF16) return launch<bhalf_t>(a, greedy, st);
