@@ -5,11 +5,14 @@
 // heaviest, equal weights from the lowest row up.
 //
 // Selection (one workgroup of 16 waves per (sequence, kv head)): the m-th largest weight
-// by its bits, 8 at a time from the top: a histogram of the digit among the rows that
-// agree with the digits found so far, then the bin that holds the m-th.  Counts are whole
-// numbers, so LDS atomics give the same result in any order.  Then each wave counts the
+// by its bits, 11 at a time from the top: a histogram of the digit among the rows that
+// agree with the digits found so far, then the bin that holds the m-th, found by one wave
+// (32 bins a lane, then the lane's own 32).  Counts are whole numbers, so LDS atomics give
+// the same result in any order.  Then each wave counts the
 // rows above and at the threshold in its part, a scan over the waves gives its first
-// place, and a second walk over its part writes the kept rows' numbers in order.
+// place, and a second walk over its part writes the kept rows' numbers in order.  The five
+// walks are latency (a serial search of 256 bins had taken 28 us of 37): up to kStaged rows
+// they read keys that the first one left in LDS.
 // Copy: 16 lanes a kept row, 16 bytes of k and of v each, HBM-bound.
 #include "paged.h"
 
@@ -17,6 +20,8 @@ namespace ss {
 namespace {
 
 constexpr int kWaves = 16;
+constexpr int kBins = 2048;
+constexpr int kStaged = 16384;  // rows whose keys LDS holds (64 KiB)
 
 struct EvictArgs {
   CacheView cache;
@@ -40,9 +45,47 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+// Sums over the lanes up to and with each.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int add_moved(int v) {
+  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ int lanes_upto(int v) {
+  v = add_moved<0x111, 0xf>(v);  // lanes 1, 2, 4, 8 below in the row
+  v = add_moved<0x112, 0xf>(v);
+  v = add_moved<0x114, 0xf>(v);
+  v = add_moved<0x118, 0xf>(v);
+  v = add_moved<0x142, 0xa>(v);  // the last lane of rows 0 and 2 to rows 1 and 3
+  return add_moved<0x143, 0xc>(v);  // and of row 1 to rows 2 and 3
+}
+
+struct Digit {
+  int bin, above;  // the need-th row from the top lies in this bin, with so many in higher ones
+};
+// By one wave: lane l takes the 32 bins below bin 2048 - 32 l, then those of the lane that
+// the row lies in.
+__device__ __forceinline__ Digit find_digit(const uint32_t* bins, int need) {
+  const int lane = threadIdx.x & 63;
+  int sum = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const u32x4 v = reinterpret_cast<const u32x4*>(bins)[(63 - lane) * 8 + i];
+    sum += (int)(v[0] + v[1] + v[2] + v[3]);
+  }
+  const int upto = lanes_upto(sum);
+  const int at = __ffsll((long long)__ballot(upto >= need)) - 1;
+  const int before = __builtin_amdgcn_readlane(upto - sum, at);
+  const int bin = (63 - at) * 32 + 31 - (lane & 31);
+  const int mine = lane < 32 ? (int)bins[bin] : 0;
+  const int inside = before + lanes_upto(mine);
+  const int hit = __ffsll((long long)__ballot(inside >= need)) - 1;
+  return Digit{__builtin_amdgcn_readlane(bin, hit), __builtin_amdgcn_readlane(inside - mine, hit)};
+}
+
 __global__ __launch_bounds__(kWaves * 64) void kv_select_kernel(EvictArgs a) {
-  __shared__ uint32_t bins[256];
-  __shared__ uint32_t found[2];  // digit, rows above it
+  __shared__ __attribute__((aligned(16))) uint32_t bins[kBins];
+  __shared__ uint32_t keys[kStaged];
+  __shared__ Digit found;
   __shared__ int counts[2][kWaves];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int head = blockIdx.x % a.cache.kv_heads;
@@ -59,44 +102,50 @@ __global__ __launch_bounds__(kWaves * 64) void kv_select_kernel(EvictArgs a) {
   const int lo = (int)a.sinks, hi = len - (int)a.recent;
   const int want = keep - lo - (len - hi);
   const float* w = a.w + (int64_t)blockIdx.x * a.rows.row_pages * a.cache.page_size;
+  const bool staged = hi - lo <= kStaged;
+  auto key_of = [&](int j) { return staged ? keys[j - lo] : weight_key(w[j]); };
   uint32_t threshold = 0;
   int need = want;  // of the rows that agree with the digits found
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = threadIdx.x; i < 256; i += kWaves * 64) bins[i] = 0;
-    __syncthreads();
-    const uint32_t mask = shift == 24 ? 0u : ~0u << (shift + 8);
-    for (int j = lo + threadIdx.x; j < hi; j += kWaves * 64) {
-      const uint32_t key = weight_key(w[j]);
-      if ((key & mask) == threshold) atomicAdd(&bins[(key >> shift) & 255], 1u);
+  if (want == 0) {
+    threshold = 0xFFFFFFFFu;  // no key is larger, and none at it is needed
+  } else {
+    // Digits of 11, 11 and 10 bits.
+#pragma unroll
+    for (int shift = 21; shift >= 0; shift -= shift == 21 ? 11 : 10) {
+      for (int i = threadIdx.x; i < kBins; i += kWaves * 64) bins[i] = 0;
+      __syncthreads();
+      const uint32_t mask = shift == 21 ? 0u : ~0u << (shift == 10 ? 21 : 10);
+      const uint32_t digit = shift == 0 ? 1023u : 2047u;
+      for (int j = lo + threadIdx.x; j < hi; j += kWaves * 64) {
+        uint32_t key;
+        if (shift == 21) {
+          key = weight_key(w[j]);
+          if (staged) keys[j - lo] = key;
+        } else {
+          key = key_of(j);
+        }
+        if ((key & mask) == threshold) atomicAdd(&bins[(key >> shift) & digit], 1u);
+      }
+      __syncthreads();
+      if (wave == 0) {
+        const Digit d = find_digit(bins, need);
+        if (lane == 0) found = d;
+      }
+      __syncthreads();
+      threshold |= (uint32_t)found.bin << shift;
+      need -= found.above;
     }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      uint32_t above = 0;
-      int d = 255;
-      while (d > 0 && above + bins[d] < (uint32_t)need) above += bins[d--];
-      found[0] = d;
-      found[1] = above;
-    }
-    __syncthreads();
-    threshold |= found[0] << shift;
-    need -= (int)found[1];
-    __syncthreads();
   }
-  // Rows above the threshold, and the first `need` at it (none with want 0, where the
-  // threshold is the largest key there can be).
+  // Rows above the threshold, and the first `need` at it.
   const int span = (int)cdiv(cdiv(hi - lo, kWaves), 64) * 64;
   const int from = lo + wave * span, to = min(hi, from + span);
   int above = 0, equal = 0;
-  for (int j = from + lane; j < to; j += 64) {
-    const uint32_t key = weight_key(w[j]);
-    above += key > threshold;
-    equal += key == threshold;
-  }
-#pragma unroll
-  for (int s = 32; s; s >>= 1) {
-    above += __shfl_xor(above, s);
-    equal += __shfl_xor(equal, s);
-  }
+  if (want > 0)
+    for (int j0 = from; j0 < to; j0 += 64) {
+      const uint32_t key = j0 + lane < to ? key_of(j0 + lane) : 0;
+      above += __popcll(__ballot(j0 + lane < to && key > threshold));
+      equal += __popcll(__ballot(j0 + lane < to && key == threshold));
+    }
   if (lane == 0) counts[0][wave] = above, counts[1][wave] = equal;
   __syncthreads();
   int above_before = 0, equal_before = 0;
@@ -105,17 +154,18 @@ __global__ __launch_bounds__(kWaves * 64) void kv_select_kernel(EvictArgs a) {
     equal_before += counts[1][i];
   }
   const uint64_t below = (1ull << lane) - 1;
-  for (int j0 = from; j0 < to; j0 += 64) {
-    const int j = j0 + lane;
-    const uint32_t key = j < to ? weight_key(w[j]) : 0;
-    const uint64_t gt = __ballot(j < to && key > threshold);
-    const uint64_t eq = __ballot(j < to && key == threshold);
-    const int ga = above_before + __popcll(gt & below), ea = equal_before + __popcll(eq & below);
-    if (j < to && (key > threshold || (key == threshold && ea < need)))
-      kept[lo + ga + min(ea, need)] = j;
-    above_before += __popcll(gt);
-    equal_before += __popcll(eq);
-  }
+  if (want > 0)
+    for (int j0 = from; j0 < to; j0 += 64) {
+      const int j = j0 + lane;
+      const uint32_t key = j < to ? key_of(j) : 0;
+      const uint64_t gt = __ballot(j < to && key > threshold);
+      const uint64_t eq = __ballot(j < to && key == threshold);
+      const int ga = above_before + __popcll(gt & below), ea = equal_before + __popcll(eq & below);
+      if (j < to && (key > threshold || (key == threshold && ea < need)))
+        kept[lo + ga + min(ea, need)] = j;
+      above_before += __popcll(gt);
+      equal_before += __popcll(eq);
+    }
   for (int j = threadIdx.x; j < lo; j += kWaves * 64) kept[j] = j;
   for (int j = threadIdx.x; j < len - hi; j += kWaves * 64) kept[lo + want + j] = hi + j;
 }

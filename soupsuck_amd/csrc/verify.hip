@@ -24,10 +24,16 @@
 namespace ss {
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kWaves = kThreads / 64;
-constexpr int kGroups = 2;                        // of 8 logits a thread
-constexpr int kChunk = kThreads * 8 * kGroups;    // 8192 logits of a workgroup
+constexpr int kChunk = 8192;  // logits of a workgroup
+// Threads of it, and groups of 8 logits that each takes: long parts where every row is
+// summed (the reductions of a workgroup cost as much as 8 logits a thread), short ones where
+// the chosen row is what a sequence waits for.
+template <int THREADS>
+struct Work {
+  static constexpr int kThreads = THREADS, kWaves = THREADS / 64, kGroups = kChunk / 8 / THREADS;
+};
+using Sum = Work<256>;
+using Pick = Work<512>;
 
 struct Stat {  // of a chunk, or of a row
   double sum;  // of weight(l, max)
@@ -106,7 +112,8 @@ __device__ __forceinline__ void weights(const float (&l)[N], float top, double c
 template <class T>
 using Vec8 = T __attribute__((ext_vector_type(8)));
 
-// Logits j .. j + 7 of a row; NaN and what lies behind the row's end are -inf.
+// Logits j .. j + 7 of a row; what lies behind the row's end is -inf, and a NaN counts as that:
+// it is no maximum, and its power is 0.
 template <class T, bool VEC>
 __device__ __forceinline__ void load8(const char* row, int64_t j, int64_t vocab, float (&x)[8]) {
   const T* p = reinterpret_cast<const T*>(row) + j;
@@ -118,38 +125,67 @@ __device__ __forceinline__ void load8(const char* row, int64_t j, int64_t vocab,
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = j + e < vocab ? (float)p[e] : -INFINITY;
   }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = x[e] == x[e] ? x[e] : -INFINITY;
 }
 
-__device__ __forceinline__ double wave_sum_f64(double v) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, kWave);
-  return v;
-}
-// Sums over the lanes up to and with each.
-__device__ __forceinline__ double wave_upto(double v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const double other = __shfl_up(v, d, kWave);
-    if (lane >= d) v += other;
+// f over the lanes up to and with each, in registers.
+template <class V, int CTRL, int ROWS, class F>
+__device__ __forceinline__ V moved(V v, V none, F f) {
+  V other;
+  if constexpr (sizeof(V) == 4) {
+    other = __builtin_bit_cast(
+        V, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, none), __builtin_bit_cast(int, v),
+                                       CTRL, ROWS, 0xf, false));
+  } else {
+    const uint64_t n = __builtin_bit_cast(uint64_t, none), u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t low =
+        __builtin_amdgcn_update_dpp((int)n, (int)u, CTRL, ROWS, 0xf, false);
+    const uint32_t high =
+        __builtin_amdgcn_update_dpp((int)(n >> 32), (int)(u >> 32), CTRL, ROWS, 0xf, false);
+    other = __builtin_bit_cast(V, (uint64_t)high << 32 | low);
   }
-  return v;
+  return f(v, other);
+}
+template <class V, class F>
+__device__ __forceinline__ V upto(V v, V none, F f) {
+  v = moved<V, 0x111, 0xf>(v, none, f);  // lanes 1, 2, 4, 8 below in the row
+  v = moved<V, 0x112, 0xf>(v, none, f);
+  v = moved<V, 0x114, 0xf>(v, none, f);
+  v = moved<V, 0x118, 0xf>(v, none, f);
+  v = moved<V, 0x142, 0xa>(v, none, f);  // the last lane of rows 0 and 2 to rows 1 and 3
+  return moved<V, 0x143, 0xc>(v, none, f);  // and of row 1 to rows 2 and 3
+}
+template <class V>
+__device__ __forceinline__ V lane_of(V v, int lane) {
+  if constexpr (sizeof(V) == 4) {
+    return __builtin_bit_cast(V, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+  } else {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t low = __builtin_amdgcn_readlane((int)u, lane);
+    const uint32_t high = __builtin_amdgcn_readlane((int)(u >> 32), lane);
+    return __builtin_bit_cast(V, (uint64_t)high << 32 | low);
+  }
+}
+__device__ __forceinline__ double wave_upto(double v) {
+  return upto(v, 0.0, [](double x, double y) { return x + y; });
+}
+__device__ __forceinline__ double wave_sum_f64(double v) { return lane_of(wave_upto(v), 63); }
+__device__ __forceinline__ float wave_top(float v) {
+  return lane_of(upto(v, -INFINITY, [](float x, float y) { return fmaxf(x, y); }), 63);
+}
+__device__ __forceinline__ int wave_least(int v) {
+  return lane_of(upto(v, INT32_MAX, [](int x, int y) { return min(x, y); }), 63);
 }
 
 // One statistic from the lanes' (those without a part: {0, -inf, INT32_MAX}).
 __device__ __forceinline__ Stat join(Stat s, double c) {
-  const float top = wave_max(s.max);
-  if (s.max != top) s.at = INT32_MAX;
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) s.at = min(s.at, __shfl_xor(s.at, m, kWave));
-  return Stat{wave_sum_f64(s.sum * weight(s.max, top, c)), top, s.at};
+  const float top = wave_top(s.max);
+  return Stat{wave_sum_f64(s.sum * weight(s.max, top, c)), top,
+              wave_least(s.max == top ? s.at : INT32_MAX)};
 }
 
 template <class T, bool VEC, bool GREEDY>
-__global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyArgs a) {
-  __shared__ Stat waves[kWaves];
+__global__ __launch_bounds__(Sum::kThreads) void verify_stats_kernel(VerifyArgs a) {
+  __shared__ Stat waves[Sum::kWaves];
   const int chunk = blockIdx.x;
   const int b = blockIdx.y / a.per;
   const int i = blockIdx.y - b * a.per;
@@ -160,27 +196,26 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyArgs a) {
                              : a.target + b * a.t_seq + i * a.t_row;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t j0 = (int64_t)chunk * kChunk + threadIdx.x * 8;
-  float x[kGroups][8];
+  float x[Sum::kGroups][8];
 #pragma unroll
-  for (int g = 0; g < kGroups; ++g) load8<T, VEC>(row, j0 + g * kThreads * 8, a.vocab, x[g]);
+  for (int g = 0; g < Sum::kGroups; ++g) load8<T, VEC>(row, j0 + g * Sum::kThreads * 8, a.vocab, x[g]);
   float top = -INFINITY;
 #pragma unroll
-  for (int g = 0; g < kGroups; ++g)
+  for (int g = 0; g < Sum::kGroups; ++g)
 #pragma unroll
     for (int e = 0; e < 8; ++e) top = fmaxf(top, x[g][e]);
-  top = wave_max(top);
+  top = wave_top(top);
   Stat s{0.0, top, INT32_MAX};
   if (GREEDY) {
 #pragma unroll
-    for (int g = kGroups - 1; g >= 0; --g)
+    for (int g = Sum::kGroups - 1; g >= 0; --g)
 #pragma unroll
       for (int e = 7; e >= 0; --e)
-        if (x[g][e] == top) s.at = (int)(j0 + g * kThreads * 8 + e);
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) s.at = min(s.at, __shfl_xor(s.at, m, kWave));
+        if (x[g][e] == top) s.at = (int)(j0 + g * Sum::kThreads * 8 + e);
+    s.at = wave_least(s.at);
   } else {
 #pragma unroll
-    for (int g = 0; g < kGroups; ++g) {
+    for (int g = 0; g < Sum::kGroups; ++g) {
       double w[8];
       weights(x[g], top, a.c, w);
 #pragma unroll
@@ -191,7 +226,7 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyArgs a) {
   if (lane == 0) waves[wave] = s;
   __syncthreads();
   if (wave) return;
-  s = join(lane < kWaves ? waves[lane] : Stat{0.0, -INFINITY, INT32_MAX}, a.c);
+  s = join(lane < Sum::kWaves ? waves[lane] : Stat{0.0, -INFINITY, INT32_MAX}, a.c);
   if (lane == 0)
     (is_draft ? a.draft_stats(b, i - a.drafts - 1) : a.target_stats(b, i))[chunk] = s;
 }
@@ -280,16 +315,16 @@ __device__ __forceinline__ double plain_part(const VerifyArgs& a, const Choice& 
 }
 
 template <class T, bool VEC>
-__global__ __launch_bounds__(kThreads) void verify_rest_kernel(VerifyArgs a) {
-  __shared__ Choice choices[kWaves];
-  __shared__ double sums[kWaves];
+__global__ __launch_bounds__(Pick::kThreads) void verify_rest_kernel(VerifyArgs a) {
+  __shared__ Choice choices[Pick::kWaves];
+  __shared__ double sums[Pick::kWaves];
   const int chunk = blockIdx.x, b = blockIdx.y;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int n = a.count(b);
   // Every wave looks at its rows up to its first choice; the lowest of theirs is the one.
   Choice mine{};
   mine.accepted = INT32_MAX;
-  for (int i = wave; i <= n; i += kWaves) {
+  for (int i = wave; i <= n; i += Pick::kWaves) {
     Choice c;
     if (choose<T>(a, b, i, n, &c)) {
       mine = c;
@@ -300,7 +335,7 @@ __global__ __launch_bounds__(kThreads) void verify_rest_kernel(VerifyArgs a) {
   __syncthreads();
   int first = 0;
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w)
+  for (int w = 1; w < Pick::kWaves; ++w)
     if (choices[w].accepted < choices[first].accepted) first = w;
   const Choice c = choices[first];
   if (chunk == 0 && threadIdx.x == 0) a.choices[b] = c;
@@ -312,9 +347,9 @@ __global__ __launch_bounds__(kThreads) void verify_rest_kernel(VerifyArgs a) {
   double sum = 0.0;
   const int64_t j0 = (int64_t)chunk * kChunk + threadIdx.x * 8;
 #pragma unroll
-  for (int g = 0; g < kGroups; ++g) {
+  for (int g = 0; g < Pick::kGroups; ++g) {
     double m[8];
-    masses<T, VEC>(a, c, b, j0 + g * kThreads * 8, false, m);
+    masses<T, VEC>(a, c, b, j0 + g * Pick::kThreads * 8, false, m);
 #pragma unroll
     for (int e = 0; e < 8; ++e) sum += m[e];
   }
@@ -324,14 +359,14 @@ __global__ __launch_bounds__(kThreads) void verify_rest_kernel(VerifyArgs a) {
   if (threadIdx.x) return;
   sum = 0.0;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) sum += sums[w];
+  for (int w = 0; w < Pick::kWaves; ++w) sum += sums[w];
   *part = sum;
 }
 
 template <class T, bool VEC>
-__global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a) {
-  __shared__ double sums[kWaves];
-  __shared__ int hits[kWaves], lasts[kWaves];
+__global__ __launch_bounds__(Pick::kThreads) void verify_pick_kernel(VerifyArgs a) {
+  __shared__ double sums[Pick::kWaves];
+  __shared__ int hits[Pick::kWaves], lasts[Pick::kWaves];
   const int b = blockIdx.x;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const Choice c = a.choices[b];
@@ -365,16 +400,16 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a) {
     if (any) {
       const int at = found ? __ffsll((long long)over) - 1 : 63 - __clzll((long long)any);
       chunk = i + at;
-      ahead = __shfl(below, at, kWave);
+      ahead = lane_of(below, at);
     }
-    sum = __shfl(upto, 63, kWave);
+    sum = lane_of(upto, 63);
   }
   int64_t token = -1;
   if (chunk >= 0) {
-    const int64_t j0 = (int64_t)chunk * kChunk + threadIdx.x * 8 * kGroups;
-    double m[kGroups][8], mine = 0.0;
+    const int64_t j0 = (int64_t)chunk * kChunk + threadIdx.x * 8 * Pick::kGroups;
+    double m[Pick::kGroups][8], mine = 0.0;
 #pragma unroll
-    for (int g = 0; g < kGroups; ++g) {
+    for (int g = 0; g < Pick::kGroups; ++g) {
       masses<T, VEC>(a, c, b, j0 + g * 8, plain, m[g]);
 #pragma unroll
       for (int e = 0; e < 8; ++e) mine += m[g][e];
@@ -390,7 +425,7 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a) {
     // (taken where rounding leaves the chunk's own sum at or below the goal).
     int hit = INT32_MAX, any = -1;
 #pragma unroll
-    for (int g = 0; g < kGroups; ++g)
+    for (int g = 0; g < Pick::kGroups; ++g)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         start += m[g][e];
@@ -399,22 +434,19 @@ __global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyArgs a) {
           if (start > goal) hit = min(hit, any);
         }
       }
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) {
-      hit = min(hit, __shfl_xor(hit, d, kWave));
-      any = max(any, __shfl_xor(any, d, kWave));
-    }
+    hit = wave_least(hit);
+    any = -wave_least(-any);
     if (lane == 0) hits[wave] = hit, lasts[wave] = any;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < Pick::kWaves; ++w) {
       hit = min(hit, hits[w]);
       any = max(any, lasts[w]);
     }
     token = hit != INT32_MAX ? hit : any;
   }
   int64_t* out = a.out + (int64_t)b * (a.drafts + 1);
-  for (int i = threadIdx.x; i <= a.drafts; i += kThreads)
+  for (int i = threadIdx.x; i <= a.drafts; i += Pick::kThreads)
     out[i] = i < c.accepted ? a.tokens[(int64_t)b * a.drafts + i] : i == c.accepted ? token : -1;
   if (threadIdx.x == 0) a.accepted[b] = c.accepted;
 }
@@ -437,7 +469,7 @@ __global__ __launch_bounds__(64) void verify_greedy_kernel(VerifyArgs a) {
 
 template <class T, bool VEC>
 int launch(const VerifyArgs& a, bool greedy, hipStream_t st) {
-  const dim3 block(kThreads);
+  const dim3 block(Sum::kThreads), pick(Pick::kThreads);
   const dim3 grid((unsigned)a.chunks, (unsigned)a.rows * a.per);
   if (greedy) {
     hipLaunchKernelGGL((verify_stats_kernel<T, VEC, true>), grid, block, 0, st, a);
@@ -449,9 +481,9 @@ int launch(const VerifyArgs& a, bool greedy, hipStream_t st) {
   hipLaunchKernelGGL((verify_stats_kernel<T, VEC, false>), grid, block, 0, st, a);
   SS_CHECK_LAUNCH("verify_stats_kernel");
   hipLaunchKernelGGL((verify_rest_kernel<T, VEC>), dim3((unsigned)a.chunks, (unsigned)a.rows),
-                     block, 0, st, a);
+                     pick, 0, st, a);
   SS_CHECK_LAUNCH("verify_rest_kernel");
-  hipLaunchKernelGGL((verify_pick_kernel<T, VEC>), dim3((unsigned)a.rows), block, 0, st, a);
+  hipLaunchKernelGGL((verify_pick_kernel<T, VEC>), dim3((unsigned)a.rows), pick, 0, st, a);
   SS_CHECK_LAUNCH("verify_pick_kernel");
   return SS_OK;
 }
