@@ -192,7 +192,7 @@ struct Span {
   }
 };
 
-template <class T, int QT, int W>
+template <class T, int QT, int W, int RW>
 struct Shared {
   float o[W][16 * QT][kPadDim];
   float m[W][16 * QT], l[W][16 * QT];
@@ -217,8 +217,8 @@ __device__ __forceinline__ u32x4 load16(Rsrc r, uint32_t lane, uint32_t all) {
 
 // The tiles [x0, x1) of a unit by the waves of the workgroup, and their join: the result
 // where the range is the whole unit, a partial one in the workspace elsewhere.
-template <class T, int QT, int W, bool SCORES>
-__device__ __forceinline__ void attend(const CachedAttnArgs& a, Shared<T, QT, W>& lds, int b,
+template <class T, int QT, int W, int RW, bool SCORES>
+__device__ __forceinline__ void attend(const CachedAttnArgs& a, Shared<T, QT, W, RW>& lds, int b,
                                        int block, int kv, const Sequence& seq, const Span& span,
                                        int x0, int x1, bool whole, int slot) {
   // Opaque, or all that follows from them is computed ahead of the segments' loop and kept
@@ -229,7 +229,11 @@ __device__ __forceinline__ void attend(const CachedAttnArgs& a, Shared<T, QT, W>
   const int col = lane & 15, grp = lane >> 4;
   const int size = a.cache.page_size;
   const int rows = min(seq.n, a.max_new) * a.group;
-  const int r0 = block * 16 * QT;
+  const int block_row = block * 16 * QT * RW;
+  const int r0 = block_row + wave % RW * 16 * QT;
+  const int stripe = wave / RW;
+  constexpr int kStripes = W / RW;
+  const int x_end = r0 < rows ? x1 : x0;  // the waves behind the last row have nothing
 
   Vec8<T> q[QT][4];  // Q[row][32 ks + 8 grp ..]
   int last[QT], low[QT];
@@ -273,11 +277,11 @@ __device__ __forceinline__ void attend(const CachedAttnArgs& a, Shared<T, QT, W>
     // Some of this wave's tiles at a time: their halves' pages in one load, the last two
     // lanes' none.
 #pragma unroll 1
-    for (int x = x0 + wave; x < x1; x += kSteps * W) {
-      const int steps = uniform(min((x1 - x + W - 1) / W, kSteps));
+    for (int x = x0 + stripe; x < x_end; x += kSteps * kStripes) {
+      const int steps = uniform(min((x_end - x + kStripes - 1) / kStripes, kSteps));
       int page = -1, row = 0;
       {
-        const int j = span.tile(x + (lane >> 1) * W) * kKeys + (lane & 1) * 16;
+        const int j = span.tile(x + (lane >> 1) * kStripes) * kKeys + (lane & 1) * 16;
         if ((lane >> 1) < steps && j < seq.len) {
           const int entry = j / size;
           page = a.rows.page(b, entry, a.cache.pages);
@@ -310,7 +314,7 @@ __device__ __forceinline__ void attend(const CachedAttnArgs& a, Shared<T, QT, W>
       load_v(0);
 #pragma unroll 1
       for (int s = 0; s < steps; ++s) {
-        const int j0 = span.tile(x + s * W) * kKeys;
+        const int j0 = span.tile(x + s * kStripes) * kKeys;
         const bool held0 = __builtin_amdgcn_readlane(page, 2 * s) >= 0;
         const bool held1 = __builtin_amdgcn_readlane(page, 2 * s + 1) >= 0;
         float sc[QT][8];
@@ -420,16 +424,17 @@ __device__ __forceinline__ void attend(const CachedAttnArgs& a, Shared<T, QT, W>
   }
   __syncthreads();
 
-  for (int item = thread; item < 16 * QT * 16; item += 64 * W) {
-    const int r = item >> 4, c = (item & 15) * 8;
-    if (r0 + r >= rows) continue;
+  for (int item = thread; item < 16 * QT * RW * 16; item += 64 * W) {
+    const int line = item >> 4, c = (item & 15) * 8;
+    if (block_row + line >= rows) continue;
+    const int half = line / (16 * QT), r = line % (16 * QT);
     float top = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < W; ++w) top = fmaxf(top, lds.m[w][r]);
+    for (int w = half; w < W; w += RW) top = fmaxf(top, lds.m[w][r]);
     const float base = top == -INFINITY ? 0.f : top;
     float sum = 0.f, o[8] = {};
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
+    for (int w = half; w < W; w += RW) {
       const float f = __builtin_amdgcn_exp2f(lds.m[w][r] - base);
       sum += f * lds.l[w][r];
       const float4v x = *reinterpret_cast<const float4v*>(&lds.o[w][r][c]);
@@ -441,8 +446,8 @@ __device__ __forceinline__ void attend(const CachedAttnArgs& a, Shared<T, QT, W>
       }
     }
     if (whole) {
-      const int i = (r0 + r) / a.group;
-      const int head = kv * a.group + r0 + r - i * a.group;
+      const int i = (block_row + line) / a.group;
+      const int head = kv * a.group + block_row + line - i * a.group;
       const float inverse = sum == 0.f ? 0.f : 1.f / sum;
       Vec8<T> out;
 #pragma unroll
@@ -453,7 +458,7 @@ __device__ __forceinline__ void attend(const CachedAttnArgs& a, Shared<T, QT, W>
         a.lse2[(int64_t)(seq.start + i) * a.hq + head] =
             sum == 0.f ? INFINITY : base - kLift<T> + log2f(sum);
     } else {
-      const int64_t part = (int64_t)slot * 16 * QT + r;
+      const int64_t part = (int64_t)slot * 16 * QT * RW + line;
       float* out = a.part_o + part * kCacheDim + c;
       *reinterpret_cast<float4v*>(out) = float4v{o[0], o[1], o[2], o[3]};
       *reinterpret_cast<float4v*>(out + 4) = float4v{o[4], o[5], o[6], o[7]};
@@ -486,18 +491,18 @@ __device__ __forceinline__ void clear_outside(const CachedAttnArgs& a) {
   }
 }
 
-template <class T, int QT, int W, bool SPLIT, bool SCORES>
+template <class T, int QT, int W, int RW, bool SPLIT, bool SCORES>
 __global__ __launch_bounds__(64 * W) void cached_attention_kernel(CachedAttnArgs a) {
-  __shared__ Shared<T, QT, W> lds;
+  __shared__ Shared<T, QT, W, RW> lds;
   const int hk = a.cache.kv_heads;
   if constexpr (!SPLIT) {
     const int line = uniform((int)(blockIdx.x / hk)), kv = (int)(blockIdx.x - line * hk);
     const int b = uniform(line / a.blocks), block = line - b * a.blocks;
     Sequence seq(a, b);
     seq.settle();
-    const Span span(a, seq, block, 16 * QT);
+    const Span span(a, seq, block, 16 * QT * RW);
     if (span.tiles)
-      attend<T, QT, W, SCORES>(a, lds, b, block, kv, seq, span, 0, span.tiles, true, 0);
+      attend<T, QT, W, RW, SCORES>(a, lds, b, block, kv, seq, span, 0, span.tiles, true, 0);
   } else {
     // Lines (sequence, block), 64 at a time: the places of each, and up to and with it.
     const int lane = threadIdx.x & 63;
@@ -509,7 +514,7 @@ __global__ __launch_bounds__(64 * W) void cached_attention_kernel(CachedAttnArgs
         if (first + lane < lines) {
           const int b = (first + lane) / a.blocks;
           const Sequence seq(a, b);
-          mine = Span(a, seq, first + lane - b * a.blocks, 16 * QT).tiles;
+          mine = Span(a, seq, first + lane - b * a.blocks, 16 * QT * RW).tiles;
           lds.seq[lane] = seq;
           lds.tiles[lane] = mine;
           if (mine) mine += kStart;
@@ -554,8 +559,8 @@ __global__ __launch_bounds__(64 * W) void cached_attention_kernel(CachedAttnArgs
             int4{(int)blockIdx.x, (int)quotient(unit + kStart + tiles - 1, range), unit > begin, 0};
       Sequence seq = lds.seq[at];
       seq.settle();
-      Span span(a, seq, block, 16 * QT);
-      attend<T, QT, W, SCORES>(a, lds, b, block, kv, seq, span, x0, x1, whole,
+      Span span(a, seq, block, 16 * QT * RW);
+      attend<T, QT, W, RW, SCORES>(a, lds, b, block, kv, seq, span, x0, x1, whole,
                                2 * blockIdx.x + (unit > begin));
       if (pos < end) __syncthreads();  // the waves' results are read before the next ones come
     }
@@ -565,14 +570,14 @@ __global__ __launch_bounds__(64 * W) void cached_attention_kernel(CachedAttnArgs
 
 // Parts of units that cross ranges: one workgroup a query row, 32 lanes of 4 columns for every
 // eighth part, joined in the order of the ranges.
-template <class T, int QT>
+template <class T, int ROWS>
 __global__ __launch_bounds__(256) void cached_join_kernel(CachedAttnArgs a) {
   __shared__ float4v sums[8][32];
   __shared__ float ml[8][2];
   const int hk = a.cache.kv_heads;
   const int line = (int)(blockIdx.x / hk), kv = (int)(blockIdx.x - line * hk);
   const int b = line / a.blocks, block = line - b * a.blocks;
-  const int row = block * 16 * QT + blockIdx.y;
+  const int row = block * ROWS + blockIdx.y;
   const int4 unit = a.units[blockIdx.x];
   const Sequence seq(a, b);
   if (row >= min(seq.n, a.max_new) * a.group || unit.x == unit.y) return;
@@ -581,7 +586,7 @@ __global__ __launch_bounds__(256) void cached_join_kernel(CachedAttnArgs a) {
   float m = -INFINITY, l = 0.f;
 #pragma unroll 4
   for (int w = unit.x + g; w <= unit.y; w += 8) {
-    const int64_t p = (int64_t)(2 * w + (w == unit.x ? unit.z : 0)) * 16 * QT + blockIdx.y;
+    const int64_t p = (int64_t)(2 * w + (w == unit.x ? unit.z : 0)) * ROWS + blockIdx.y;
     const float2v s = *reinterpret_cast<const float2v*>(a.part_ml + p * 2);
     const float4v x = *reinterpret_cast<const float4v*>(a.part_o + p * kCacheDim + 4 * c);
     const float top = fmaxf(m, s[0]), base = top == -INFINITY ? 0.f : top;
@@ -728,11 +733,13 @@ __global__ __launch_bounds__(256) void cached_weights_again_kernel(CachedAttnArg
   }
 }
 
-constexpr int waves_of(int qt) { return qt == 4 ? 4 : 8; }
+// Waves of a workgroup side by side on the query rows of a block: one as long as a sequence
+// has at most 32.
+constexpr int kWaves = 8;
 
 // How a call is laid out, from what the host knows.
 struct Layout {
-  int max_new, qt, blocks, workers;  // workers 0: one workgroup a unit
+  int max_new, block_rows, blocks, workers;  // query rows of a block; workers 0: one workgroup a unit
   int64_t units;
   int score_rows;           // 0: no scores kept
   int64_t score_keys;
@@ -740,18 +747,17 @@ struct Layout {
   Layout(int rows, int64_t tokens, int q_heads, int kv_heads, int new_bound, int64_t max_length,
          bool weights) {
     max_new = (int)(new_bound < tokens ? new_bound : tokens);
-    const int64_t block_rows = (int64_t)(max_new > 0 ? max_new : 1) * (q_heads / kv_heads);
-    // 16 query rows a wave as long as a sequence has no more; 64 read the cache a fourth as
-    // often as 16.
-    qt = block_rows <= 16 ? 1 : block_rows <= 32 ? 2 : 4;
-    blocks = (int)cdiv(block_rows, 16 * qt);
+    const int64_t of_sequence = (int64_t)(max_new > 0 ? max_new : 1) * (q_heads / kv_heads);
+    block_rows = of_sequence <= 16 ? 16 : of_sequence <= 32 ? 32 : of_sequence <= 64 ? 64 : 128;
+    blocks = (int)cdiv(of_sequence, block_rows);
     units = (int64_t)rows * blocks * kv_heads;
-    workers = max_length <= kWholeTiles * kKeys * waves_of(qt) ? 0 : device_cu_count();
+    const int stripes = kWaves / (block_rows <= 32 ? 1 : block_rows / 32);
+    workers = max_length <= kWholeTiles * kKeys * stripes ? 0 : device_cu_count();
     score_keys = cdiv(max_length > 0 ? max_length : 1, kKeys) * kKeys;
     score_rows = 0;
-    if (weights && block_rows <= 32 &&
-        (size_t)rows * kv_heads * block_rows * score_keys * 4 <= kScoreBytes)
-      score_rows = (int)block_rows;
+    if (weights && of_sequence <= 32 &&
+        (size_t)rows * kv_heads * of_sequence * score_keys * 4 <= kScoreBytes)
+      score_rows = (int)of_sequence;
     bytes = 0;
     auto take = [&](size_t n) {
       const size_t at = bytes;
@@ -760,44 +766,47 @@ struct Layout {
     };
     lse = take(weights ? (size_t)tokens * q_heads * 4 : 0);
     list = take(workers ? (size_t)units * sizeof(int4) : 0);
-    ml = take((size_t)workers * 2 * 16 * qt * 2 * 4);
-    o = take((size_t)workers * 2 * 16 * qt * kCacheDim * 4);
+    ml = take((size_t)workers * 2 * block_rows * 2 * 4);
+    o = take((size_t)workers * 2 * block_rows * kCacheDim * 4);
     scores = take((size_t)rows * kv_heads * score_rows * score_keys * 4);
   }
 };
 
-template <class T, int QT, bool SCORES>
+template <class T, int QT, int RW, bool SCORES>
 int launch_attention(const CachedAttnArgs& a, const Layout& p, hipStream_t st) {
-  constexpr int W = waves_of(QT);
+  const dim3 block(64 * kWaves);
   if (!p.workers) {
-    hipLaunchKernelGGL((cached_attention_kernel<T, QT, W, false, SCORES>), dim3((unsigned)p.units),
-                       dim3(64 * W), 0, st, a);
+    hipLaunchKernelGGL((cached_attention_kernel<T, QT, kWaves, RW, false, SCORES>),
+                       dim3((unsigned)p.units), block, 0, st, a);
     SS_CHECK_LAUNCH("cached_attention_kernel");
     return SS_OK;
   }
-  hipLaunchKernelGGL((cached_attention_kernel<T, QT, W, true, SCORES>), dim3((unsigned)p.workers),
-                     dim3(64 * W), 0, st, a);
+  hipLaunchKernelGGL((cached_attention_kernel<T, QT, kWaves, RW, true, SCORES>),
+                     dim3((unsigned)p.workers), block, 0, st, a);
   SS_CHECK_LAUNCH("cached_attention_kernel");
   const int64_t rows = (int64_t)a.max_new * a.group;
-  hipLaunchKernelGGL((cached_join_kernel<T, QT>),
-                     dim3((unsigned)p.units, (unsigned)(rows < 16 * QT ? rows : 16 * QT)),
+  hipLaunchKernelGGL((cached_join_kernel<T, 16 * QT * RW>),
+                     dim3((unsigned)p.units, (unsigned)(rows < p.block_rows ? rows : p.block_rows)),
                      dim3(256), 0, st, a);
   SS_CHECK_LAUNCH("cached_join_kernel");
   return SS_OK;
 }
 
+template <class T, bool SCORES>
+int launch_attention(const CachedAttnArgs& a, const Layout& p, hipStream_t st) {
+  if (p.block_rows == 16) return launch_attention<T, 1, 1, SCORES>(a, p, st);
+  if (p.block_rows == 32) return launch_attention<T, 2, 1, SCORES>(a, p, st);
+  if constexpr (SCORES) return SS_ERR_UNSUPPORTED;  // more rows keep none
+  else
+    return p.block_rows == 64 ? launch_attention<T, 2, 2, false>(a, p, st)
+                              : launch_attention<T, 2, 4, false>(a, p, st);
+}
+
 template <class T>
 int launch(const CachedAttnArgs& a, const Layout& p, hipStream_t st) {
   if (a.tokens > 0) {
-    int rc;
-    if (p.qt == 1)
-      rc = p.score_rows ? launch_attention<T, 1, true>(a, p, st)
-                        : launch_attention<T, 1, false>(a, p, st);
-    else if (p.qt == 2)
-      rc = p.score_rows ? launch_attention<T, 2, true>(a, p, st)
-                        : launch_attention<T, 2, false>(a, p, st);
-    else
-      rc = launch_attention<T, 4, false>(a, p, st);
+    const int rc = p.score_rows ? launch_attention<T, true>(a, p, st)
+                                : launch_attention<T, false>(a, p, st);
     if (rc) return rc;
   }
   if (!a.w_out) return SS_OK;
