@@ -249,6 +249,17 @@ __device__ __forceinline__ void attend(const CachedAttnArgs& a, Shared<T, QT, W,
     last[t] = seq.last(token);
     low[t] = seq.low(a, token);
   }
+  // The maximum and the masks want a positive scale: a negative one changes the queries' sign
+  // (exact), a zero one makes them zeros.
+  float scale = a.scale_log2;
+  if (!(scale > 0.f) && scale == scale) {
+    const T sign = scale < 0.f ? (T)-1.f : (T)0.f;
+#pragma unroll
+    for (int t = 0; t < QT; ++t)
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) q[t][ks] *= sign;
+    scale = scale < 0.f ? -scale : 1.f;
+  }
   const int sinks = clamp_to(a.sinks, 0, seq.len);
   // Tiles that every row of the block sees whole.
   const int clear_end = seq.last(span.i0) + 1, clear_low = seq.low(a, span.i1);
@@ -326,7 +337,7 @@ __device__ __forceinline__ void attend(const CachedAttnArgs& a, Shared<T, QT, W,
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) c = mfma(kf[u][ks], q[t][ks], c);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sc[t][4 * u + i] = c[i] * a.scale_log2;
+            for (int i = 0; i < 4; ++i) sc[t][4 * u + i] = c[i];
           }
         // Not before the products: their operands' registers take the next keys.
         __builtin_amdgcn_sched_barrier(0);
@@ -355,7 +366,8 @@ __device__ __forceinline__ void attend(const CachedAttnArgs& a, Shared<T, QT, W,
 #pragma unroll
               for (int u = 0; u < 2; ++u)
                 *reinterpret_cast<float4v*>(out + 16 * u) =
-                    float4v{sc[t][4 * u], sc[t][4 * u + 1], sc[t][4 * u + 2], sc[t][4 * u + 3]};
+                    scale * float4v{sc[t][4 * u], sc[t][4 * u + 1], sc[t][4 * u + 2],
+                                    sc[t][4 * u + 3]};
             }
         }
         Vec8<T> p[QT];
@@ -365,17 +377,18 @@ __device__ __forceinline__ void attend(const CachedAttnArgs& a, Shared<T, QT, W,
 #pragma unroll
           for (int i = 1; i < 8; ++i) top = fmaxf(top, sc[t][i]);
           top = fmaxf(m[t], group_max(top));
-          const float base = top == -INFINITY ? 0.f : top;
+          const float base = top == -INFINITY ? 0.f : top * scale;
           if (__any(top > m[t])) {
-            const float keep = __builtin_amdgcn_exp2f(m[t] - base);
+            const float keep = __builtin_amdgcn_exp2f(m[t] * scale - base);
             l[t] *= keep;
 #pragma unroll
             for (int e = 0; e < 8; ++e) acc[t][e] *= keep;
             m[t] = top;
           }
+          const float lower = base - kLift<T>;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const float w = __builtin_amdgcn_exp2f(sc[t][i] - base + kLift<T>);
+            const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][i], scale, -lower));
             l[t] += w;
             p[t][i] = (T)w;
           }
@@ -401,7 +414,7 @@ __device__ __forceinline__ void attend(const CachedAttnArgs& a, Shared<T, QT, W,
       const float sum = group_sum(l[t]);
       if (only < 0 || token_of(t) == only) {
         const int r = 16 * t + col;
-        if (grp == 0) lds.m[wave][r] = m[t], lds.l[wave][r] = sum;
+        if (grp == 0) lds.m[wave][r] = m[t] * scale, lds.l[wave][r] = sum;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
