@@ -30,14 +30,15 @@
 //
 // Masked rows: a tile that every query row sees whole takes no mask.  In the others scores
 // are replaced (never multiplied) by -inf and the values of rows that no query row sees by
-// 0, so that nothing stored there counts.  A row that some tokens of the block see and
-// others do not keeps its value, and an infinity or NaN in it would reach the others as 0
-// times it: a wave that ends with one such in o repeats its tiles token by token.
+// 0, so that nothing stored there counts.  In a row that some tokens of a wave see and others
+// do not an infinity or NaN would reach the others as 0 times it: such values are taken as 0
+// there, and added at the end to the rows that see them.
 //
 // Weights: the scores (fp32, base 2) are left in the workspace, 4 bytes a query row and
 // key against 256 for the key again, and added up once the statistics are known; where
 // they would be many (more than 32 query rows a kv head, or more than kScoreBytes in all)
 // the keys are multiplied again.
+#include <algorithm>
 #include <type_traits>
 
 #include "paged.h"
@@ -48,6 +49,7 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kKeys = 32;       // of a tile
+constexpr int kRowBytes = kCacheDim * 2;
 constexpr int kPadDim = kCacheDim + 4;  // fp32 row of the waves' results in LDS
 constexpr int kWholeTiles = 4;  // of a wave
 constexpr size_t kScoreBytes = (size_t)512 << 20;
@@ -172,29 +174,49 @@ struct Span {
   int i0, i1;     // tokens of the block
   int low, high;  // rows [low, high) and the sinks below low
   int sink_tiles, first, tiles;
+  int clear_low, clear_end, sinks;  // what every row of the block sees: [clear_low, clear_end), sinks
   __device__ __forceinline__ Span(const CachedAttnArgs& a, const Sequence& s, int block,
                                   int block_rows) {
     const int rows = min(s.n, a.max_new) * a.group;
     const int r0 = block * block_rows;
     i0 = r0 / a.group;
     i1 = (min(rows, r0 + block_rows) - 1) / a.group;
-    tiles = low = high = sink_tiles = first = 0;
+    tiles = low = high = sink_tiles = first = clear_low = clear_end = 0;
+    sinks = clamp_to(a.sinks, 0, s.len);
     if (r0 >= rows) return;
     high = s.last(i1) + 1;
+    clear_end = s.last(i0) + 1;
+    clear_low = s.low(a, i1);
     low = min(s.low(a, i0), high);
     sink_tiles = (clamp_to(a.sinks, 0, low) + kKeys - 1) / kKeys;
     first = max(low / kKeys, sink_tiles);
     // a block that sees nothing still has its zeros to write
     tiles = max(sink_tiles + max((high + kKeys - 1) / kKeys - first, 0), 1);
   }
+  // Whether every row sees the whole tile from row j on.
+  __device__ __forceinline__ bool clear(int j) const {
+    return j + kKeys <= clear_end && (j >= clear_low || j + kKeys <= sinks);
+  }
   __device__ __forceinline__ int tile(int x) const {
     return x < sink_tiles ? x : x - sink_tiles + first;
   }
 };
 
+// The kernel's arguments, loaded where they are used and not kept in registers until then.
+typedef const __attribute__((address_space(4))) CachedAttnArgs LateArgs;
+__device__ __forceinline__ LateArgs* late_args() {
+  auto p = (LateArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return p;
+}
+
 template <class T, int QT, int W, int RW>
 struct Shared {
-  float o[W][16 * QT][kPadDim];
+  // A wave's keys while it goes through its tiles, then its results.
+  union {
+    float o[16 * QT][kPadDim];
+    char keys[kKeys * kRowBytes];
+  } wave[W];
   float m[W][16 * QT], l[W][16 * QT];
   int64_t upto[64];
   int tiles[64];
@@ -203,21 +225,91 @@ struct Shared {
 
 typedef __amdgpu_buffer_rsrc_t Rsrc;
 
-// The 16 cache rows of half tile h of a wave, whose page and row in it lane h holds.
-__device__ __forceinline__ Rsrc half_tile(int page, int row, int h, const char* base,
-                                          int64_t page_bytes, int64_t row_bytes) {
-  const int p = __builtin_amdgcn_readlane(page, h);
-  const int r = __builtin_amdgcn_readlane(row, h);
-  const char* at = base + (int64_t)max(p, 0) * page_bytes + (int64_t)r * row_bytes;
-  return __builtin_amdgcn_make_buffer_rsrc((void*)at, 0, p < 0 ? 0 : -1, 0x00027000);
-}
+// The 16 cache rows of half tile h of a wave, whose first one's address lane h holds (with
+// the top bit set where no page holds them: addresses have 48).
+struct Halves {
+  uint32_t low, high;
+  __device__ __forceinline__ void set(const char* at, bool held) {
+    low = (uint32_t)(uintptr_t)at;
+    high = (uint32_t)((uintptr_t)at >> 32) | (held ? 0u : 0x80000000u);
+  }
+  __device__ __forceinline__ bool held(int h) const {
+    return (int)__builtin_amdgcn_readlane(high, h) >= 0;
+  }
+  __device__ __forceinline__ Rsrc rows(int h) const {
+    const uint32_t lo = __builtin_amdgcn_readlane(low, h), hi = __builtin_amdgcn_readlane(high, h);
+    return __builtin_amdgcn_make_buffer_rsrc((void*)((uint64_t)hi << 32 | lo), 0, ~((int)hi >> 31),
+                                             0x00027000);
+  }
+};
+template <bool ONCE>
 __device__ __forceinline__ u32x4 load16(Rsrc r, uint32_t lane, uint32_t all) {
-  return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, lane, all, 0));
+  return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, lane, all, ONCE * 2));
+}
+// The lanes' 16 bytes to lds, side by side.
+template <bool ONCE>
+__device__ __forceinline__ void load16_to(char* lds, Rsrc r, uint32_t lane, uint32_t all) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(
+      r, (__attribute__((address_space(3))) void*)lds, 16, lane, all, 0, ONCE * 2);
+}
+
+// Whether two 16-bit values hold an infinity or NaN (in the upper bits of each).
+template <class T>
+__device__ __forceinline__ uint32_t not_finite(uint32_t v) {
+  constexpr uint32_t least = std::is_same<T, half_t>::value ? 0x04000400u : 0x00800080u;
+  return ((v & 0x7fff7fffu) + least) & 0x80008000u;
+}
+
+template <class T>
+__device__ __forceinline__ float value(uint32_t v) {
+  return (float)__builtin_bit_cast(T, (uint16_t)v);
+}
+
+// The infinities and NaN that a wave's products left out, to the rows that see them (two
+// columns a lane): its tiles again, rarely.
+template <class T, int QT>
+__device__ __noinline__ void add_left_out(LateArgs* late, float (*o)[kPadDim], int b, Sequence seq,
+                                          Span span, int kv, int r0, int x, int x_end, int stripes) {
+  CachedAttnArgs a;
+  __builtin_memcpy(&a, (const void*)late, sizeof a);
+  const int lane = threadIdx.x & 63, size = a.cache.page_size;
+  const int rows = min(16 * QT, min(seq.n, a.max_new) * a.group - r0);
+  const char* v_base = a.cache.v + (int64_t)kv * a.cache.v_head + lane * 4;
+  for (; x < x_end; x += stripes) {
+    const int j0 = span.tile(x) * kKeys;
+    const bool clear = span.clear(j0) && a.rows.page(b, j0 / size, a.cache.pages) >= 0 &&
+                       a.rows.page(b, (j0 + 16) / size, a.cache.pages) >= 0;
+    for (int j = j0; j < min(j0 + kKeys, seq.len) && !clear; ++j) {
+      const int entry = j / size;
+      const int page = a.rows.page(b, entry, a.cache.pages);
+      if (page < 0) continue;
+      const uint32_t v = *reinterpret_cast<const uint32_t*>(
+          v_base + (int64_t)page * a.cache.v_page + (int64_t)(j - entry * size) * a.cache.v_row);
+      const uint32_t odd = not_finite<T>(v);
+      if (!odd) continue;
+      for (int r = 0; r < rows; ++r) {
+        const int i = (r0 + r) / a.group;
+        if (j > seq.last(i) || (j < seq.low(a, i) && j >= a.sinks)) continue;
+        if (odd & 0x8000u) o[r][2 * lane] += value<T>(v);
+        if (odd >> 31) o[r][2 * lane + 1] += value<T>(v >> 16);
+      }
+    }
+  }
+}
+
+// The operand of columns 8 c + e from eight keys' rows, two keys a register.
+__device__ __forceinline__ u32x4 turned(const u32x4 (&v)[8], int e) {
+  u32x4 out;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    out[i] = __builtin_amdgcn_perm(v[2 * i + 1][e >> 1], v[2 * i][e >> 1],
+                                   e & 1 ? 0x07060302u : 0x05040100u);
+  return out;
 }
 
 // The tiles [x0, x1) of a unit by the waves of the workgroup, and their join: the result
 // where the range is the whole unit, a partial one in the workspace elsewhere.
-template <class T, int QT, int W, int RW, bool SCORES>
+template <class T, int QT, int W, int RW, bool SCORES, bool ONCE>
 __device__ __forceinline__ void attend(const CachedAttnArgs& a, Shared<T, QT, W, RW>& lds, int b,
                                        int block, int kv, const Sequence& seq, const Span& span,
                                        int x0, int x1, bool whole, int slot) {
@@ -236,18 +328,17 @@ __device__ __forceinline__ void attend(const CachedAttnArgs& a, Shared<T, QT, W,
   const int x_end = r0 < rows ? x1 : x0;  // the waves behind the last row have nothing
 
   Vec8<T> q[QT][4];  // Q[row][32 ks + 8 grp ..]
-  int last[QT], low[QT];
-  auto token_of = [&](int t) { return min(r0 + 16 * t + col, rows - 1) / a.group; };
+  int last[QT], low[QT], token[QT];
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
     const int r = min(r0 + 16 * t + col, rows - 1);
-    const int token = r / a.group;
-    const char* p = a.q + (int64_t)(seq.start + token) * a.q_tok +
-                    (int64_t)(kv * a.group + r - token * a.group) * a.q_head + grp * 16;
+    token[t] = r / a.group;
+    const char* p = a.q + (int64_t)(seq.start + token[t]) * a.q_tok +
+                    (int64_t)(kv * a.group + r - token[t] * a.group) * a.q_head + grp * 16;
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) q[t][ks] = *reinterpret_cast<const Vec8<T>*>(p + ks * 64);
-    last[t] = seq.last(token);
-    low[t] = seq.low(a, token);
+    last[t] = seq.last(token[t]);
+    low[t] = seq.low(a, token[t]);
   }
   // The maximum and the masks want a positive scale: a negative one changes the queries' sign
   // (exact), a zero one makes them zeros.
@@ -260,10 +351,18 @@ __device__ __forceinline__ void attend(const CachedAttnArgs& a, Shared<T, QT, W,
       for (int ks = 0; ks < 4; ++ks) q[t][ks] *= sign;
     scale = scale < 0.f ? -scale : 1.f;
   }
-  const int sinks = clamp_to(a.sinks, 0, seq.len);
-  // Tiles that every row of the block sees whole.
-  const int clear_end = seq.last(span.i0) + 1, clear_low = seq.low(a, span.i1);
-  const uint32_t k_lane = (uint32_t)col * (uint32_t)a.cache.k_row + grp * 16;
+  const int sinks = span.sinks;
+  // Keys go through LDS: four whole rows an instruction (as the operand's 16 rows of 64 bytes
+  // the same bytes took the texture unit four times as long).  Chunk c of row r lies at c ^ r,
+  // so that the 16 rows of an operand's read take different banks.
+  char* keys = lds.wave[wave].keys;
+  uint32_t k_lane[4];
+  int k_read[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    k_lane[i] = (uint32_t)grp * (uint32_t)a.cache.k_row + (col ^ (4 * i + grp)) * 16;
+    k_read[i] = col * kRowBytes + ((4 * i + grp) ^ col) * 16;
+  }
   const uint32_t v_lane = (uint32_t)(4 * grp) * (uint32_t)a.cache.v_row + col * 16;
   const char* k_base = a.cache.k + (int64_t)kv * a.cache.k_head;
   const char* v_base = a.cache.v + (int64_t)kv * a.cache.v_head;
@@ -271,13 +370,15 @@ __device__ __forceinline__ void attend(const CachedAttnArgs& a, Shared<T, QT, W,
                                           a.score_keys
                          : nullptr;
 
-  int only = -1;  // the token whose rows alone count, or all
-  for (;;) {
-    const int see_low = only < 0 ? span.low : seq.low(a, only);
-    const int see_high = only < 0 ? span.high : seq.last(only) + 1;
+  // Tokens of this wave's rows.
+  const int t0 = uniform(min(r0, rows - 1) / a.group);
+  const int t1 = uniform(min(r0 + 16 * QT - 1, rows - 1) / a.group);
+  const int see_low = seq.low(a, t0), see_high = seq.last(t1) + 1;
+  const bool several = t0 != t1;
+  uint32_t left_out = 0;
+  {
     float4v acc[QT][8];
     float m[QT], l[QT];
-    bool partly = false;
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
 #pragma unroll
@@ -290,34 +391,40 @@ __device__ __forceinline__ void attend(const CachedAttnArgs& a, Shared<T, QT, W,
 #pragma unroll 1
     for (int x = x0 + stripe; x < x_end; x += kSteps * kStripes) {
       const int steps = uniform(min((x_end - x + kStripes - 1) / kStripes, kSteps));
-      int page = -1, row = 0;
+      Halves k_at, v_at;
       {
+        int page = -1, row = 0;
         const int j = span.tile(x + (lane >> 1) * kStripes) * kKeys + (lane & 1) * 16;
         if ((lane >> 1) < steps && j < seq.len) {
           const int entry = j / size;
           page = a.rows.page(b, entry, a.cache.pages);
           row = j - entry * size;
         }
+        k_at.set(k_base + (int64_t)max(page, 0) * a.cache.k_page + (int64_t)row * a.cache.k_row,
+                 page >= 0);
+        v_at.set(v_base + (int64_t)max(page, 0) * a.cache.v_page + (int64_t)row * a.cache.v_row,
+                 page >= 0);
       }
-      Vec8<T> kf[2][4];
       u32x4 vf[8];
-      // Of a half that no page holds, or behind the last tile, nothing is fetched.
+      // Of a half that no page holds, or behind the last tile, nothing is fetched (or, where
+      // the bounds of a load to LDS are not looked at, rows of page 0 that are masked).
       auto load_k = [&](int s) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const auto half = half_tile(page, row, 2 * s + u, k_base, a.cache.k_page, a.cache.k_row);
+          const Rsrc half = k_at.rows(2 * s + u);
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks)
-            kf[u][ks] = __builtin_bit_cast(Vec8<T>, load16(half, k_lane + ks * 64, 0));
+          for (int i = 0; i < 4; ++i)
+            load16_to<ONCE>(keys + (4 * u + i) * 4 * kRowBytes, half, k_lane[i],
+                      4 * i * (uint32_t)a.cache.k_row);
         }
       };
       auto load_v = [&](int s) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const auto half = half_tile(page, row, 2 * s + u, v_base, a.cache.v_page, a.cache.v_row);
+          const Rsrc half = v_at.rows(2 * s + u);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            vf[4 * u + i] = load16(half, v_lane, i * (uint32_t)a.cache.v_row);
+            vf[4 * u + i] = load16<ONCE>(half, v_lane, i * (uint32_t)a.cache.v_row);
         }
       };
       load_k(0);
@@ -326,26 +433,30 @@ __device__ __forceinline__ void attend(const CachedAttnArgs& a, Shared<T, QT, W,
 #pragma unroll 1
       for (int s = 0; s < steps; ++s) {
         const int j0 = span.tile(x + s * kStripes) * kKeys;
-        const bool held0 = __builtin_amdgcn_readlane(page, 2 * s) >= 0;
-        const bool held1 = __builtin_amdgcn_readlane(page, 2 * s + 1) >= 0;
+        // This tile's keys have landed: only its values' eight loads may be on their way.
+        asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+        const bool held0 = k_at.held(2 * s);
+        const bool held1 = k_at.held(2 * s + 1);
         float sc[QT][8];
 #pragma unroll
-        for (int t = 0; t < QT; ++t)
+        for (int u = 0; u < 2; ++u) {
+          float4v c[QT] = {};
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            float4v c{0.f, 0.f, 0.f, 0.f};
+          for (int ks = 0; ks < 4; ++ks) {
+            const Vec8<T> k = *reinterpret_cast<const Vec8<T>*>(keys + u * 16 * kRowBytes +
+                                                                k_read[ks]);
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks) c = mfma(kf[u][ks], q[t][ks], c);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sc[t][4 * u + i] = c[i];
+            for (int t = 0; t < QT; ++t) c[t] = mfma(k, q[t][ks], c[t]);
           }
-        // Not before the products: their operands' registers take the next keys.
+#pragma unroll
+          for (int t = 0; t < QT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[t][4 * u + i] = c[t][i];
+        }
+        // Not before the products: the next keys take their operands' place.
         __builtin_amdgcn_sched_barrier(0);
         load_k(s + 1);
-        const bool clear = j0 + kKeys <= clear_end && held0 && held1 &&
-                           (j0 >= clear_low || j0 + kKeys <= sinks);
-        if (!clear) {
-          partly = true;
+        if (!(held0 && held1 && span.clear(j0))) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const int j = j0 + 4 * grp + (i & 3) + 16 * (i >> 2);
@@ -356,6 +467,16 @@ __device__ __forceinline__ void attend(const CachedAttnArgs& a, Shared<T, QT, W,
             const bool seen = held & (j < see_high) & ((j >= see_low) | (j < sinks));
 #pragma unroll
             for (int w = 0; w < 4; ++w) vf[i][w] = seen ? vf[i][w] : 0u;
+          }
+          if (several) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+              for (int w = 0; w < 4; ++w) {
+                const uint32_t odd = not_finite<T>(vf[i][w]);
+                vf[i][w] &= ~((odd >> 15) * 0xffffu);
+                left_out |= odd;
+              }
           }
         }
         if constexpr (SCORES) {
@@ -395,48 +516,37 @@ __device__ __forceinline__ void attend(const CachedAttnArgs& a, Shared<T, QT, W,
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          u32x4 v;
+          const Vec8<T> v = __builtin_bit_cast(Vec8<T>, turned(vf, e));
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            v[i] = __builtin_amdgcn_perm(vf[2 * i + 1][e >> 1], vf[2 * i][e >> 1],
-                                         e & 1 ? 0x07060302u : 0x05040100u);
-#pragma unroll
-          for (int t = 0; t < QT; ++t)
-            acc[t][e] = mfma(__builtin_bit_cast(Vec8<T>, v), p[t], acc[t][e]);
+          for (int t = 0; t < QT; ++t) acc[t][e] = mfma(v, p[t], acc[t][e]);
         }
         __builtin_amdgcn_sched_barrier(0);
         load_v(s + 1);
       }
+      // The loads behind the last tile may still write to the keys' place.
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
-    bool odd = false;
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
       const float sum = group_sum(l[t]);
-      if (only < 0 || token_of(t) == only) {
-        const int r = 16 * t + col;
-        if (grp == 0) lds.m[wave][r] = m[t] * scale, lds.l[wave][r] = sum;
+      const int r = 16 * t + col;
+      if (grp == 0) lds.m[wave][r] = m[t] * scale, lds.l[wave][r] = sum;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int u = 0; u < 2; ++u)
-            *reinterpret_cast<float4v*>(&lds.o[wave][r][32 * grp + 8 * i + 4 * u]) =
-                float4v{acc[t][4 * u][i], acc[t][4 * u + 1][i], acc[t][4 * u + 2][i],
-                        acc[t][4 * u + 3][i]};
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) odd |= !(fabsf(acc[t][e][i]) < INFINITY);
-    }
-    if (only < 0) {
-      if (span.i0 == span.i1 || !partly || !__any(odd)) break;
-      only = span.i0;
-    } else if (only++ == span.i1) {
-      break;
+        for (int u = 0; u < 2; ++u)
+          *reinterpret_cast<float4v*>(&lds.wave[wave].o[r][32 * grp + 8 * i + 4 * u]) =
+              float4v{acc[t][4 * u][i], acc[t][4 * u + 1][i], acc[t][4 * u + 2][i],
+                      acc[t][4 * u + 3][i]};
     }
   }
+  if (__any(left_out))
+    add_left_out<T, QT>(late_args(), lds.wave[wave].o, b, seq, span, kv, r0, x0 + stripe, x_end,
+                        kStripes);
   __syncthreads();
 
+  LateArgs* late = late_args();
+  const int group = late->group;
   for (int item = thread; item < 16 * QT * RW * 16; item += 64 * W) {
     const int line = item >> 4, c = (item & 15) * 8;
     if (block_row + line >= rows) continue;
@@ -450,8 +560,8 @@ __device__ __forceinline__ void attend(const CachedAttnArgs& a, Shared<T, QT, W,
     for (int w = half; w < W; w += RW) {
       const float f = __builtin_amdgcn_exp2f(lds.m[w][r] - base);
       sum += f * lds.l[w][r];
-      const float4v x = *reinterpret_cast<const float4v*>(&lds.o[w][r][c]);
-      const float4v y = *reinterpret_cast<const float4v*>(&lds.o[w][r][c + 4]);
+      const float4v x = *reinterpret_cast<const float4v*>(&lds.wave[w].o[r][c]);
+      const float4v y = *reinterpret_cast<const float4v*>(&lds.wave[w].o[r][c + 4]);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         o[i] += f * x[i];
@@ -459,33 +569,33 @@ __device__ __forceinline__ void attend(const CachedAttnArgs& a, Shared<T, QT, W,
       }
     }
     if (whole) {
-      const int i = (block_row + line) / a.group;
-      const int head = kv * a.group + block_row + line - i * a.group;
+      const int i = (block_row + line) / group;
+      const int head = kv * group + block_row + line - i * group;
       const float inverse = sum == 0.f ? 0.f : 1.f / sum;
       Vec8<T> out;
 #pragma unroll
       for (int e = 0; e < 8; ++e) out[e] = (T)(sum == 0.f ? 0.f : o[e] * inverse);
-      *reinterpret_cast<Vec8<T>*>(a.o + (int64_t)(seq.start + i) * a.o_tok + head * a.o_head +
+      *reinterpret_cast<Vec8<T>*>(late->o + (int64_t)(seq.start + i) * late->o_tok + head * late->o_head +
                                   c * 2) = out;
-      if (a.lse2 && c == 0)
-        a.lse2[(int64_t)(seq.start + i) * a.hq + head] =
+      if (late->lse2 && c == 0)
+        late->lse2[(int64_t)(seq.start + i) * late->hq + head] =
             sum == 0.f ? INFINITY : base - kLift<T> + log2f(sum);
     } else {
       const int64_t part = (int64_t)slot * 16 * QT * RW + line;
-      float* out = a.part_o + part * kCacheDim + c;
+      float* out = late->part_o + part * kCacheDim + c;
       *reinterpret_cast<float4v*>(out) = float4v{o[0], o[1], o[2], o[3]};
       *reinterpret_cast<float4v*>(out + 4) = float4v{o[4], o[5], o[6], o[7]};
-      if (c == 0) *reinterpret_cast<float2v*>(a.part_ml + part * 2) = float2v{top, sum};
+      if (c == 0) *reinterpret_cast<float2v*>(late->part_ml + part * 2) = float2v{top, sum};
     }
   }
   // Tokens behind the bound on a sequence's new ones have no part in the call.
   if (whole || x1 == span.tiles)
-    if (seq.n > a.max_new && block == a.blocks - 1)
-      for (int64_t i = thread; i < (int64_t)(seq.n - a.max_new) * a.group * 16; i += 64 * W) {
-        const int64_t r = i / 16 + (int64_t)a.max_new * a.group;
-        const int64_t t = r / a.group;
-        const int64_t at = (seq.start + t) * a.o_tok + (kv * a.group + r - t * a.group) * a.o_head;
-        *reinterpret_cast<u32x4*>(a.o + at + (i & 15) * 16) = u32x4{0, 0, 0, 0};
+    if (seq.n > late->max_new && block == late->blocks - 1)
+      for (int64_t i = thread; i < (int64_t)(seq.n - late->max_new) * group * 16; i += 64 * W) {
+        const int64_t r = i / 16 + (int64_t)late->max_new * group;
+        const int64_t t = r / group;
+        const int64_t at = (seq.start + t) * late->o_tok + (kv * group + r - t * group) * late->o_head;
+        *reinterpret_cast<u32x4*>(late->o + at + (i & 15) * 16) = u32x4{0, 0, 0, 0};
       }
 }
 
@@ -504,7 +614,7 @@ __device__ __forceinline__ void clear_outside(const CachedAttnArgs& a) {
   }
 }
 
-template <class T, int QT, int W, int RW, bool SPLIT, bool SCORES>
+template <class T, int QT, int W, int RW, bool SPLIT, bool SCORES, bool ONCE>
 __global__ __launch_bounds__(64 * W) void cached_attention_kernel(CachedAttnArgs a) {
   __shared__ Shared<T, QT, W, RW> lds;
   const int hk = a.cache.kv_heads;
@@ -515,7 +625,7 @@ __global__ __launch_bounds__(64 * W) void cached_attention_kernel(CachedAttnArgs
     seq.settle();
     const Span span(a, seq, block, 16 * QT * RW);
     if (span.tiles)
-      attend<T, QT, W, RW, SCORES>(a, lds, b, block, kv, seq, span, 0, span.tiles, true, 0);
+      attend<T, QT, W, RW, SCORES, ONCE>(a, lds, b, block, kv, seq, span, 0, span.tiles, true, 0);
   } else {
     // Lines (sequence, block), 64 at a time: the places of each, and up to and with it.
     const int lane = threadIdx.x & 63;
@@ -573,7 +683,7 @@ __global__ __launch_bounds__(64 * W) void cached_attention_kernel(CachedAttnArgs
       Sequence seq = lds.seq[at];
       seq.settle();
       Span span(a, seq, block, 16 * QT * RW);
-      attend<T, QT, W, RW, SCORES>(a, lds, b, block, kv, seq, span, x0, x1, whole,
+      attend<T, QT, W, RW, SCORES, ONCE>(a, lds, b, block, kv, seq, span, x0, x1, whole,
                                2 * blockIdx.x + (unit > begin));
       if (pos < end) __syncthreads();  // the waves' results are read before the next ones come
     }
@@ -785,16 +895,16 @@ struct Layout {
   }
 };
 
-template <class T, int QT, int RW, bool SCORES>
+template <class T, int QT, int RW, bool SCORES, bool ONCE>
 int launch_attention(const CachedAttnArgs& a, const Layout& p, hipStream_t st) {
   const dim3 block(64 * kWaves);
   if (!p.workers) {
-    hipLaunchKernelGGL((cached_attention_kernel<T, QT, kWaves, RW, false, SCORES>),
+    hipLaunchKernelGGL((cached_attention_kernel<T, QT, kWaves, RW, false, SCORES, ONCE>),
                        dim3((unsigned)p.units), block, 0, st, a);
     SS_CHECK_LAUNCH("cached_attention_kernel");
     return SS_OK;
   }
-  hipLaunchKernelGGL((cached_attention_kernel<T, QT, kWaves, RW, true, SCORES>),
+  hipLaunchKernelGGL((cached_attention_kernel<T, QT, kWaves, RW, true, SCORES, ONCE>),
                      dim3((unsigned)p.workers), block, 0, st, a);
   SS_CHECK_LAUNCH("cached_attention_kernel");
   const int64_t rows = (int64_t)a.max_new * a.group;
@@ -805,14 +915,28 @@ int launch_attention(const CachedAttnArgs& a, const Layout& p, hipStream_t st) {
   return SS_OK;
 }
 
+// Bytes of keys and values that the bounds allow from which on they are loaded past the caches
+// (nt): 64 sequences of 7800 keys 186 -> 165 us, one of 131071 59 -> 53, 64 of 500 (66 MB)
+// 19 -> 17; but one of 16384 (17 MB) 16 -> 17, and rows that four waves share 36 -> 45 us.
+constexpr int64_t kOnceBytes = (int64_t)32 << 20;
+
 template <class T, bool SCORES>
 int launch_attention(const CachedAttnArgs& a, const Layout& p, hipStream_t st) {
-  if (p.block_rows == 16) return launch_attention<T, 1, 1, SCORES>(a, p, st);
-  if (p.block_rows == 32) return launch_attention<T, 2, 1, SCORES>(a, p, st);
-  if constexpr (SCORES) return SS_ERR_UNSUPPORTED;  // more rows keep none
-  else
-    return p.block_rows == 64 ? launch_attention<T, 2, 2, false>(a, p, st)
-                              : launch_attention<T, 2, 4, false>(a, p, st);
+  if (p.block_rows > 32) {
+    if constexpr (SCORES) return SS_ERR_UNSUPPORTED;  // so many rows keep none
+    else
+      return p.block_rows == 64 ? launch_attention<T, 2, 2, false, false>(a, p, st)
+                                : launch_attention<T, 2, 4, false, false>(a, p, st);
+  }
+  int64_t keys = a.max_length;
+  if (a.window && a.window < keys && a.sinks < keys)
+    keys = std::min(keys, a.window + a.sinks + a.max_new);
+  const bool once = keys >= kOnceBytes / 512 / ((int64_t)a.sequences * a.cache.kv_heads);
+  if (p.block_rows == 16)
+    return once ? launch_attention<T, 1, 1, SCORES, true>(a, p, st)
+                : launch_attention<T, 1, 1, SCORES, false>(a, p, st);
+  return once ? launch_attention<T, 2, 1, SCORES, true>(a, p, st)
+              : launch_attention<T, 2, 1, SCORES, false>(a, p, st);
 }
 
 template <class T>
