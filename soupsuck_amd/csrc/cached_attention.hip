@@ -806,6 +806,7 @@ __global__ __launch_bounds__(256) void cached_weights_again_kernel(CachedAttnArg
     const int j0 = (int)first, size = a.cache.page_size;
     Vec8<T> kf[2][4];
     bool held[2];
+    const int sinks = clamp_to(a.sinks, 0, seq.len);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int j = j0 + 16 * u, entry = j / size;
@@ -818,25 +819,38 @@ __global__ __launch_bounds__(256) void cached_weights_again_kernel(CachedAttnArg
       for (int ks = 0; ks < 4; ++ks)
         kf[u][ks] = *reinterpret_cast<const Vec8<T>*>(base + ks * 64);
     }
-    for (int r0 = 0; r0 < rows; r0 += 16) {
+    // The next 16 query rows are on their way while these are multiplied.
+    struct Rows {
+      Vec8<T> q[4];
+      float lse;
+      int last, low;
+    };
+    auto rows_from = [&](int r0) {
+      Rows x;
       const int r = min(r0 + col, rows - 1), i = r / a.group;
       const int head = kv * a.group + r - i * a.group;
       const char* p = a.q + (int64_t)(seq.start + i) * a.q_tok + head * a.q_head + grp * 16;
-      const float lse = a.lse2[(int64_t)(seq.start + i) * a.hq + head];
-      const int last = r0 + col < rows ? seq.last(i) : -1, low = seq.low(a, i);
-      Vec8<T> q[4];
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks) q[ks] = *reinterpret_cast<const Vec8<T>*>(p + ks * 64);
+      for (int ks = 0; ks < 4; ++ks) x.q[ks] = *reinterpret_cast<const Vec8<T>*>(p + ks * 64);
+      x.lse = a.lse2[(int64_t)(seq.start + i) * a.hq + head];
+      x.last = r0 + col < rows ? seq.last(i) : -1;
+      x.low = seq.low(a, i);
+      return x;
+    };
+    Rows next = rows_from(0);
+    for (int r0 = 0; r0 < rows; r0 += 16) {
+      const Rows now = next;
+      if (r0 + 16 < rows) next = rows_from(r0 + 16);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         float4v c{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) c = mfma(kf[u][ks], q[ks], c);
+        for (int ks = 0; ks < 4; ++ks) c = mfma(kf[u][ks], now.q[ks], c);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int j = j0 + 16 * u + 4 * grp + e;
-          const float w = __builtin_amdgcn_exp2f(c[e] * a.scale_log2 - lse);
-          if (held[u] && j <= last && (j >= low || j < a.sinks)) sum[4 * u + e] += w;
+          const float w = __builtin_amdgcn_exp2f(c[e] * a.scale_log2 - now.lse);
+          sum[4 * u + e] += held[u] & (j <= now.last) & ((j >= now.low) | (j < sinks)) ? w : 0.f;
         }
       }
     }

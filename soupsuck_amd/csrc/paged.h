@@ -81,7 +81,7 @@ inline int check_table(const char* who, const ss_paged_cache* c, const int32_t* 
                "%s: bad block table sizes (rows %d, pages a row %d, stride %lld)", who, rows,
                row_pages, (long long)stride);
   SS_CHECK_ARG(table && lengths, "%s: null block table or lengths", who);
-  SS_CHECK_ARG((int64_t)row_pages * c->page_size <= INT32_MAX, "%s: a row holds %lld rows", who,
+  SS_CHECK_ARG((int64_t)row_pages * c->page_size <= INT32_MAX - 2048, "%s: a row holds %lld rows", who,
                (long long)row_pages * c->page_size);
   return SS_OK;
 }
