@@ -589,8 +589,9 @@ size_t ss_cached_attention_workspace_size(int rows, int64_t tokens, int q_heads,
  * and (window == 0 or j > p - window or j < sinks); one that sees nothing gives 0.
  * What is not seen has no part in the result, infinities and NaN included.  q / o
  * [tokens, q_heads, 128] of the cache's type, (base, token stride, head stride) as
- * above.  max_new >= the most tokens of a sequence, max_length >= the greatest
- * length (rows beyond it are not read).  weights_out (NULL: none) fp32 [rows,
+ * above; the cache's rows less than 2^26 elements apart.  max_new >= the most tokens
+ * of a sequence (those behind it get 0), max_length >= the greatest length (rows
+ * beyond it are not read); tokens that no sequence has get 0.  weights_out (NULL: none) fp32 [rows,
  * kv_heads, row_pages * page_size] receives weights_in (NULL: 0; may be weights_out
  * itself) plus each cache row's probabilities, summed over the tokens and the q heads
  * of its kv head.  workspace: at least ss_cached_attention_workspace_size() bytes,

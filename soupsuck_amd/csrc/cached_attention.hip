@@ -14,11 +14,15 @@
 // column; the accumulator of two 16-key halves is the operand P^T of O^T += V^T P^T as it
 // stands, slots 8 h .. + 7 of lane group h being keys 4 h + i and 16 + 4 h + i.  V is read
 // as whole rows (lane c of a group takes columns 8 c .. + 7 of a key) and turned in
-// registers: tile e of O^T holds the columns 8 c + e.  K rows are the MFMA operand as they
-// lie.  Neither passes through LDS: at HBM's rate a CU gets 13 bytes a clock, against
-// which the 32 permutes and 16 MFMAs of a 16 KiB tile are small, and what counts is the
-// loads in flight: 16 KiB a wave, the next tile's keys issued before this one's softmax
-// and its values before the next scores.
+// registers: tile e of O^T holds the columns 8 c + e.  K goes by DMA to a place in LDS that the
+// wave has for itself and is the operand from there.
+//
+// What bounds it: HBM, at which rate a CU gets 10 to 13 bytes a clock; against that the 32 permutes
+// and 16 MFMAs of a 16 KiB tile are small (from L2 the same loop runs at 21 TB/s), and what
+// counts is the loads in flight: 16 KiB a wave, the next tile's keys issued before this
+// one's softmax and its values before the next scores.  131071 keys, 28 / 4 heads (268 MB):
+// 47.8 us and 5 us for the join, 5.1 TB/s in all and 6.2 in the loop; 64 sequences of 7800
+// (1.02 GB) 164 us, 6.2 TB/s.  Short ones are latency: 518 keys 8.6 us.
 //
 // Split over the keys (cached_attention_kernel<.., true>): the tiles of all units form one
 // line that is cut into equal ranges, one a workgroup, from the lengths on the device, so
@@ -36,7 +40,7 @@
 //
 // Weights: the scores (fp32, base 2) are left in the workspace, 4 bytes a query row and
 // key against 256 for the key again, and added up once the statistics are known; where
-// they would be many (more than 32 query rows a kv head, or more than kScoreBytes in all)
+// they would be many (more than kScoreRows query rows a kv head, or more than kScoreBytes in all)
 // the keys are multiplied again.
 #include <algorithm>
 #include <type_traits>
@@ -51,11 +55,19 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kKeys = 32;       // of a tile
 constexpr int kRowBytes = kCacheDim * 2;
 constexpr int kPadDim = kCacheDim + 4;  // fp32 row of the waves' results in LDS
-constexpr int kWholeTiles = 4;  // of a wave
+// Tiles of a wave up to which a unit is one workgroup's: 518 keys 9 us so and 17 us cut, where
+// the cut, a second start and the join launch take 8 us; 2048 keys 14 us cut, and 2 us for
+// each further tile of a wave if not.
+constexpr int kWholeTiles = 4;
+// Up to 32 query rows the scores (written and read) are no more than the keys again; 64
+// sequences with weights 202 us, with the keys again 230 us.
+constexpr int kScoreRows = 32;
 constexpr size_t kScoreBytes = (size_t)512 << 20;
 constexpr int kSteps = 31;      // tiles of a wave whose pages are looked up at once
-constexpr int kMinTiles = 8;    // of a range
-constexpr int kStart = 8;       // tiles that a unit's start and join take the time of
+constexpr int kMinTiles = 8;    // of a range: one a wave
+// Tiles that a unit's start and join take the time of: 16 ragged sequences 47 us with 0, 32
+// with 4, 26.7 with 8, 26.5 with 12; 33 new tokens of 4 sequences 34, 36 and 42 us.
+constexpr int kStart = 8;
 constexpr int64_t kMaxGrid = (int64_t)1 << 23;  // workgroups of a launch
 
 struct CachedAttnArgs {
@@ -885,6 +897,8 @@ struct Layout {
          bool weights) {
     max_new = (int)(new_bound < tokens ? new_bound : tokens);
     const int64_t of_sequence = (int64_t)(max_new > 0 ? max_new : 1) * (q_heads / kv_heads);
+    // A wave takes 16 rows, or 32, and up to four waves of 32 share a tile: 33 new tokens of 4
+    // sequences (231 rows) 40 us in blocks of 128, 43 in blocks of 64.
     block_rows = of_sequence <= 16 ? 16 : of_sequence <= 32 ? 32 : of_sequence <= 64 ? 64 : 128;
     blocks = (int)cdiv(of_sequence, block_rows);
     units = (int64_t)rows * blocks * kv_heads;
@@ -892,7 +906,7 @@ struct Layout {
     workers = max_length <= kWholeTiles * kKeys * stripes ? 0 : device_cu_count();
     score_keys = cdiv(max_length > 0 ? max_length : 1, kKeys) * kKeys;
     score_rows = 0;
-    if (weights && of_sequence <= 32 &&
+    if (weights && of_sequence <= kScoreRows &&
         (size_t)rows * kv_heads * of_sequence * score_keys * 4 <= kScoreBytes)
       score_rows = (int)of_sequence;
     bytes = 0;

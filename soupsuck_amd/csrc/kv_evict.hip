@@ -8,12 +8,13 @@
 // by its bits, 11 at a time from the top: a histogram of the digit among the rows that
 // agree with the digits found so far, then the bin that holds the m-th, found by one wave
 // (32 bins a lane, then the lane's own 32).  Counts are whole numbers, so LDS atomics give
-// the same result in any order.  Then each wave counts the
-// rows above and at the threshold in its part, a scan over the waves gives its first
-// place, and a second walk over its part writes the kept rows' numbers in order.  The five
-// walks are latency (a serial search of 256 bins had taken 28 us of 37): up to kStaged rows
-// they read keys that the first one left in LDS.
-// Copy: 16 lanes a kept row, 16 bytes of k and of v each, HBM-bound.
+// the same result in any order.  Then each wave counts the rows above and at the threshold
+// in its part, a scan over the waves gives its first place, and a second walk over its part
+// writes the kept rows' numbers in order.  The five walks are latency: 5.5 us for 1281 rows
+// (37.7 with 8-bit digits and a serial search), 12 us for 128 lines of up to 8191; up to
+// kStaged rows they read keys that the first one left in LDS.
+// Copy: 16 lanes a kept row, 16 bytes of k and of v each, HBM-bound: 490 MB in 99 us, the
+// rate of a large copy.
 #include "paged.h"
 
 namespace ss {

@@ -232,7 +232,7 @@ def cached_attention(q, cache, block_table, lengths, cu_seqlens, max_new, max_le
 
     A token sees the rows up to its own; with ``window`` only the last ``window`` of them and
     the sequence's first ``sinks``.  A token that sees none gives zeros.  ``max_new`` and
-    ``max_length`` bound a sequence's new tokens and its length.
+    ``max_length`` bound a sequence's new tokens (those behind it give zeros) and its length.
 
     ``weights_out`` (fp32 [rows, kv_heads, pages a row * page_size]) receives ``weights`` (None:
     zeros; may be the same tensor) plus every cache row's attention weight, summed over the new tokens
