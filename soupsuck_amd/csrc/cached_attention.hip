@@ -39,8 +39,9 @@
 // there, and added at the end to the rows that see them.
 //
 // Weights: the scores (fp32, base 2) are left in the workspace, 4 bytes a query row and
-// key against 256 for the key again, and added up once the statistics are known; where
-// they would be many (more than kScoreRows query rows a kv head, or more than kScoreBytes in all)
+// key against 256 for the key again, and added up once the statistics are known.  The
+// stores cost more than their bytes (152 us without, 183 with 50 MB of them in 918).  Where
+// the scores would be many (more than kScoreRows query rows a kv head, or more than kScoreBytes in all)
 // the keys are multiplied again.
 #include <algorithm>
 #include <type_traits>
@@ -55,13 +56,12 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kKeys = 32;       // of a tile
 constexpr int kRowBytes = kCacheDim * 2;
 constexpr int kPadDim = kCacheDim + 4;  // fp32 row of the waves' results in LDS
-// Tiles of a wave up to which a unit is one workgroup's: 518 keys 9 us so and 17 us cut, where
-// the cut, a second start and the join launch take 8 us; 2048 keys 14 us cut, and 2 us for
-// each further tile of a wave if not.
+// Tiles of a wave up to which a unit is one workgroup's: 518 keys 9.1 us so and 13.4 cut, 1000
+// keys 11.8 and 14.3, 64 sequences of 1000 26 and 30; 2048 keys 16.3 and 14.4.
 constexpr int kWholeTiles = 4;
-// Up to 32 query rows the scores (written and read) are no more than the keys again; 64
-// sequences with weights 202 us, with the keys again 230 us.
-constexpr int kScoreRows = 32;
+// Query rows of a kv head up to which their scores are kept: 64 sequences with 7 rows 200 us,
+// with the keys again 264; 4 sequences with 28 rows 60 and 34.
+constexpr int kScoreRows = 16;
 constexpr size_t kScoreBytes = (size_t)512 << 20;
 constexpr int kSteps = 31;      // tiles of a wave whose pages are looked up at once
 constexpr int kMinTiles = 8;    // of a range: one a wave
@@ -756,47 +756,42 @@ __global__ __launch_bounds__(256) void cached_join_kernel(CachedAttnArgs a) {
         sum == 0.f ? INFINITY : base - kLift<T> + log2f(sum);
 }
 
-// Weights of 1024 cache rows of one kv head from the scores, a thread to every 256th.
+// Weights of 512 cache rows of one kv head from the scores, every 256th to a thread.  The loads
+// take no branch, so that several rows' are in flight (with one: a third longer).  64
+// sequences with 7 rows, the whole call: 206, 200 and 201 us with 1, 2 and 4 rows a thread.
+constexpr int kWeightRows = 2;
+
 __global__ __launch_bounds__(256) void cached_weights_kernel(CachedAttnArgs a) {
   const int64_t cap = (int64_t)a.rows.row_pages * a.cache.page_size;
-  const int64_t pieces = cdiv(cap, 1024), unit = blockIdx.x / pieces;
-  const int64_t piece = blockIdx.x - unit * pieces;
+  const int64_t pieces = cdiv(cap, 256 * kWeightRows), unit = blockIdx.x / pieces;
+  const int64_t first = (blockIdx.x - unit * pieces) * 256 * kWeightRows;
   const int b = (int)(unit / a.cache.kv_heads), kv = (int)(unit - (int64_t)b * a.cache.kv_heads);
   const Sequence seq(a, b);
-  const int n = min(seq.n, a.max_new);
-  const int64_t line = ((int64_t)b * a.cache.kv_heads + kv) * cap;
-  const float* scores = a.scores + ((int64_t)b * a.cache.kv_heads + kv) * a.score_rows *
-                                       a.score_keys;
-  const int64_t j0 = piece * 1024 + threadIdx.x;
-  float sum[4] = {};
+  const int n = first < seq.len ? min(seq.n, a.max_new) : 0;
+  float sum[kWeightRows] = {};
+  int64_t j[kWeightRows], held[kWeightRows];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const int64_t j = j0 + 256 * e;
-    if (a.w_in && j < cap) sum[e] = a.w_in[line + j];
+  for (int e = 0; e < kWeightRows; ++e) {
+    j[e] = first + threadIdx.x + 256 * e;
+    held[e] = min(j[e], a.score_keys - 1);
+    if (a.w_in && j[e] < cap) sum[e] = a.w_in[unit * cap + j[e]];
   }
-  if (piece * 1024 < seq.len) {
-    for (int i = 0; i < n; ++i) {
-      const int last = seq.last(i), low = seq.low(a, i);
-      bool seen[4];
+  const float* scores = a.scores + unit * a.score_rows * a.score_keys;
+  for (int i = 0; i < n; ++i) {
+    const int last = seq.last(i), low = seq.low(a, i);
+    const float* lse = a.lse2 + (int64_t)(seq.start + i) * a.hq + kv * a.group;
+    const float* row = scores + (int64_t)i * a.group * a.score_keys;
+#pragma unroll 8
+    for (int g = 0; g < a.group; ++g)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int64_t j = j0 + 256 * e;
-        seen[e] = j <= last && (j >= low || j < a.sinks);
+      for (int e = 0; e < kWeightRows; ++e) {
+        const float w = __builtin_amdgcn_exp2f(row[g * a.score_keys + held[e]] - lse[g]);
+        sum[e] += (j[e] <= last) & ((j[e] >= low) | (j[e] < a.sinks)) ? w : 0.f;
       }
-      for (int g = 0; g < a.group; ++g) {
-        const float lse = a.lse2[(int64_t)(seq.start + i) * a.hq + kv * a.group + g];
-        const float* s = scores + (int64_t)(i * a.group + g) * a.score_keys + j0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (seen[e]) sum[e] += __builtin_amdgcn_exp2f(s[256 * e] - lse);
-      }
-    }
   }
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const int64_t j = j0 + 256 * e;
-    if (j < cap) a.w_out[line + j] = sum[e];
-  }
+  for (int e = 0; e < kWeightRows; ++e)
+    if (j[e] < cap) a.w_out[unit * cap + j[e]] = sum[e];
 }
 
 // Weights by multiplying the keys again: one wave to 32 cache rows of one kv head, all the
@@ -885,6 +880,7 @@ __global__ __launch_bounds__(256) void cached_weights_again_kernel(CachedAttnArg
 // Waves of a workgroup side by side on the query rows of a block: one as long as a sequence
 // has at most 32.
 constexpr int kWaves = 8;
+static_assert(kScoreRows == 16, "scores are kept by blocks of 16 rows only");
 
 // How a call is laid out, from what the host knows.
 struct Layout {
@@ -898,7 +894,7 @@ struct Layout {
     max_new = (int)(new_bound < tokens ? new_bound : tokens);
     const int64_t of_sequence = (int64_t)(max_new > 0 ? max_new : 1) * (q_heads / kv_heads);
     // A wave takes 16 rows, or 32, and up to four waves of 32 share a tile: 33 new tokens of 4
-    // sequences (231 rows) 40 us in blocks of 128, 43 in blocks of 64.
+    // sequences (231 rows) 36 us in blocks of 128, 39 in blocks of 64.
     block_rows = of_sequence <= 16 ? 16 : of_sequence <= 32 ? 32 : of_sequence <= 64 ? 64 : 128;
     blocks = (int)cdiv(of_sequence, block_rows);
     units = (int64_t)rows * blocks * kv_heads;
@@ -950,21 +946,18 @@ constexpr int64_t kOnceBytes = (int64_t)32 << 20;
 
 template <class T, bool SCORES>
 int launch_attention(const CachedAttnArgs& a, const Layout& p, hipStream_t st) {
-  if (p.block_rows > 32) {
-    if constexpr (SCORES) return SS_ERR_UNSUPPORTED;  // so many rows keep none
-    else
-      return p.block_rows == 64 ? launch_attention<T, 2, 2, false, false>(a, p, st)
-                                : launch_attention<T, 2, 4, false, false>(a, p, st);
-  }
+  if (!SCORES && p.block_rows > 32)
+    return p.block_rows == 64 ? launch_attention<T, 2, 2, false, false>(a, p, st)
+                              : launch_attention<T, 2, 4, false, false>(a, p, st);
   int64_t keys = a.max_length;
   if (a.window && a.window < keys && a.sinks < keys)
     keys = std::min(keys, a.window + a.sinks + a.max_new);
   const bool once = keys >= kOnceBytes / 512 / ((int64_t)a.sequences * a.cache.kv_heads);
-  if (p.block_rows == 16)
+  if (SCORES || p.block_rows == 16)
     return once ? launch_attention<T, 1, 1, SCORES, true>(a, p, st)
                 : launch_attention<T, 1, 1, SCORES, false>(a, p, st);
-  return once ? launch_attention<T, 2, 1, SCORES, true>(a, p, st)
-              : launch_attention<T, 2, 1, SCORES, false>(a, p, st);
+  return once ? launch_attention<T, 2, 1, false, true>(a, p, st)
+              : launch_attention<T, 2, 1, false, false>(a, p, st);
 }
 
 template <class T>
@@ -978,7 +971,7 @@ int launch(const CachedAttnArgs& a, const Layout& p, hipStream_t st) {
   const int64_t cap = (int64_t)a.rows.row_pages * a.cache.page_size;
   const int64_t units = (int64_t)a.sequences * a.cache.kv_heads;
   if (p.score_rows || a.tokens == 0)
-    hipLaunchKernelGGL(cached_weights_kernel, dim3((unsigned)(units * cdiv(cap, 1024))),
+    hipLaunchKernelGGL(cached_weights_kernel, dim3((unsigned)(units * cdiv(cap, 256 * kWeightRows))),
                        dim3(256), 0, st, a);
   else
     hipLaunchKernelGGL(cached_weights_again_kernel<T>,
