@@ -21,8 +21,8 @@
 // and 16 MFMAs of a 16 KiB tile are small (from L2 the same loop runs at 21 TB/s), and what
 // counts is the loads in flight: 16 KiB a wave, the next tile's keys issued before this
 // one's softmax and its values before the next scores.  131071 keys, 28 / 4 heads (268 MB):
-// 47.8 us and 5 us for the join, 5.1 TB/s in all and 6.2 in the loop; 64 sequences of 7800
-// (1.02 GB) 164 us, 6.2 TB/s.  Short ones are latency: 518 keys 8.6 us.
+// 48 us and 5 us for the join, 5.1 TB/s in all and 6.2 in the loop; 64 sequences of 7800
+// (1.02 GB) 164 us, 6.2 TB/s.  Short ones are latency: 518 keys 8.8 us.
 //
 // Split over the keys (cached_attention_kernel<.., true>): the tiles of all units form one
 // line that is cut into equal ranges, one a workgroup, from the lengths on the device, so
@@ -41,8 +41,8 @@
 // Weights: the scores (fp32, base 2) are left in the workspace, 4 bytes a query row and
 // key against 256 for the key again, and added up once the statistics are known.  The
 // stores cost more than their bytes (152 us without, 183 with 50 MB of them in 918).  Where
-// the scores would be many (more than kScoreRows query rows a kv head, or more than kScoreBytes in all)
-// the keys are multiplied again.
+// the scores would be many (more than kScoreRows query rows a kv head, or more than
+// kScoreBytes in all) the keys are multiplied again.
 #include <algorithm>
 #include <type_traits>
 
@@ -64,10 +64,13 @@ constexpr int kWholeTiles = 4;
 constexpr int kScoreRows = 16;
 constexpr size_t kScoreBytes = (size_t)512 << 20;
 constexpr int kSteps = 31;      // tiles of a wave whose pages are looked up at once
-constexpr int kMinTiles = 8;    // of a range: one a wave
 // Tiles that a unit's start and join take the time of: 16 ragged sequences 47 us with 0, 32
 // with 4, 26.7 with 8, 26.5 with 12; 33 new tokens of 4 sequences 34, 36 and 42 us.
 constexpr int kStart = 8;
+// Tiles of a range at least.  With one for each wave and a start (16) many ranges of a small
+// call held the end of one unit and the start of another, one after the other: 8 sequences
+// x 5 tokens 24.0 us against 18.2; with 3 18.9, 131071 keys the same with each.
+constexpr int kMinRange = kStart + 1;
 constexpr int64_t kMaxGrid = (int64_t)1 << 23;  // workgroups of a launch
 
 struct CachedAttnArgs {
@@ -666,7 +669,7 @@ __global__ __launch_bounds__(64 * W) void cached_attention_kernel(CachedAttnArgs
     }
     total = uniform(total) * hk;
     const int64_t range = max(uniform(quotient(total + a.workers - 1, a.workers)),
-                              (int64_t)(kMinTiles + kStart));
+                              (int64_t)kMinRange);
     const int64_t begin = uniform((int64_t)(blockIdx.x * range));
     const int64_t end = min(begin + range, total);
     int base = 0;
