@@ -205,8 +205,10 @@ struct Span {
     low = min(s.low(a, i0), high);
     sink_tiles = (clamp_to(a.sinks, 0, low) + kKeys - 1) / kKeys;
     first = max(low / kKeys, sink_tiles);
-    // a block that sees nothing still has its zeros to write
-    tiles = max(sink_tiles + max((high + kKeys - 1) / kKeys - first, 0), 1);
+    tiles = sink_tiles + max((high + kKeys - 1) / kKeys - first, 0);
+    // A block that sees nothing still has its zeros to write, and does so over tile 0: the one
+    // behind the last row would put its scores behind the score row's end.
+    if (!tiles) first = 0, tiles = 1;
   }
   // Whether every row sees the whole tile from row j on.
   __device__ __forceinline__ bool clear(int j) const {
