@@ -2,7 +2,11 @@
 //
 // o = sum_j softmax_j(scale q . k_j) v_j over the rows j that the token at row p sees
 // (j <= p, and inside the window or among the sinks), with a running maximum and sum in
-// fp32: m' = max(m, s), l' = l 2^(m - m') + 2^(s - m'), o' likewise, in base-2 scores.
+// fp32: m' = max(m, s), l' = l 2^(c (m - m')) + 2^(c (s - m')), o' likewise, s = q . k and
+// c = |scale| log2(e).  The maximum is taken off before the scale, here, in the joins and for
+// the weights: c s would be rounded to steps of whole powers of two at |c s| = 2^24, and two
+// such roundings against each other take a weight past what fp16 holds; s - m' is exact at
+// the top and next to it.
 //
 // A unit of work is one kv head over one block of a sequence's query rows (token-major, the
 // q heads of the group side by side: all of them share the cache's rows, which are read
@@ -82,11 +86,12 @@ struct CachedAttnArgs {
   const char* q; int64_t q_tok, q_head;  // bytes
   char* o; int64_t o_tok, o_head;
   int hq, group;
-  float scale_log2;
+  float scale_log2;  // |scale| log2(e), 1 for a scale of zero
+  float q_sign;      // of the scale
   int64_t window, sinks;
   const float* w_in;
   float* w_out;
-  float* lse2;  // [tokens][hq], base 2; +inf where a row sees nothing
+  float2v* stats;  // [tokens][hq]: greatest q . k and 1 / sum; +inf and 0 where a row sees nothing
   int max_new, blocks;      // new tokens of a sequence at most; row blocks of as many
   int workers;              // ranges
   int4* units;              // [sequences][blocks][kv heads]: first, last worker, slot of the first
@@ -111,6 +116,12 @@ __device__ __forceinline__ float4v mfma(Vec8<bhalf_t> a, Vec8<bhalf_t> b, float4
 // weights beside a large one count together.
 template <class T>
 constexpr float kLift = std::is_same<T, half_t>::value ? 15.f : 0.f;
+
+// What the weights need of a row, from its maximum and its (lifted) sum.
+template <class T>
+__device__ __forceinline__ float2v row_stats(float top, float sum, float inverse) {
+  return sum == 0.f ? float2v{INFINITY, 0.f} : float2v{top, inverse * __builtin_exp2f(kLift<T>)};
+}
 
 // Over the four lane groups: each swap leaves a pair of rows (halves) of lanes side by side.
 template <class F>
@@ -359,14 +370,12 @@ __device__ __forceinline__ void attend(const CachedAttnArgs& a, Shared<T, QT, W,
   }
   // The maximum and the masks want a positive scale: a negative one changes the queries' sign
   // (exact), a zero one makes them zeros.
-  float scale = a.scale_log2;
-  if (!(scale > 0.f) && scale == scale) {
-    const T sign = scale < 0.f ? (T)-1.f : (T)0.f;
+  const float scale = a.scale_log2;
+  if (a.q_sign != 1.f) {
 #pragma unroll
     for (int t = 0; t < QT; ++t)
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks) q[t][ks] *= sign;
-    scale = scale < 0.f ? -scale : 1.f;
+      for (int ks = 0; ks < 4; ++ks) q[t][ks] *= (T)a.q_sign;
   }
   const int sinks = span.sinks;
   // Keys go through LDS: four whole rows an instruction (as the operand's 16 rows of 64 bytes
@@ -503,9 +512,8 @@ __device__ __forceinline__ void attend(const CachedAttnArgs& a, Shared<T, QT, W,
               float* out = scores + (int64_t)(16 * t + col) * a.score_keys + j0 + 4 * grp;
 #pragma unroll
               for (int u = 0; u < 2; ++u)
-                *reinterpret_cast<float4v*>(out + 16 * u) =
-                    scale * float4v{sc[t][4 * u], sc[t][4 * u + 1], sc[t][4 * u + 2],
-                                    sc[t][4 * u + 3]};
+                *reinterpret_cast<float4v*>(out + 16 * u) = float4v{
+                    sc[t][4 * u], sc[t][4 * u + 1], sc[t][4 * u + 2], sc[t][4 * u + 3]};
             }
         }
         Vec8<T> p[QT];
@@ -515,18 +523,18 @@ __device__ __forceinline__ void attend(const CachedAttnArgs& a, Shared<T, QT, W,
 #pragma unroll
           for (int i = 1; i < 8; ++i) top = fmaxf(top, sc[t][i]);
           top = fmaxf(m[t], group_max(top));
-          const float base = top == -INFINITY ? 0.f : top * scale;
+          const float base = top == -INFINITY ? 0.f : top;
           if (__any(top > m[t])) {
-            const float keep = __builtin_amdgcn_exp2f(m[t] * scale - base);
+            const float keep = __builtin_amdgcn_exp2f((m[t] - base) * scale);
             l[t] *= keep;
 #pragma unroll
             for (int e = 0; e < 8; ++e) acc[t][e] *= keep;
             m[t] = top;
           }
-          const float lower = base - kLift<T>;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][i], scale, -lower));
+            const float w =
+                __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][i] - base, scale, kLift<T>));
             l[t] += w;
             p[t][i] = (T)w;
           }
@@ -547,7 +555,7 @@ __device__ __forceinline__ void attend(const CachedAttnArgs& a, Shared<T, QT, W,
     for (int t = 0; t < QT; ++t) {
       const float sum = group_sum(l[t]);
       const int r = 16 * t + col;
-      if (grp == 0) lds.m[wave][r] = m[t] * scale, lds.l[wave][r] = sum;
+      if (grp == 0) lds.m[wave][r] = m[t], lds.l[wave][r] = sum;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -575,7 +583,7 @@ __device__ __forceinline__ void attend(const CachedAttnArgs& a, Shared<T, QT, W,
     float sum = 0.f, o[8] = {};
 #pragma unroll
     for (int w = half; w < W; w += RW) {
-      const float f = __builtin_amdgcn_exp2f(lds.m[w][r] - base);
+      const float f = __builtin_amdgcn_exp2f((lds.m[w][r] - base) * late->scale_log2);
       sum += f * lds.l[w][r];
       const float4v x = *reinterpret_cast<const float4v*>(&lds.wave[w].o[r][c]);
       const float4v y = *reinterpret_cast<const float4v*>(&lds.wave[w].o[r][c + 4]);
@@ -594,9 +602,8 @@ __device__ __forceinline__ void attend(const CachedAttnArgs& a, Shared<T, QT, W,
       for (int e = 0; e < 8; ++e) out[e] = (T)(sum == 0.f ? 0.f : o[e] * inverse);
       *reinterpret_cast<Vec8<T>*>(late->o + (int64_t)(seq.start + i) * late->o_tok + head * late->o_head +
                                   c * 2) = out;
-      if (late->lse2 && c == 0)
-        late->lse2[(int64_t)(seq.start + i) * late->hq + head] =
-            sum == 0.f ? INFINITY : base - kLift<T> + log2f(sum);
+      if (late->stats && c == 0)
+        late->stats[(int64_t)(seq.start + i) * late->hq + head] = row_stats<T>(base, sum, inverse);
     } else {
       const int64_t part = (int64_t)slot * 16 * QT * RW + line;
       float* out = late->part_o + part * kCacheDim + c;
@@ -730,7 +737,8 @@ __global__ __launch_bounds__(256) void cached_join_kernel(CachedAttnArgs a) {
     const float2v s = *reinterpret_cast<const float2v*>(a.part_ml + p * 2);
     const float4v x = *reinterpret_cast<const float4v*>(a.part_o + p * kCacheDim + 4 * c);
     const float top = fmaxf(m, s[0]), base = top == -INFINITY ? 0.f : top;
-    const float f = __builtin_amdgcn_exp2f(m - base), h = __builtin_amdgcn_exp2f(s[0] - base);
+    const float f = __builtin_amdgcn_exp2f((m - base) * a.scale_log2);
+    const float h = __builtin_amdgcn_exp2f((s[0] - base) * a.scale_log2);
     o = o * f + x * h;
     l = l * f + s[1] * h;
     m = top;
@@ -746,7 +754,7 @@ __global__ __launch_bounds__(256) void cached_join_kernel(CachedAttnArgs a) {
   o = float4v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float f = __builtin_amdgcn_exp2f(ml[i][0] - base);
+    const float f = __builtin_amdgcn_exp2f((ml[i][0] - base) * a.scale_log2);
     sum += f * ml[i][1];
     o += f * sums[i][c];
   }
@@ -756,9 +764,8 @@ __global__ __launch_bounds__(256) void cached_join_kernel(CachedAttnArgs a) {
   const float inverse = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
   for (int e = 0; e < 4; ++e) out[e] = (T)(sum == 0.f ? 0.f : o[e] * inverse);
-  if (a.lse2 && c == 0)
-    a.lse2[(int64_t)(seq.start + i) * a.hq + head] =
-        sum == 0.f ? INFINITY : base - kLift<T> + log2f(sum);
+  if (a.stats && c == 0)
+    a.stats[(int64_t)(seq.start + i) * a.hq + head] = row_stats<T>(base, sum, inverse);
 }
 
 // Weights of 512 cache rows of one kv head from the scores, every 256th to a thread.  The loads
@@ -784,13 +791,15 @@ __global__ __launch_bounds__(256) void cached_weights_kernel(CachedAttnArgs a) {
   const float* scores = a.scores + unit * a.score_rows * a.score_keys;
   for (int i = 0; i < n; ++i) {
     const int last = seq.last(i), low = seq.low(a, i);
-    const float* lse = a.lse2 + (int64_t)(seq.start + i) * a.hq + kv * a.group;
+    const float2v* stats = a.stats + (int64_t)(seq.start + i) * a.hq + kv * a.group;
     const float* row = scores + (int64_t)i * a.group * a.score_keys;
 #pragma unroll 8
     for (int g = 0; g < a.group; ++g)
 #pragma unroll
       for (int e = 0; e < kWeightRows; ++e) {
-        const float w = __builtin_amdgcn_exp2f(row[g * a.score_keys + held[e]] - lse[g]);
+        const float2v s = stats[g];
+        const float w = __builtin_amdgcn_exp2f((row[g * a.score_keys + held[e]] - s[0]) *
+                                               a.scale_log2) * s[1];
         sum[e] += (j[e] <= last) & ((j[e] >= low) | (j[e] < a.sinks)) ? w : 0.f;
       }
   }
@@ -834,7 +843,7 @@ __global__ __launch_bounds__(256) void cached_weights_again_kernel(CachedAttnArg
     // The next 16 query rows are on their way while these are multiplied.
     struct Rows {
       Vec8<T> q[4];
-      float lse;
+      float2v stats;
       int last, low;
     };
     auto rows_from = [&](int r0) {
@@ -844,15 +853,18 @@ __global__ __launch_bounds__(256) void cached_weights_again_kernel(CachedAttnArg
       const char* p = a.q + (int64_t)(seq.start + i) * a.q_tok + head * a.q_head + grp * 16;
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) x.q[ks] = *reinterpret_cast<const Vec8<T>*>(p + ks * 64);
-      x.lse = a.lse2[(int64_t)(seq.start + i) * a.hq + head];
+      x.stats = a.stats[(int64_t)(seq.start + i) * a.hq + head];
       x.last = r0 + col < rows ? seq.last(i) : -1;
       x.low = seq.low(a, i);
       return x;
     };
     Rows next = rows_from(0);
     for (int r0 = 0; r0 < rows; r0 += 16) {
-      const Rows now = next;
+      Rows now = next;
       if (r0 + 16 < rows) next = rows_from(r0 + 16);
+      if (a.q_sign != 1.f)
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) now.q[ks] *= (T)a.q_sign;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         float4v c{0.f, 0.f, 0.f, 0.f};
@@ -861,7 +873,8 @@ __global__ __launch_bounds__(256) void cached_weights_again_kernel(CachedAttnArg
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int j = j0 + 16 * u + 4 * grp + e;
-          const float w = __builtin_amdgcn_exp2f(c[e] * a.scale_log2 - now.lse);
+          const float w = __builtin_amdgcn_exp2f((c[e] - now.stats[0]) * a.scale_log2) *
+                          now.stats[1];
           sum[4 * u + e] += held[u] & (j <= now.last) & ((j >= now.low) | (j < sinks)) ? w : 0.f;
         }
       }
@@ -893,7 +906,7 @@ struct Layout {
   int64_t units;
   int score_rows;           // 0: no scores kept
   int64_t score_keys;
-  size_t lse, list, ml, o, scores, bytes;  // workspace offsets
+  size_t stats, list, ml, o, scores, bytes;  // workspace offsets
   Layout(int rows, int64_t tokens, int q_heads, int kv_heads, int new_bound, int64_t max_length,
          bool weights) {
     max_new = (int)(new_bound < tokens ? new_bound : tokens);
@@ -916,7 +929,7 @@ struct Layout {
       bytes += (n + 255) / 256 * 256;
       return at;
     };
-    lse = take(weights ? (size_t)tokens * q_heads * 4 : 0);
+    stats = take(weights ? (size_t)tokens * q_heads * sizeof(float2v) : 0);
     list = take(workers ? (size_t)units * sizeof(int4) : 0);
     ml = take((size_t)workers * 2 * block_rows * 2 * 4);
     o = take((size_t)workers * 2 * block_rows * kCacheDim * 4);
@@ -1035,8 +1048,9 @@ extern "C" int ss_cached_attention(const ss_paged_cache* cache, const void* q, i
   CachedAttnArgs a{cache_view(cache), TableView{table, table_stride, row_pages, lengths},
                    cu_seqlens, rows, tokens, max_length, (const char*)q, q_tok * 2, q_head * 2,
                    (char*)o, o_tok * 2, o_head * 2, q_heads, q_heads / cache->kv_heads,
-                   scale * kLog2e, window, sinks, weights_in, weights_out,
-                   weights_out ? (float*)(ws + p.lse) : nullptr, p.max_new, p.blocks, p.workers,
+                   scale == 0.f ? 1.f : fabsf(scale) * kLog2e,
+                   scale < 0.f ? -1.f : scale == 0.f ? 0.f : 1.f, window, sinks, weights_in, weights_out,
+                   weights_out ? (float2v*)(ws + p.stats) : nullptr, p.max_new, p.blocks, p.workers,
                    (int4*)(ws + p.list), (float*)(ws + p.ml), (float*)(ws + p.o),
                    (float*)(ws + p.scores), p.score_rows, p.score_keys};
   const hipStream_t st = (hipStream_t)stream;
