@@ -179,18 +179,22 @@ def answer(model, prompts, tokens, drafts=4, temperature=0.0, budget=None, page=
     texts = [list(p) for p in prompts]
     pending = [list(p) for p in prompts]      # tokens that the cache does not hold yet
     passes = 0
-    while min(len(t) - len(p) for t, p in zip(texts, prompts)) < tokens:
-        drafted = [guess(t, drafts) for t in texts]
-        new = [p + d for p, d in zip(pending, drafted)]
+    while True:
+        # A row that has its tokens brings no more: the table has room for those alone.
+        going = [len(t) - len(p) < tokens for t, p in zip(texts, prompts)]
+        if not any(going):
+            break
+        drafted = [guess(t, drafts) if go else [] for t, go in zip(texts, going)]
+        new = [p + d if go else [] for p, d, go in zip(pending, drafted, going)]
         logits = session.forward(new)
         passes += 1
         # Row i of a sequence's logits follows its first i guesses.
         rows = []
         end = 0
-        for p, d, n in zip(pending, drafted, new):
+        for d, n in zip(drafted, new):
             end += len(n)
-            first = end - len(d) - 1
-            rows.append([min(first + i, end - 1) for i in range(drafts + 1)])
+            first = max(end - len(d) - 1, 0)
+            rows.append([max(min(first + i, end - 1), 0) for i in range(drafts + 1)])
         target = logits[torch.tensor(rows, device=device)]
         guesses = torch.tensor([d + [0] * (drafts - len(d)) for d in drafted],
                                dtype=torch.int64, device=device)
@@ -200,6 +204,8 @@ def answer(model, prompts, tokens, drafts=4, temperature=0.0, budget=None, page=
             draft_counts=torch.tensor([len(d) for d in drafted], dtype=torch.int32, device=device))
         accepted, out = accepted.tolist(), out.tolist()
         for row, n in enumerate(accepted):
+            if not going[row]:
+                continue
             session.take_back(row, len(drafted[row]) - n)
             texts[row] += out[row][:n + 1]
             pending[row] = [out[row][n]]
