@@ -172,6 +172,8 @@ def guess(text, most):
 
 def answer(model, prompts, tokens, drafts=4, temperature=0.0, budget=None, page=16, seed=0):
     """(texts, forward passes, evictions): each prompt with ``tokens`` more tokens."""
+    if not prompts or not all(prompts):
+        raise ValueError("answer: needs prompts of at least one token")
     device = model.embedding.device
     gen = torch.Generator(device=device).manual_seed(seed)
     longest = max(len(p) for p in prompts) + tokens + 2 * drafts + 2

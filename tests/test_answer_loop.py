@@ -59,3 +59,10 @@ def test_right_guesses_save_passes():
     texts, passes, _ = example.answer(Rule(), prompts, 40, drafts=4)
     assert texts == [_expected(p, 40) for p in prompts]
     assert passes < 40
+
+
+@pytest.mark.parametrize("prompts", [[], [[]], [[1, 2], []], [[], [5]]])
+def test_prompts_without_a_token_are_refused(prompts):
+    """There is no row of logits behind them; another sequence's must not answer for them."""
+    with pytest.raises(ValueError, match="at least one token"):
+        example.answer(Rule(), prompts, 3)
