@@ -7,7 +7,8 @@ answers a batch of prompts of different lengths.  Each step the next tokens are 
 text so far (the tokens that followed its last two before), one forward pass gives the
 logits behind every guess, and ``verify_drafts`` keeps the guesses that the model would have
 made.  In that pass ``append_kv`` puts the rotated keys and the values into the sequences'
-pages, ``cached_attention`` reads them and adds up every row's attention weight, and when a
+pages, ``cached_attention`` reads them and adds up every row's attention weight (again for the
+tokens that stay where some were refused: a weight is a vote of the text's own tokens), and when a
 sequence is well past its budget ``evict_kv`` moves each head's heaviest rows to fresh pages.
 """
 
@@ -90,7 +91,10 @@ class Session:
         self.lengths = [0] * rows                     # cache rows
         self.positions = [0] * rows                   # places in the text: eviction leaves them
         shape = (rows, model.kv_heads, width * page)
-        self.weights = [torch.zeros(shape, device=device) for _ in model.layers] if budget else None
+        # Every row's attention weight, and the same with the pass in hand; that pass's queries.
+        self.weights, self.voted = ([torch.zeros(shape, device=device) for _ in model.layers]
+                                    if budget else None for _ in range(2))
+        self.counts, self.queries = [0] * rows, [None] * len(model.layers)
         self.evictions = 0
 
     def _int32(self, values):
@@ -104,7 +108,7 @@ class Session:
 
     def forward(self, new):
         """Logits [tokens, vocab] of each row's new tokens, which enter the cache."""
-        counts = [len(n) for n in new]
+        self.counts = counts = [len(n) for n in new]
         for row, n in enumerate(counts):
             self.lengths[row] += n
             self._hold(row, self.lengths[row])
@@ -115,10 +119,8 @@ class Session:
 
         def attend(i, q, k, v):
             q = append_kv(self.caches[i], k, v, self.table, lengths, cu, q=q, cos=cos, sin=sin)
-            sums = self.weights[i] if self.weights else None
-            return cached_attention(q, self.caches[i], self.table, lengths, cu, max(counts),
-                                    max(self.lengths), DIM ** -0.5, weights=sums,
-                                    weights_out=sums)
+            self.queries[i] = q
+            return self._attend(i, q, lengths, cu, max(counts))
 
         tokens = torch.tensor([t for n in new for t in n], device=device)
         with torch.no_grad():
@@ -126,22 +128,35 @@ class Session:
         self.positions = [p + n for p, n in zip(self.positions, counts)]
         return logits
 
-    def take_back(self, row, n):
-        """The last n tokens of a row were not accepted."""
-        self.lengths[row] -= n
-        self.positions[row] -= n
+    def _attend(self, i, q, lengths, cu, max_new):
+        return cached_attention(q, self.caches[i], self.table, lengths, cu, max_new,
+                                max(self.lengths), DIM ** -0.5,
+                                weights=self.weights[i] if self.weights else None,
+                                weights_out=self.voted[i] if self.weights else None)
 
-    def tidy(self):
-        """Rows that were taken back have no weight; sequences well past the budget are cut
-        to it."""
+    def settle(self, refused):
+        """The last ``refused[row]`` tokens of the pass are not in the text: their rows leave the
+        cache, and the weights are those that the others' queries give."""
+        self.lengths = [n - r for n, r in zip(self.lengths, refused)]
+        self.positions = [n - r for n, r in zip(self.positions, refused)]
         if not self.weights:
             return
-        lengths = self._int32(self.lengths)
-        gone = torch.arange(self.weights[0].shape[2], device=lengths.device) >= lengths[:, None]
-        for sums in self.weights:
-            sums.masked_fill_(gone[:, None], 0.0)
-        if max(self.lengths) <= self.budget + self.slack:
+        if any(refused):
+            stay = [n - r for n, r in zip(self.counts, refused)]
+            device = self.table.device
+            starts = [sum(self.counts[:row]) for row in range(len(stay))]
+            index = torch.tensor([s + i for s, n in zip(starts, stay) for i in range(n)],
+                                 device=device)
+            lengths, cu = self._int32(self.lengths), row_offsets(stay, device)
+            for i, q in enumerate(self.queries):
+                self._attend(i, q[index], lengths, cu, max(stay))
+        self.weights, self.voted = self.voted, self.weights
+
+    def tidy(self):
+        """Sequences well past the budget are cut to it."""
+        if not self.weights or max(self.lengths) <= self.budget + self.slack:
             return
+        lengths = self._int32(self.lengths)
         old = self.pages
         keep = [min(n, self.budget) for n in self.lengths]
         self.pages = [[self.free.pop() for _ in range(-(-n // self.page))] for n in keep]
@@ -205,10 +220,10 @@ def answer(model, prompts, tokens, drafts=4, temperature=0.0, budget=None, page=
             target, guesses, uniform, temperature=temperature,
             draft_counts=torch.tensor([len(d) for d in drafted], dtype=torch.int32, device=device))
         accepted, out = accepted.tolist(), out.tolist()
+        session.settle([len(d) - n if go else 0 for d, n, go in zip(drafted, accepted, going)])
         for row, n in enumerate(accepted):
             if not going[row]:
                 continue
-            session.take_back(row, len(drafted[row]) - n)
             texts[row] += out[row][:n + 1]
             pending[row] = [out[row][n]]
         session.tidy()

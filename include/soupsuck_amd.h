@@ -594,7 +594,8 @@ size_t ss_cached_attention_workspace_size(int rows, int64_t tokens, int q_heads,
  * beyond it are not read); tokens that no sequence has get 0.  weights_out (NULL: none) fp32 [rows,
  * kv_heads, row_pages * page_size] receives weights_in (NULL: 0; may be weights_out
  * itself) plus each cache row's probabilities, summed over the tokens and the q heads
- * of its kv head.  workspace: at least ss_cached_attention_workspace_size() bytes,
+ * of its kv head: of all tokens of the call, drafts that are refused later among
+ * them (a call of the accepted ones alone gives theirs).  workspace: at least ss_cached_attention_workspace_size() bytes,
  * 16-byte aligned, fully written before it is read. */
 int ss_cached_attention(const ss_paged_cache* cache, const void* q, int64_t q_tok, int64_t q_head,
                         int q_heads, const int32_t* table, int64_t table_stride, int row_pages,

@@ -236,7 +236,9 @@ def cached_attention(q, cache, block_table, lengths, cu_seqlens, max_new, max_le
 
     ``weights_out`` (fp32 [rows, kv_heads, pages a row * page_size]) receives ``weights`` (None:
     zeros; may be the same tensor) plus every cache row's attention weight, summed over the new tokens
-    and the q heads of its kv head: what ``evict_kv`` ranks by.
+    and the q heads of its kv head: what ``evict_kv`` ranks by.  All of the call's tokens count. Drafted
+    ones that may yet be refused are better left out: ask for the weights of the accepted ones in
+    a call of their own (their queries, ``lengths`` and offsets without the refused).
     """
     nodes = native.nodes() if _is_cache(cache) else None
     if nodes is not None:
