@@ -572,7 +572,8 @@ typedef struct ss_paged_cache {
  * token's rows of cos / sin [tokens, 128] (cs_dtype the cache's or SS_F32).  Inputs
  * are (base, token stride, head stride) in elements, of the cache's type, with a
  * unit last stride, 16-byte aligned bases and strides that are multiples of 8 (of
- * 4 for fp32 cos / sin).  A token whose row the sequence does not hold is skipped. */
+ * 4 for fp32 cos / sin).  Of a token whose row no sequence holds (rows may be 0) k and v
+ * are skipped; its q is rotated like the others. */
 int ss_kv_append(const ss_paged_cache* cache, const void* k, int64_t k_tok, int64_t k_head,
                  const void* v, int64_t v_tok, int64_t v_head, const void* q, int64_t q_tok,
                  int64_t q_head, int q_heads, const void* cos, int64_t cos_tok, const void* sin,

@@ -638,6 +638,15 @@ __device__ __forceinline__ void clear_outside(const CachedAttnArgs& a) {
   }
 }
 
+// Zeros for every token of a call without sequences.
+__global__ __launch_bounds__(256) void cached_zeros_kernel(CachedAttnArgs a) {
+  const int64_t item = (int64_t)blockIdx.x * 256 + threadIdx.x, row = item / 16;
+  if (row >= a.tokens * a.hq) return;
+  const int64_t t = row / a.hq;
+  *reinterpret_cast<u32x4*>(a.o + t * a.o_tok + (row - t * a.hq) * a.o_head + (item & 15) * 16) =
+      u32x4{0, 0, 0, 0};
+}
+
 template <class T, int QT, int W, int RW, bool SPLIT, bool SCORES, bool ONCE>
 __global__ __launch_bounds__(64 * W) void cached_attention_kernel(CachedAttnArgs a) {
   __shared__ Shared<T, QT, W, RW> lds;
@@ -980,6 +989,12 @@ int launch_attention(const CachedAttnArgs& a, const Layout& p, hipStream_t st) {
 
 template <class T>
 int launch(const CachedAttnArgs& a, const Layout& p, hipStream_t st) {
+  if (a.sequences == 0) {
+    hipLaunchKernelGGL(cached_zeros_kernel, dim3((unsigned)cdiv(a.tokens * a.hq, 16)), dim3(256), 0,
+                       st, a);
+    SS_CHECK_LAUNCH("cached_zeros_kernel");
+    return SS_OK;
+  }
   if (a.tokens > 0) {
     const int rc = p.score_rows ? launch_attention<T, true>(a, p, st)
                                 : launch_attention<T, false>(a, p, st);
@@ -1027,8 +1042,8 @@ extern "C" int ss_cached_attention(const ss_paged_cache* cache, const void* q, i
   SS_CHECK_ARG(window >= 0 && sinks >= 0, "%s: negative window or sinks", who);
   SS_CHECK_ARG(q_heads > 0 && q_heads % cache->kv_heads == 0,
                "%s: %d q heads are no multiple of %d kv heads", who, q_heads, cache->kv_heads);
-  if (rows == 0 || (tokens == 0 && !weights_out)) return SS_OK;
-  SS_CHECK_ARG(cu_seqlens && (tokens == 0 || (q && o)), "%s: null pointer", who);
+  if (tokens == 0 && (rows == 0 || !weights_out)) return SS_OK;
+  SS_CHECK_ARG((rows == 0 || cu_seqlens) && (tokens == 0 || (q && o)), "%s: null pointer", who);
   SS_CHECK_ARG(aligned16(q) && aligned16(o) && ((q_tok | q_head | o_tok | o_head) & 7) == 0,
                "%s: needs 16-byte aligned bases and strides that are multiples of 8", who);
   SS_CHECK_ARG(max_new > 0 || tokens == 0, "%s: tokens, but max_new is 0", who);

@@ -73,6 +73,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
   if (is_q) {
     to = a.qo + t * a.qo_tok + h * a.qo_head;
   } else {
+    if (a.sequences == 0) return;
     const int b = sequence_of(a.cu, a.sequences, t);
     if (b < 0) return;
     // Row of the token: the sequence's own tokens are its last ones.
@@ -106,8 +107,8 @@ extern "C" int ss_kv_append(const ss_paged_cache* cache, const void* k, int64_t 
   if (const int rc = check_table(who, cache, table, table_stride, row_pages, lengths, rows))
     return rc;
   SS_CHECK_ARG(tokens >= 0, "%s: negative token count", who);
-  if (tokens == 0 || rows == 0) return SS_OK;
-  SS_CHECK_ARG(k && v && cu_seqlens, "%s: null pointer", who);
+  if (tokens == 0) return SS_OK;
+  SS_CHECK_ARG(k && v && (rows == 0 || cu_seqlens), "%s: null pointer", who);
   SS_CHECK_ARG((q == nullptr) == (q_out == nullptr) && (!q || q_heads > 0),
                "%s: q and q_out go together", who);
   SS_CHECK_ARG((cos == nullptr) == (sin == nullptr), "%s: cos and sin go together", who);

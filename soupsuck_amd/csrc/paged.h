@@ -80,7 +80,7 @@ inline int check_table(const char* who, const ss_paged_cache* c, const int32_t* 
   SS_CHECK_ARG(rows >= 0 && row_pages > 0 && stride >= row_pages,
                "%s: bad block table sizes (rows %d, pages a row %d, stride %lld)", who, rows,
                row_pages, (long long)stride);
-  SS_CHECK_ARG(table && lengths, "%s: null block table or lengths", who);
+  SS_CHECK_ARG(rows == 0 || (table && lengths), "%s: null block table or lengths", who);
   SS_CHECK_ARG((int64_t)row_pages * c->page_size <= INT32_MAX - 2048, "%s: a row holds %lld rows", who,
                (long long)row_pages * c->page_size);
   return SS_OK;

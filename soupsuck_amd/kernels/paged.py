@@ -255,8 +255,6 @@ def cached_attention(q, cache, block_table, lengths, cu_seqlens, max_new, max_le
     device = q.device
     out = torch.empty(q.shape, dtype=q.dtype, device=device)
     rows = block_table.shape[0]
-    if rows == 0:
-        return out.zero_()
     size = _lib.load().ss_cached_attention_workspace_size(
         rows, tokens, heads, cache.k.shape[1], max_new, max_length, weights_out is not None)
     with torch.cuda.device(device):
