@@ -12,7 +12,7 @@ import torch
 
 from oracle import cache as ocache
 from soupsuck_amd import _lib
-from soupsuck_amd.kernels.paged import PagedCache
+from soupsuck_amd.kernels.paged import PagedCache, cached_attention
 from tests.cache_util import attention_bound, build, host, offsets
 from tests.test_gpu_cache import SCALE, _tokens
 
@@ -67,4 +67,29 @@ def test_windows_past_the_bound(device, bound, new, hq, sinks, dtype):
     want[:, :, :bound] += w
     error = np.zeros_like(want)
     error[:, :, :bound] = w * 2 * 2.0 ** -24 * (128 * reach + 4 * (1 + reach) + bound)
+    assert (np.abs(host(sums) - want) <= error + 2 * 2.0 ** -24 * want + 1e-12).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("bound", [4000, 131072, 3 * 10 ** 6, 2 ** 31 - 1])
+@pytest.mark.parametrize("new,hq", [(1, 12), (2, 14), (4, 12), (20, 6)])
+def test_the_bound_has_no_part_in_the_result(device, bound, new, hq, dtype):
+    """Large bounds choose loads past the caches and keep no scores for the weights; what is
+    summed, and so the tolerance, is the sequences' own rows."""
+    print(f"case bound {bound} {new} {hq} {dtype}", flush=True)
+    lengths = (700, new, 90, 1200)
+    c = build(lengths, 2, 16, dtype, device, seed=17)
+    cu = offsets((new,) * 4, device)
+    q = _tokens(new * 4, hq, dtype, device, 0)
+    base = torch.rand((4, 2, c.table.shape[1] * 16),
+                      generator=torch.Generator().manual_seed(5)).to(device)
+    sums = torch.full_like(base, float("nan"))
+    out = cached_attention(q, PagedCache(c.k, c.v), c.table, c.lengths, cu, new, bound, SCALE,
+                           weights=base, weights_out=sums)
+    ref, spread, reach, w = ocache.attention(host(q), host(c.k), host(c.v), c.table.tolist(),
+                                             lengths, cu.tolist(), SCALE)
+    rows = max(lengths)
+    assert (np.abs(host(out) - ref) <= attention_bound(dtype, ref, spread, reach, rows)).all()
+    want = host(base) + w
+    error = w * 2 * 2.0 ** -24 * (128 * reach + 4 * (1 + reach) + rows)
     assert (np.abs(host(sums) - want) <= error + 2 * 2.0 ** -24 * want + 1e-12).all()
