@@ -26,7 +26,7 @@
 // counts is the loads in flight: 16 KiB a wave, the next tile's keys issued before this
 // one's softmax and its values before the next scores.  131071 keys, 28 / 4 heads (268 MB):
 // 48 us and 5 us for the join, 5.1 TB/s in all and 6.2 in the loop; 64 sequences of 7800
-// (1.02 GB) 164 us, 6.2 TB/s.  Short ones are latency: 518 keys 8.8 us.
+// (1.02 GB) 164 us, 6.2 TB/s.  Short ones are latency: 518 keys 8.9 us.
 //
 // Split over the keys (cached_attention_kernel<.., true>): the tiles of all units form one
 // line that is cut into equal ranges, one a workgroup, from the lengths on the device, so
@@ -44,7 +44,7 @@
 //
 // Weights: the scores (fp32, base 2) are left in the workspace, 4 bytes a query row and
 // key against 256 for the key again, and added up once the statistics are known.  The
-// stores cost more than their bytes (152 us without, 183 with 50 MB of them in 918).  Where
+// stores cost more than their bytes (148 us without, 183 with 50 MB of them in 918).  Where
 // the scores would be many (more than kScoreRows query rows a kv head, or more than
 // kScoreBytes in all) the keys are multiplied again.
 #include <algorithm>
@@ -60,11 +60,16 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kKeys = 32;       // of a tile
 constexpr int kRowBytes = kCacheDim * 2;
 constexpr int kPadDim = kCacheDim + 4;  // fp32 row of the waves' results in LDS
-// Tiles of a wave up to which a unit is one workgroup's: 518 keys 9.1 us so and 13.4 cut, 1000
-// keys 11.8 and 14.3, 64 sequences of 1000 26 and 30; 2048 keys 16.3 and 14.4.
+// Tiles of a wave up to which a unit is one workgroup's.  So and cut, one sequence and eight, us:
+// 6 query rows a kv head (4 tiles are 1024 keys) 1000 keys 11.9 / 12.5 and 12.4 / 14.7, 2000 keys
+// 16.5 / 13.9 and 20.8 / 15.0; 30 rows, 500 keys 13.0 / 15.4 and 13.4 / 17.1, 1100 keys 16.2 / 15.8
+// and 16.4 / 17.3; 54 rows (512 keys) 500 keys 16.0 / 16.3 and 16.3 / 18.7, 700 keys 17.5 / 16.4 and
+// 17.8 / 18.7; 198 rows (256 keys) 250 keys 16.6 / 20.0 and 17.4 / 25.3.
 constexpr int kWholeTiles = 4;
-// Query rows of a kv head up to which their scores are kept: 64 sequences with 7 rows 200 us,
-// with the keys again 264; 4 sequences with 28 rows 60 and 34.
+// Query rows of a kv head up to which their scores are kept (those of one 16-row block): kept
+// and with the keys again, 64 sequences of 7000 keys with 7 rows 196 and 249 us, 14 rows 215 and
+// 252, 16 rows (two kv heads) 117 and 135; 4 of them 27.9 / 32.4, 32.7 / 33.6, 25.2 / 26.8; 4 of
+// 1000 18.1 / 17.4, 22.0 / 18.3, 18.0 / 18.1.  4 sequences with 28 rows took 60 and 34.
 constexpr int kScoreRows = 16;
 constexpr size_t kScoreBytes = (size_t)512 << 20;
 constexpr int kSteps = 31;      // tiles of a wave whose pages are looked up at once
