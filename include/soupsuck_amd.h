@@ -625,6 +625,93 @@ int ss_kv_evict(const ss_paged_cache* cache, const int32_t* table, int64_t table
                 int64_t budget, int64_t sinks, int64_t recent, int32_t* out_lengths,
                 float* out_weights, void* workspace, size_t workspace_bytes, void* stream);
 
+/* Reads the packed tokens' rows back as append wrote them: k and v [count, tokens,
+ * kv_heads, 128] (contiguous, 16-byte aligned, of the caches' type) receive, for each of
+ * `count` caches of one shape, strides and type (one a layer), the last cu_seqlens[b + 1] -
+ * cu_seqlens[b] rows of every sequence in order; 0 for a row that the sequence does not hold. */
+int ss_kv_read(const ss_paged_cache* const* caches, int count, const int32_t* table,
+               int64_t table_stride, int row_pages, const int32_t* lengths,
+               const int32_t* cu_seqlens, int rows, int64_t tokens, void* k, void* v,
+               void* stream);
+
+/* Block tables of sequences that continue others (beams): row i of out_table (int32
+ * [new_rows, row_pages], contiguous) and out_lengths (int32 [new_rows]) take the length of
+ * old row p = parents[i] (int32; one outside [0, rows) counts as an empty sequence) and its
+ * full pages.  The entry behind those, where the next token goes, is spare[i], to which the
+ * rows that p has beyond its full pages are copied in each of `count` caches of one
+ * shape, strides and type; -1 where p holds no page with those.  Entries behind it are -1.
+ * The spare pages must not be pages that `table` names, nor named twice; full pages are
+ * shared from then on. */
+int ss_kv_fork(const ss_paged_cache* const* caches, int count, const int32_t* table,
+               int64_t table_stride, int row_pages, const int32_t* lengths, int rows,
+               const int32_t* parents, const int32_t* spare, int new_rows, int32_t* out_table,
+               int32_t* out_lengths, void* stream);
+
+/* A paged cache that holds its rows in 4 bits: 128 keys and 128 values of a head in blocks
+ * of 32 with a scale 2^e, codes of 1 sign, 2 exponent and 1 mantissa bit (0, 0.5, 1, 1.5,
+ * 2, 3, 4, 6).  e is the least with which no code is past 6, from -13 to 13 for SS_F16 and
+ * from -125 to 125 for SS_BF16 (what is past 6 2^e then is held as that); codes round to
+ * nearest even.  A block with an infinity or NaN is held as NaN.  data: base of
+ * [pages, kv_heads, page_size / 16, 2176] bytes with any page, head and group strides
+ * (bytes, multiples of 16), 16-byte aligned.  A group of 16 rows is: key codes
+ * [block 4][row 16][16 bytes], value codes [row / 4][dimension / 8][row % 4][4 bytes] (of
+ * two codes in a byte the low one is the lower dimension's), key scales and value scales
+ * [block 4][row 16], a byte e + 127 each (255: NaN).  dtype (SS_F16 or SS_BF16) is that of the
+ * tensors around it. */
+typedef struct ss_paged_cache4 {
+  void* data;
+  int64_t page, head, group;
+  int pages, page_size, kv_heads, head_dim;
+  int dtype;
+} ss_paged_cache4;
+
+/* ss_kv_append into a 4-bit cache.  The rotated key is not rounded before it becomes codes. */
+int ss_kv_append4(const ss_paged_cache4* cache, const void* k, int64_t k_tok, int64_t k_head,
+                  const void* v, int64_t v_tok, int64_t v_head, const void* q, int64_t q_tok,
+                  int64_t q_head, int q_heads, const void* cos, int64_t cos_tok, const void* sin,
+                  int64_t sin_tok, int cs_dtype, const int32_t* table, int64_t table_stride,
+                  int row_pages, const int32_t* lengths, const int32_t* cu_seqlens, int rows,
+                  int64_t tokens, void* q_out, int64_t qo_tok, int64_t qo_head, void* stream);
+
+/* ss_cached_attention over a 4-bit cache, without weights. */
+size_t ss_cached_attention4_workspace_size(int rows, int64_t tokens, int q_heads, int kv_heads,
+                                           int max_new, int64_t max_length);
+int ss_cached_attention4(const ss_paged_cache4* cache, const void* q, int64_t q_tok,
+                         int64_t q_head, int q_heads, const int32_t* table, int64_t table_stride,
+                         int row_pages, const int32_t* lengths, const int32_t* cu_seqlens,
+                         int rows, int64_t tokens, int max_new, int64_t max_length, float scale,
+                         int64_t window, int64_t sinks, void* o, int64_t o_tok, int64_t o_head,
+                         void* workspace, size_t workspace_bytes, void* stream);
+
+/* ss_kv_read and ss_kv_fork over 4-bit caches; fork copies whole groups of 16 rows. */
+int ss_kv_read4(const ss_paged_cache4* const* caches, int count, const int32_t* table,
+                int64_t table_stride, int row_pages, const int32_t* lengths,
+                const int32_t* cu_seqlens, int rows, int64_t tokens, void* k, void* v,
+                void* stream);
+int ss_kv_fork4(const ss_paged_cache4* const* caches, int count, const int32_t* table,
+                int64_t table_stride, int row_pages, const int32_t* lengths, int rows,
+                const int32_t* parents, const int32_t* spare, int new_rows, int32_t* out_table,
+                int32_t* out_lengths, void* stream);
+
+/* ---------------------------------------------------------------- beams ---
+ * Scratch bytes of ss_select_beams. */
+size_t ss_select_beams_workspace_size(int sequences, int beams, int64_t vocab, int count,
+                                      int dtype);
+
+/* The `count` best continuations of each sequence's beams: of all (beam, token) those with the
+ * greatest scores[beam] + logits[beam, token] - log sum exp logits[beam] (fp64 from the
+ * sum on; NaN counts as -inf), best first; of equal ones the lower beam's, the greater logit
+ * (a NaN logit as -inf), the lower token.  logits [sequences, beams, vocab] are fp16, bf16 or fp32, (base,
+ * sequence stride, beam stride) in elements with a unit last stride; scores fp32
+ * [sequences, beams], contiguous (-inf for a beam that is not there).  out_scores fp32,
+ * parents int32 (the beam) and tokens int64, [sequences, count].  At most 64 beams and a
+ * count of 64 (and of beams * vocab), beams * count at most 2048, 65535 sequences.  workspace: at least
+ * ss_select_beams_workspace_size() bytes, 16-byte aligned. */
+int ss_select_beams(const void* logits, int64_t l_seq, int64_t l_beam, int dtype,
+                    const float* scores, int sequences, int beams, int64_t vocab, int count,
+                    float* out_scores, int32_t* parents, int64_t* tokens, void* workspace,
+                    size_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------- drafted tokens ---
  * Scratch bytes of ss_verify_drafts (drafted: 1 with draft logits). */
 size_t ss_verify_drafts_workspace_size(int rows, int drafts, int64_t vocab, int drafted);

@@ -40,6 +40,14 @@ class PagedCacheStruct(ctypes.Structure):
                 ("dtype", _int)]
 
 
+class PagedCache4Struct(ctypes.Structure):
+    """ss_paged_cache4 of include/soupsuck_amd.h."""
+
+    _fields_ = [("data", _c_void_p), ("page", _i64), ("head", _i64), ("group", _i64),
+                ("pages", _int), ("page_size", _int), ("kv_heads", _int), ("head_dim", _int),
+                ("dtype", _int)]
+
+
 # name -> argument types (restype is int unless listed in _RESTYPES)
 SIGNATURES = {
     "ss_abi_version": [],
@@ -152,6 +160,17 @@ SIGNATURES = {
     "ss_kv_evict": [_c_void_p, _c_void_p, _i64, _int, _c_void_p, _int, _i64, _c_void_p,
                     _c_void_p, _i64, _int, _i64, _i64, _i64, _c_void_p, _c_void_p, _c_void_p,
                     _size, _c_void_p],
+    "ss_kv_read": [_c_void_p, _int, _c_void_p, _i64, _int, _c_void_p, _c_void_p, _int, _i64,
+                   _c_void_p, _c_void_p, _c_void_p],
+    "ss_kv_fork": [_c_void_p, _int, _c_void_p, _i64, _int, _c_void_p, _int, _c_void_p, _c_void_p,
+                   _int, _c_void_p, _c_void_p, _c_void_p],
+    "ss_cached_attention4_workspace_size": [_int, _i64, _int, _int, _int, _i64],
+    "ss_cached_attention4": [_c_void_p, _c_void_p, _i64, _i64, _int, _c_void_p, _i64, _int,
+                             _c_void_p, _c_void_p, _int, _i64, _int, _i64, _f32, _i64, _i64,
+                             _c_void_p, _i64, _i64, _c_void_p, _size, _c_void_p],
+    "ss_select_beams_workspace_size": [_int, _int, _i64, _int, _int],
+    "ss_select_beams": [_c_void_p, _i64, _i64, _int, _c_void_p, _int, _int, _i64, _int,
+                        _c_void_p, _c_void_p, _c_void_p, _c_void_p, _size, _c_void_p],
     "ss_verify_drafts_workspace_size": [_int, _int, _i64, _int],
     "ss_verify_drafts": [_c_void_p, _i64, _i64] * 2 + [_int] + [_c_void_p] * 3
                         + [_int, _int, _i64, _f64] + [_c_void_p] * 3 + [_size, _c_void_p],
@@ -160,12 +179,16 @@ SIGNATURES = {
     "ss_ce_finalize_dx": [_c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p, _int, _i64, _i64,
                           _c_void_p],
 }
+SIGNATURES.update({f"{name}4": SIGNATURES[name]
+                   for name in ("ss_kv_append", "ss_kv_read", "ss_kv_fork")})
 _RESTYPES = {"ss_last_error": ctypes.c_char_p, "ss_nf4_gemm_workspace_size": _size,
              "ss_lora_workspace_size": _size, "ss_qlora_rank_workspace_size": _size,
              "ss_gemm_f16_workspace_size": _size, "ss_add_rmsnorm_dgamma_waves": _i64,
              "ss_attn_varlen_bwd_workspace_size": _size,
              "ss_cached_attention_workspace_size": _size, "ss_kv_evict_workspace_size": _size,
-             "ss_verify_drafts_workspace_size": _size}
+             "ss_verify_drafts_workspace_size": _size,
+             "ss_cached_attention4_workspace_size": _size,
+             "ss_select_beams_workspace_size": _size}
 
 _lock = threading.Lock()
 _lib = None

@@ -1,0 +1,375 @@
+// Attention of new tokens over a paged cache that holds its rows in 4 bits (paged4.h).
+//
+// o = sum_j softmax_j(scale q . k_j) v_j with a running maximum and sum in fp32, units of work and
+// their split over the keys as over a 16-bit cache (cached_units.h).  Keys and values
+// become 16-bit numbers in registers, exactly (two significant bits times a power of two), on
+// v_cvt_scalef32_pk, which takes the block's scale with it; all products are 16-bit MFMAs,
+// so that the result is that of a 16-bit cache with the same rows.
+//
+// Products (v_mfma_f32_16x16x32): S^T = K Q^T and O^T += V^T P^T, operands as over a 16-bit
+// cache.  A group of 16 rows is laid out for it: 16 bytes a lane are one key's 32
+// dimensions of one block, the operands of four products as they stand (the queries' dimensions
+// are taken in the same order: lane group g has 32 g + 8 s .. + 7 of product s), and 16 bytes
+// are four keys' values in eight columns, which permutes pair by key.
+#include "cached_units.h"
+#include "paged4.h"
+
+namespace ss {
+namespace {
+
+constexpr int kDeep = 3;       // tiles of a wave on their way
+constexpr int kSteps = 27;     // tiles of a wave whose pages are looked up at once
+static_assert(kSteps % kDeep == 0 && 2 * (kSteps + kDeep) <= kWave, "a lane for every half tile");
+
+template <int QT, int W>
+struct Shared4 : Results<QT, W> {
+  struct alignas(16) {
+    float o[16 * QT][kPadDim];
+  } wave[W];
+};
+
+// 32 rows of one kv head: two groups' parts, as the lanes load them.
+struct Tile4 {
+  u32x4 k[2], v[2];
+  uint32_t ks[2], vs[2];  // a key's scale; those of four values' rows
+};
+
+// NaN for the rows that see a value block that is, which a wave's products left out: its tiles
+// again, rarely (two columns a lane).
+template <int QT>
+__device__ __noinline__ void add_left_out4(LateArgs* late, float (*o)[kPadDim], int b, Sequence seq,
+                                           Span span, int kv, int r0, int x, int x_end,
+                                           int stripes) {
+  CachedAttnArgs a;
+  __builtin_memcpy(&a, (const void*)late, sizeof a);
+  const int lane = threadIdx.x & 63, size = a.cache.page_size;
+  const int rows = min(16 * QT, min(seq.n, a.max_new) * a.group - r0);
+  const char* base = a.cache.k + (int64_t)kv * a.cache.k_head + kValueScales;
+  for (; x < x_end; x += stripes) {
+    const int j0 = span.tile(x) * kKeys;
+    for (int j = j0; j < min(j0 + kKeys, seq.len); ++j) {
+      const int entry = j / size, row = j - entry * size;
+      const int page = a.rows.page(b, entry, a.cache.pages);
+      if (page < 0) continue;
+      const uint8_t scale = *reinterpret_cast<const uint8_t*>(
+          base + (int64_t)page * a.cache.k_page + (int64_t)(row >> 4) * a.cache.k_row +
+          scale_at(row & 15, lane >> 4));
+      if (scale != kNotFinite) continue;
+      for (int r = 0; r < rows; ++r) {
+        const int i = (r0 + r) / a.group;
+        if (j > seq.last(i) || (j < seq.low(a, i) && j >= a.sinks)) continue;
+        o[r][2 * lane] = o[r][2 * lane + 1] = NAN;
+      }
+    }
+  }
+}
+
+// The tiles [x0, x1) of a unit by the waves of the workgroup, and their join.
+template <class T, int QT, int W, int RW, bool ONCE>
+__device__ __forceinline__ void attend4(const CachedAttnArgs& a, Shared4<QT, W>& lds, int b,
+                                        int block, int kv, const Sequence& seq, const Span& span,
+                                        int x0, int x1, bool whole, int slot) {
+  // Opaque, so that what follows from them is not kept in registers through the segments' loop.
+  int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6));
+  asm volatile("" : "+v"(lane), "+s"(wave));
+  const int thread = 64 * wave + lane;
+  const int col = lane & 15, grp = lane >> 4;
+  const int size = a.cache.page_size;
+  const int rows = min(seq.n, a.max_new) * a.group;
+  const int block_row = block * 16 * QT * RW;
+  const int r0 = block_row + wave % RW * 16 * QT;
+  const int stripe = wave / RW;
+  constexpr int kStripes = W / RW;
+  const int x_end = r0 < rows ? x1 : x0;  // the waves behind the last row have nothing
+
+  Vec8<T> q[QT][4];  // Q[row][32 grp + 8 s ..]
+  int last[QT], low[QT];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int r = min(r0 + 16 * t + col, rows - 1);
+    const int token = r / a.group;
+    const char* p = a.q + (int64_t)(seq.start + token) * a.q_tok +
+                    (int64_t)(kv * a.group + r - token * a.group) * a.q_head + grp * 64;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) q[t][s] = *reinterpret_cast<const Vec8<T>*>(p + s * 16);
+    last[t] = seq.last(token);
+    low[t] = seq.low(a, token);
+  }
+  // The maximum and the masks want a positive scale: a negative one changes the queries' sign
+  // (exact), a zero one makes them zeros.
+  const float scale = a.scale_log2;
+  if (a.q_sign != 1.f) {
+#pragma unroll
+    for (int t = 0; t < QT; ++t)
+#pragma unroll
+      for (int s = 0; s < 4; ++s) q[t][s] *= (T)a.q_sign;
+  }
+  const int sinks = span.sinks;
+  const char* base = a.cache.k + (int64_t)kv * a.cache.k_head;
+  const uint32_t lane16 = lane * 16, value_scales = scale_at(4 * grp, col >> 2);
+
+  // Tokens of this wave's rows.
+  const int t0 = uniform(min(r0, rows - 1) / a.group);
+  const int t1 = uniform(min(r0 + 16 * QT - 1, rows - 1) / a.group);
+  const int see_low = seq.low(a, t0), see_high = seq.last(t1) + 1;
+  const bool several = t0 != t1;
+  bool left_out = false;
+  {
+    float4v acc[QT][8];
+    float m[QT], l[QT];
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[t][e] = float4v{0.f, 0.f, 0.f, 0.f};
+      m[t] = -INFINITY;
+      l[t] = 0.f;
+    }
+    // Some of this wave's tiles at a time: their groups' addresses in one load, the lanes behind
+    // them none.
+#pragma unroll 1
+    for (int x = x0 + stripe; x < x_end; x += kSteps * kStripes) {
+      const int steps = uniform(min((x_end - x + kStripes - 1) / kStripes, kSteps));
+      Halves at;
+      {
+        int page = -1, row = 0;
+        const int j = span.tile(x + (lane >> 1) * kStripes) * kKeys + (lane & 1) * 16;
+        if ((lane >> 1) < steps && j < seq.len) {
+          const int entry = j / size;
+          page = a.rows.page(b, entry, a.cache.pages);
+          row = j - entry * size;
+        }
+        at.set(base + (int64_t)max(page, 0) * a.cache.k_page +
+                   (int64_t)(row >> 4) * a.cache.k_row,
+               page >= 0);
+      }
+      // Of a group that no page holds, or behind the last tile, nothing is fetched: zeros.
+      auto fetch = [&](Tile4& tile, int s) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const Rsrc group = at.rows(2 * s + u);
+          tile.k[u] = load16<ONCE>(group, lane16, 0);
+          tile.v[u] = load16<ONCE>(group, lane16, kValues);
+          tile.ks[u] = __builtin_amdgcn_raw_buffer_load_b8(group, lane, kKeyScales, ONCE * 2);
+          tile.vs[u] =
+              __builtin_amdgcn_raw_buffer_load_b32(group, value_scales, kValueScales, ONCE * 2);
+        }
+      };
+      auto attend_tile = [&](Tile4& tile, int s) {
+        const int j0 = span.tile(x + s * kStripes) * kKeys;
+        const bool held0 = at.held(2 * s), held1 = at.held(2 * s + 1);
+        float sc[QT][8];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const float ks = scale_of(tile.ks[u]);
+          float4v c[QT] = {};
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const Vec8<T> k = __builtin_bit_cast(Vec8<T>, decoded<T>(tile.k[u][w], ks));
+#pragma unroll
+            for (int t = 0; t < QT; ++t) c[t] = mfma(k, q[t][w], c[t]);
+          }
+#pragma unroll
+          for (int t = 0; t < QT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[t][4 * u + i] = c[t][i];
+        }
+        if (!(held0 && held1 && span.clear(j0))) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int j = j0 + 4 * grp + (i & 3) + 16 * (i >> 2);
+            const bool held = i < 4 ? held0 : held1;
+#pragma unroll
+            for (int t = 0; t < QT; ++t)
+              sc[t][i] = held & (j <= last[t]) & ((j >= low[t]) | (j < sinks)) ? sc[t][i] : -INFINITY;
+            // Values that no row of the wave sees become zeros, and so do NaN ones that some
+            // see and others do not.
+            const bool seen = held & (j < see_high) & ((j >= see_low) | (j < sinks));
+            uint32_t& scales = tile.vs[i >> 2];
+            const uint32_t byte = 255u << 8 * (i & 3);
+            const bool odd = seen & several & ((scales & byte) == byte);
+            left_out |= odd;
+            const bool counts = seen & !odd;
+            tile.v[i >> 2][i & 3] = counts ? tile.v[i >> 2][i & 3] : 0u;
+            scales = counts ? scales : (scales & ~byte) | 127u << 8 * (i & 3);
+          }
+        }
+        Vec8<T> p[QT];
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+          float top = sc[t][0];
+#pragma unroll
+          for (int i = 1; i < 8; ++i) top = fmaxf(top, sc[t][i]);
+          top = fmaxf(m[t], group_max(top));
+          const float base_score = top == -INFINITY ? 0.f : top;
+          if (__any(top > m[t])) {
+            const float keep = __builtin_amdgcn_exp2f((m[t] - base_score) * scale);
+            l[t] *= keep;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[t][e] *= keep;
+            m[t] = top;
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float w =
+                __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][i] - base_score, scale, kLift<T>));
+            l[t] += w;
+            p[t][i] = (T)w;
+          }
+        }
+        u32x4 vf[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          vf[i] = decoded<T>(tile.v[i >> 2][i & 3],
+                             scale_of(tile.vs[i >> 2] >> 8 * (i & 3) & 255u));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const Vec8<T> v = __builtin_bit_cast(Vec8<T>, turned(vf, e));
+#pragma unroll
+          for (int t = 0; t < QT; ++t) acc[t][e] = mfma(v, p[t], acc[t][e]);
+        }
+      };
+      Tile4 tiles[kDeep];
+#pragma unroll
+      for (int d = 0; d < kDeep; ++d) fetch(tiles[d], d);
+#pragma unroll 1
+      for (int s = 0; s < steps; s += kDeep)
+#pragma unroll
+        for (int d = 0; d < kDeep; ++d) {
+          if (s + d < steps) attend_tile(tiles[d], s + d);
+          // Not before the products, which the registers' old contents are for.
+          __builtin_amdgcn_sched_barrier(0);
+          fetch(tiles[d], s + d + kDeep);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      const float sum = group_sum(l[t]);
+      const int r = 16 * t + col;
+      if (grp == 0) lds.m[wave][r] = m[t], lds.l[wave][r] = sum;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          *reinterpret_cast<float4v*>(&lds.wave[wave].o[r][32 * grp + 8 * i + 4 * u]) =
+              float4v{acc[t][4 * u][i], acc[t][4 * u + 1][i], acc[t][4 * u + 2][i],
+                      acc[t][4 * u + 3][i]};
+    }
+  }
+  if (__any(left_out))
+    add_left_out4<QT>(late_args(), lds.wave[wave].o, b, seq, span, kv, r0, x0 + stripe, x_end,
+                      kStripes);
+  finish_unit<T, QT, W, RW>(lds, lds.wave, thread, block, block_row, rows, kv, seq, span, x1,
+                            whole, slot);
+}
+
+template <class T, int QT, int W, int RW, bool SPLIT, bool ONCE>
+__global__ __launch_bounds__(64 * W) void cached_attention4_kernel(CachedAttnArgs a) {
+  __shared__ Shared4<QT, W> lds;
+  auto unit = [&](int b, int block, int kv, const Sequence& seq, const Span& span, int x0, int x1,
+                  bool whole, int slot) {
+    attend4<T, QT, W, RW, ONCE>(a, lds, b, block, kv, seq, span, x0, x1, whole, slot);
+  };
+  if constexpr (SPLIT) for_ranges<QT, W, RW>(a, lds, unit);
+  else for_unit<QT, RW>(a, unit);
+  if (blockIdx.x == 0) clear_outside<W>(a);
+}
+
+template <class T, int QT, int RW, bool ONCE>
+int launch_attention4(const CachedAttnArgs& a, const Layout& p, hipStream_t st) {
+  const dim3 block(64 * kWaves);
+  if (!p.workers) {
+    hipLaunchKernelGGL((cached_attention4_kernel<T, QT, kWaves, RW, false, ONCE>),
+                       dim3((unsigned)p.units), block, 0, st, a);
+    SS_CHECK_LAUNCH("cached_attention4_kernel");
+    return SS_OK;
+  }
+  hipLaunchKernelGGL((cached_attention4_kernel<T, QT, kWaves, RW, true, ONCE>),
+                     dim3((unsigned)p.workers), block, 0, st, a);
+  SS_CHECK_LAUNCH("cached_attention4_kernel");
+  const int64_t rows = (int64_t)a.max_new * a.group;
+  hipLaunchKernelGGL((cached_join_kernel<T, 16 * QT * RW>),
+                     dim3((unsigned)p.units, (unsigned)(rows < p.block_rows ? rows : p.block_rows)),
+                     dim3(256), 0, st, a);
+  SS_CHECK_LAUNCH("cached_join_kernel");
+  return SS_OK;
+}
+
+// Bytes of rows that the bounds allow from which on they are loaded past the caches (nt), as over
+// a 16-bit cache.
+constexpr int64_t kOnceBytes = (int64_t)32 << 20;
+
+template <class T>
+int launch4(const CachedAttnArgs& a, const Layout& p, hipStream_t st) {
+  if (a.sequences == 0) {
+    hipLaunchKernelGGL(cached_zeros_kernel, dim3((unsigned)cdiv(a.tokens * a.hq, 16)), dim3(256), 0,
+                       st, a);
+    SS_CHECK_LAUNCH("cached_zeros_kernel");
+    return SS_OK;
+  }
+  if (p.block_rows > 32)
+    return p.block_rows == 64 ? launch_attention4<T, 2, 2, false>(a, p, st)
+                              : launch_attention4<T, 2, 4, false>(a, p, st);
+  int64_t keys = a.max_length;
+  if (a.window && a.window < keys && a.sinks < keys)
+    keys = std::min(keys, a.window + a.sinks + a.max_new);
+  const bool once = keys >= kOnceBytes * kGroupRows / kGroupBytes /
+                                ((int64_t)a.sequences * a.cache.kv_heads);
+  if (p.block_rows == 16)
+    return once ? launch_attention4<T, 1, 1, true>(a, p, st)
+                : launch_attention4<T, 1, 1, false>(a, p, st);
+  return once ? launch_attention4<T, 2, 1, true>(a, p, st)
+              : launch_attention4<T, 2, 1, false>(a, p, st);
+}
+
+}  // namespace
+}  // namespace ss
+
+extern "C" size_t ss_cached_attention4_workspace_size(int rows, int64_t tokens, int q_heads,
+                                                      int kv_heads, int max_new,
+                                                      int64_t max_length) {
+  if (rows <= 0 || tokens <= 0 || q_heads <= 0 || kv_heads <= 0 || max_new < 0 ||
+      max_length < 0 || q_heads % kv_heads)
+    return 0;
+  return ss::Layout(rows, tokens, q_heads, kv_heads, max_new, max_length, false).bytes;
+}
+
+extern "C" int ss_cached_attention4(const ss_paged_cache4* cache, const void* q, int64_t q_tok,
+                                    int64_t q_head, int q_heads, const int32_t* table,
+                                    int64_t table_stride, int row_pages, const int32_t* lengths,
+                                    const int32_t* cu_seqlens, int rows, int64_t tokens,
+                                    int max_new, int64_t max_length, float scale, int64_t window,
+                                    int64_t sinks, void* o, int64_t o_tok, int64_t o_head,
+                                    void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace ss;
+  const char* who = "ss_cached_attention4";
+  if (const int rc = check_cache(who, cache)) return rc;
+  if (const int rc = check_table(who, cache, table, table_stride, row_pages, lengths, rows))
+    return rc;
+  SS_CHECK_ARG(tokens >= 0 && max_new >= 0 && max_length >= 0, "%s: negative size", who);
+  SS_CHECK_ARG(window >= 0 && sinks >= 0, "%s: negative window or sinks", who);
+  SS_CHECK_ARG(q_heads > 0 && q_heads % cache->kv_heads == 0,
+               "%s: %d q heads are no multiple of %d kv heads", who, q_heads, cache->kv_heads);
+  if (tokens == 0) return SS_OK;
+  SS_CHECK_ARG((rows == 0 || cu_seqlens) && q && o, "%s: null pointer", who);
+  SS_CHECK_ARG(aligned16(q) && aligned16(o) && ((q_tok | q_head | o_tok | o_head) & 7) == 0,
+               "%s: needs 16-byte aligned bases and strides that are multiples of 8", who);
+  SS_CHECK_ARG(max_new > 0, "%s: tokens, but max_new is 0", who);
+  const Layout p(rows, tokens, q_heads, cache->kv_heads, max_new, max_length, false);
+  SS_CHECK_ARG(tokens <= (int64_t)INT32_MAX / q_heads && p.units <= kMaxGrid / 4,
+               "%s: too many tokens in one call", who);
+  const size_t need = ss_cached_attention4_workspace_size(rows, tokens, q_heads, cache->kv_heads,
+                                                          max_new, max_length);
+  SS_CHECK_ARG(need <= workspace_bytes && (need == 0 || (workspace && aligned16(workspace))),
+               "%s: workspace of %zu bytes, needs %zu", who, workspace_bytes, need);
+  char* ws = (char*)workspace;
+  CachedAttnArgs a{cache_view(cache), TableView{table, table_stride, row_pages, lengths},
+                   cu_seqlens, rows, tokens, max_length, (const char*)q, q_tok * 2, q_head * 2,
+                   (char*)o, o_tok * 2, o_head * 2, q_heads, q_heads / cache->kv_heads,
+                   scale == 0.f ? 1.f : fabsf(scale) * kLog2e,
+                   scale < 0.f ? -1.f : scale == 0.f ? 0.f : 1.f, window, sinks, nullptr, nullptr,
+                   nullptr, p.max_new, p.blocks, p.workers, (int4*)(ws + p.list),
+                   (float*)(ws + p.ml), (float*)(ws + p.o), nullptr, 0, p.score_keys};
+  const hipStream_t st = (hipStream_t)stream;
+  return cache->dtype == SS_F16 ? launch4<half_t>(a, p, st) : launch4<bhalf_t>(a, p, st);
+}

@@ -75,8 +75,9 @@ inline int check_cache(const char* who, const ss_paged_cache* c) {
   return SS_OK;
 }
 
-inline int check_table(const char* who, const ss_paged_cache* c, const int32_t* table,
-                       int64_t stride, int row_pages, const int32_t* lengths, int rows) {
+template <class Cache>
+int check_table(const char* who, const Cache* c, const int32_t* table, int64_t stride,
+                int row_pages, const int32_t* lengths, int rows) {
   SS_CHECK_ARG(rows >= 0 && row_pages > 0 && stride >= row_pages,
                "%s: bad block table sizes (rows %d, pages a row %d, stride %lld)", who, rows,
                row_pages, (long long)stride);

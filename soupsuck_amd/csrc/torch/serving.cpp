@@ -10,6 +10,8 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
+#include <cstddef>
+#include <cstring>
 
 #include "calls.h"
 
@@ -99,12 +101,35 @@ bool packed(const Tensor& t, int64_t heads) {
          !t.requires_grad() && strided(t);
 }
 
-py::object append_kv(int64_t cache_pointer, const Tensor& pages, py::handle k_arg,
+// A cache by its struct's address: of 16 bits, or of 4 (whose memory is bytes).
+struct Cache {
+  const ss_paged_cache* wide = nullptr;
+  const ss_paged_cache4* four = nullptr;
+  int kv_heads, page_size;
+  at::ScalarType dtype;
+  Cache(int64_t pointer, bool is_four) {
+    if (is_four) {
+      four = reinterpret_cast<const ss_paged_cache4*>(pointer);
+      set(*four);
+    } else {
+      wide = reinterpret_cast<const ss_paged_cache*>(pointer);
+      set(*wide);
+    }
+  }
+  template <class C>
+  void set(const C& c) {
+    kv_heads = c.kv_heads;
+    page_size = c.page_size;
+    dtype = c.dtype == SS_F16 ? at::kHalf : at::kBFloat16;
+  }
+};
+
+py::object append_kv(int64_t cache_pointer, const Tensor& pages, bool is_four, py::handle k_arg,
                      py::handle v_arg, py::handle table_arg, py::handle lengths_arg,
                      py::handle cu_arg, py::handle q_arg, py::handle cos_arg,
                      py::handle sin_arg) {
-  const auto* cache = reinterpret_cast<const ss_paged_cache*>(cache_pointer);
-  const at::ScalarType dtype = pages.scalar_type();
+  const Cache cache(cache_pointer, is_four);
+  const at::ScalarType dtype = cache.dtype;
   Checked c(pages);
   const Table rows(c, table_arg, lengths_arg);
   const Tensor cu = c.take(cu_arg, at::kInt, 1);
@@ -120,8 +145,8 @@ py::object append_kv(int64_t cache_pointer, const Tensor& pages, py::handle k_ar
   auto turns = [&](const Tensor& t) {
     return t.size(0) == tokens && t.size(1) == kHeadDim && strided(t);
   };
-  if (!(cu.size(0) == rows.rows + 1 && cu.is_contiguous() && packed(k, cache->kv_heads) &&
-        packed(v, cache->kv_heads) && v.size(0) == tokens && cos.defined() == sin.defined() &&
+  if (!(cu.size(0) == rows.rows + 1 && cu.is_contiguous() && packed(k, cache.kv_heads) &&
+        packed(v, cache.kv_heads) && v.size(0) == tokens && cos.defined() == sin.defined() &&
         (!cos.defined() || (turns(cos) && turns(sin))) &&
         (!q.defined() || (cos.defined() && packed(q, -1) && q.size(0) == tokens && q.size(1) > 0))))
     return py::none();
@@ -131,30 +156,34 @@ py::object append_kv(int64_t cache_pointer, const Tensor& pages, py::handle k_ar
     c10::DeviceGuard guard(pages.device());
     if (q.defined()) out = at::empty(q.sizes(), q.options());
     const bool turned = cos.defined(), queries = q.defined();
-    check(ss_kv_append(cache, ptr<void>(k), k.stride(0), k.stride(1), ptr<void>(v), v.stride(0),
-                       v.stride(1), ptr<void>(q), queries ? q.stride(0) : 0,
-                       queries ? q.stride(1) : 0, queries ? (int)q.size(1) : 0, ptr<void>(cos),
-                       turned ? cos.stride(0) : 0, ptr<void>(sin), turned ? sin.stride(0) : 0,
-                       turned ? code_of(cos) : SS_F32, ptr<int32_t>(rows.table), rows.stride,
-                       (int)rows.width, ptr<int32_t>(rows.lengths), ptr<int32_t>(cu),
-                       (int)rows.rows, tokens, ptr<void>(out), queries ? out.stride(0) : 0,
-                       queries ? out.stride(1) : 0, stream_of(pages)),
-          "ss_kv_append");
+    auto append = [&](auto* call, const auto* to, const char* name) {
+      check(call(to, ptr<void>(k), k.stride(0), k.stride(1), ptr<void>(v), v.stride(0),
+                         v.stride(1), ptr<void>(q), queries ? q.stride(0) : 0,
+                         queries ? q.stride(1) : 0, queries ? (int)q.size(1) : 0, ptr<void>(cos),
+                         turned ? cos.stride(0) : 0, ptr<void>(sin), turned ? sin.stride(0) : 0,
+                         turned ? code_of(cos) : SS_F32, ptr<int32_t>(rows.table), rows.stride,
+                         (int)rows.width, ptr<int32_t>(rows.lengths), ptr<int32_t>(cu),
+                         (int)rows.rows, tokens, ptr<void>(out), queries ? out.stride(0) : 0,
+                         queries ? out.stride(1) : 0, stream_of(pages)),
+            name);
+    };
+    if (is_four) append(&ss_kv_append4, cache.four, "ss_kv_append4");
+    else append(&ss_kv_append, cache.wide, "ss_kv_append");
   }
   return q.defined() ? py::cast(out) : py::bool_(true);
 }
 
-bool weights_fit(const Tensor& t, const Table& rows, const ss_paged_cache* cache) {
-  return t.size(0) == rows.rows && t.size(1) == cache->kv_heads &&
-         t.size(2) == rows.width * cache->page_size && t.is_contiguous();
+bool weights_fit(const Tensor& t, const Table& rows, int kv_heads, int page_size) {
+  return t.size(0) == rows.rows && t.size(1) == kv_heads &&
+         t.size(2) == rows.width * page_size && t.is_contiguous();
 }
 
-py::object cached_attention(int64_t cache_pointer, const Tensor& pages, py::handle q_arg,
+py::object cached_attention(int64_t cache_pointer, const Tensor& pages, bool is_four, py::handle q_arg,
                             py::handle table_arg, py::handle lengths_arg, py::handle cu_arg,
                             py::handle max_new_arg, py::handle max_length_arg,
                             py::handle scale_arg, py::handle window_arg, py::handle sinks_arg,
                             py::handle weights_arg, py::handle weights_out_arg) {
-  const auto* cache = reinterpret_cast<const ss_paged_cache*>(cache_pointer);
+  const Cache cache(cache_pointer, is_four);
   int64_t max_new, max_length, window = 0, sinks;
   double scale;
   if (!whole(max_new_arg, 1, (int64_t)1 << 31, &max_new) ||
@@ -165,33 +194,47 @@ py::object cached_attention(int64_t cache_pointer, const Tensor& pages, py::hand
   Checked c(pages);
   const Table rows(c, table_arg, lengths_arg);
   const Tensor cu = c.take(cu_arg, at::kInt, 1);
-  const Tensor q = c.take(q_arg, pages.scalar_type(), 3);
+  const Tensor q = c.take(q_arg, cache.dtype, 3);
   const Tensor weights = c.take_or_none(weights_arg, at::kFloat, 3);
   const Tensor weights_out = c.take_or_none(weights_out_arg, at::kFloat, 3);
   if (!c.ok) return py::none();
   const int64_t tokens = q.size(0), heads = q.size(1);
   if (!(cu.size(0) == rows.rows + 1 && cu.is_contiguous() && packed(q, -1) && heads > 0 &&
-        heads % cache->kv_heads == 0 && heads < INT32_MAX &&
-        (!weights.defined() || (weights_out.defined() && weights_fit(weights, rows, cache))) &&
-        (!weights_out.defined() || weights_fit(weights_out, rows, cache))))
+        heads % cache.kv_heads == 0 && heads < INT32_MAX &&
+        (!weights.defined() || (weights_out.defined() && weights_fit(weights, rows, cache.kv_heads, cache.page_size))) &&
+        (!weights_out.defined() || !is_four) &&
+        (!weights_out.defined() || weights_fit(weights_out, rows, cache.kv_heads, cache.page_size))))
     return py::none();
   Tensor out;
   {
     py::gil_scoped_release unlocked;
     c10::DeviceGuard guard(pages.device());
     out = at::empty(q.sizes(), q.options());
-    const size_t size = ss_cached_attention_workspace_size(
-        (int)rows.rows, tokens, (int)heads, cache->kv_heads, (int)max_new, max_length,
-        weights_out.defined());
-    const Tensor scratch = workspace(size, q);
-    check(ss_cached_attention(cache, ptr<void>(q), q.stride(0), q.stride(1), (int)heads,
-                              ptr<int32_t>(rows.table), rows.stride, (int)rows.width,
-                              ptr<int32_t>(rows.lengths), ptr<int32_t>(cu), (int)rows.rows,
-                              tokens, (int)max_new, max_length, (float)scale, window, sinks,
-                              ptr<float>(weights), ptr<float>(weights_out), ptr<void>(out),
-                              out.stride(0), out.stride(1), ptr<void>(scratch), size,
-                              stream_of(pages)),
-          "ss_cached_attention");
+    if (is_four) {
+      const size_t size = ss_cached_attention4_workspace_size(
+          (int)rows.rows, tokens, (int)heads, cache.kv_heads, (int)max_new, max_length);
+      const Tensor scratch = workspace(size, q);
+      check(ss_cached_attention4(cache.four, ptr<void>(q), q.stride(0), q.stride(1), (int)heads,
+                                 ptr<int32_t>(rows.table), rows.stride, (int)rows.width,
+                                 ptr<int32_t>(rows.lengths), ptr<int32_t>(cu), (int)rows.rows,
+                                 tokens, (int)max_new, max_length, (float)scale, window, sinks,
+                                 ptr<void>(out), out.stride(0), out.stride(1),
+                                 ptr<void>(scratch), size, stream_of(pages)),
+            "ss_cached_attention4");
+    } else {
+      const size_t size = ss_cached_attention_workspace_size(
+          (int)rows.rows, tokens, (int)heads, cache.kv_heads, (int)max_new, max_length,
+          weights_out.defined());
+      const Tensor scratch = workspace(size, q);
+      check(ss_cached_attention(cache.wide, ptr<void>(q), q.stride(0), q.stride(1), (int)heads,
+                                ptr<int32_t>(rows.table), rows.stride, (int)rows.width,
+                                ptr<int32_t>(rows.lengths), ptr<int32_t>(cu), (int)rows.rows,
+                                tokens, (int)max_new, max_length, (float)scale, window, sinks,
+                                ptr<float>(weights), ptr<float>(weights_out), ptr<void>(out),
+                                out.stride(0), out.stride(1), ptr<void>(scratch), size,
+                                stream_of(pages)),
+            "ss_cached_attention");
+    }
   }
   return py::cast(out);
 }
@@ -212,7 +255,7 @@ py::object evict_kv(int64_t cache_pointer, const Tensor& pages, py::handle table
   const Table out(c, out_table_arg, lengths_arg);
   const Tensor weights = c.take(weights_arg, at::kFloat, 3);
   if (!c.ok || out.rows != rows.rows || budget > out.width * cache->page_size ||
-      !weights_fit(weights, rows, cache))
+      !weights_fit(weights, rows, cache->kv_heads, cache->page_size))
     return py::none();
   Tensor out_lengths, out_weights;
   {
@@ -231,6 +274,133 @@ py::object evict_kv(int64_t cache_pointer, const Tensor& pages, py::handle table
           "ss_kv_evict");
   }
   return py::make_tuple(out_lengths, out_weights);
+}
+
+// The caches of a call: alike, on one device, by their structs' addresses.
+struct Caches {
+  std::vector<int64_t> pointers;
+  bool ok = true;
+  Caches(const py::list& addresses, const py::list& memory, bool is_four, const Tensor& first) {
+    for (size_t i = 0; i < addresses.size(); ++i) {
+      pointers.push_back(addresses[i].cast<int64_t>());
+      const Argument pages(memory[i]);
+      ok = ok && pages.ok && pages.t.defined() && pages.t.device() == first.device();
+      if (is_four) same<ss_paged_cache4>(offsetof(ss_paged_cache4, page), i);
+      else same<ss_paged_cache>(offsetof(ss_paged_cache, k_page), i);
+    }
+    ok = ok && !pointers.empty();
+  }
+  // Everything but the bases (the C entries compare the strides of v).
+  template <class C>
+  void same(size_t from, size_t i) {
+    const auto *a = reinterpret_cast<const C*>(pointers[0]),
+               *b = reinterpret_cast<const C*>(pointers[i]);
+    ok = ok && a->pages == b->pages && a->page_size == b->page_size &&
+         a->kv_heads == b->kv_heads && a->dtype == b->dtype &&
+         !memcmp((const char*)a + from, (const char*)b + from, 3 * sizeof(int64_t));
+  }
+  template <class C>
+  const C* const* all() const {
+    return reinterpret_cast<const C* const*>(pointers.data());
+  }
+  int count() const { return (int)pointers.size(); }
+};
+
+py::object read_kv(const py::list& addresses, const Tensor& pages, bool is_four,
+                   const py::list& memory, py::handle table_arg, py::handle lengths_arg,
+                   py::handle cu_arg, py::handle tokens_arg, bool several) {
+  int64_t tokens;
+  const Caches caches(addresses, memory, is_four, pages);
+  if (!caches.ok || !whole(tokens_arg, 1, (int64_t)1 << 31, &tokens)) return py::none();
+  const Cache cache(caches.pointers[0], is_four);
+  Checked c(pages);
+  const Table rows(c, table_arg, lengths_arg);
+  const Tensor cu = c.take(cu_arg, at::kInt, 1);
+  if (!c.ok || cu.size(0) != rows.rows + 1 || !cu.is_contiguous()) return py::none();
+  Tensor k, v;
+  {
+    py::gil_scoped_release unlocked;
+    c10::DeviceGuard guard(pages.device());
+    k = several ? empty({caches.count(), tokens, cache.kv_heads, kHeadDim}, pages, cache.dtype)
+                : empty({tokens, cache.kv_heads, kHeadDim}, pages, cache.dtype);
+    v = at::empty_like(k);
+    auto read = [&](auto* call, auto* const* all, const char* name) {
+      check(call(all, caches.count(), ptr<int32_t>(rows.table), rows.stride, (int)rows.width,
+                 ptr<int32_t>(rows.lengths), ptr<int32_t>(cu), (int)rows.rows, tokens,
+                 ptr<void>(k), ptr<void>(v), stream_of(pages)),
+            name);
+    };
+    if (is_four) read(&ss_kv_read4, caches.all<ss_paged_cache4>(), "ss_kv_read4");
+    else read(&ss_kv_read, caches.all<ss_paged_cache>(), "ss_kv_read");
+  }
+  return py::make_tuple(k, v);
+}
+
+py::object fork_kv(const py::list& addresses, const Tensor& pages, bool is_four,
+                   const py::list& memory, py::handle table_arg, py::handle lengths_arg,
+                   py::handle parents_arg, py::handle spare_arg) {
+  const Caches caches(addresses, memory, is_four, pages);
+  if (!caches.ok) return py::none();
+  Checked c(pages);
+  const Table rows(c, table_arg, lengths_arg);
+  const Tensor parents = c.take(parents_arg, at::kInt, 1), spare = c.take(spare_arg, at::kInt, 1);
+  if (!c.ok || parents.size(0) == 0 || parents.size(0) >= INT32_MAX ||
+      spare.size(0) != parents.size(0) || !parents.is_contiguous() || !spare.is_contiguous())
+    return py::none();
+  Tensor table, lengths;
+  {
+    py::gil_scoped_release unlocked;
+    c10::DeviceGuard guard(pages.device());
+    table = empty({parents.size(0), rows.width}, parents, at::kInt);
+    lengths = empty({parents.size(0)}, parents, at::kInt);
+    auto fork = [&](auto* call, auto* const* all, const char* name) {
+      check(call(all, caches.count(), ptr<int32_t>(rows.table), rows.stride, (int)rows.width,
+                 ptr<int32_t>(rows.lengths), (int)rows.rows, ptr<int32_t>(parents),
+                 ptr<int32_t>(spare), (int)parents.size(0), ptr<int32_t>(table),
+                 ptr<int32_t>(lengths), stream_of(pages)),
+            name);
+    };
+    if (is_four) fork(&ss_kv_fork4, caches.all<ss_paged_cache4>(), "ss_kv_fork4");
+    else fork(&ss_kv_fork, caches.all<ss_paged_cache>(), "ss_kv_fork");
+  }
+  return py::make_tuple(table, lengths);
+}
+
+py::object select_beams(py::handle logits_arg, py::handle scores_arg, py::handle count_arg) {
+  int64_t count;
+  const Argument first(logits_arg);
+  if (!first.ok || !first.t.defined() || first.t.dim() != 3 || first.t.requires_grad() ||
+      !whole(count_arg, 1, 65, &count))
+    return py::none();
+  const Tensor& logits = first.t;
+  const at::ScalarType dtype = logits.scalar_type();
+  if (dtype != at::kHalf && dtype != at::kBFloat16 && dtype != at::kFloat) return py::none();
+  Checked c(logits);
+  const Tensor scores = c.take(scores_arg, at::kFloat, 2);
+  if (!c.ok) return py::none();
+  const int64_t rows = logits.size(0), beams = logits.size(1), vocab = logits.size(2);
+  if (!(rows > 0 && rows <= 65535 && beams > 0 && beams <= 64 && vocab > 0 &&
+        vocab < INT32_MAX - 65536 && count <= beams * vocab && beams * count <= 2048 &&
+        (logits.stride(2) == 1 || vocab == 1) && scores.size(0) == rows &&
+        scores.size(1) == beams && scores.is_contiguous()))
+    return py::none();
+  Tensor out, parents, tokens;
+  {
+    py::gil_scoped_release unlocked;
+    c10::DeviceGuard guard(logits.device());
+    out = empty({rows, count}, logits, at::kFloat);
+    parents = empty({rows, count}, logits, at::kInt);
+    tokens = empty({rows, count}, logits, at::kLong);
+    const size_t size = ss_select_beams_workspace_size((int)rows, (int)beams, vocab, (int)count,
+                                                       code_of(logits));
+    const Tensor scratch = workspace(size, logits);
+    check(ss_select_beams(ptr<void>(logits), logits.stride(0), logits.stride(1), code_of(logits),
+                          ptr<float>(scores), (int)rows, (int)beams, vocab, (int)count,
+                          ptr<float>(out), ptr<int32_t>(parents), ptr<int64_t>(tokens),
+                          ptr<void>(scratch), size, stream_of(logits)),
+          "ss_select_beams");
+  }
+  return py::make_tuple(out, parents, tokens);
 }
 
 py::object verify_drafts(py::handle target_arg, py::handle tokens_arg, py::handle uniform_arg,
@@ -287,5 +457,8 @@ void define_serving(py::module_& m) {
   m.def("append_kv", &append_kv);
   m.def("cached_attention", &cached_attention);
   m.def("evict_kv", &evict_kv);
+  m.def("read_kv", &read_kv);
+  m.def("fork_kv", &fork_kv);
+  m.def("select_beams", &select_beams);
   m.def("verify_drafts", &verify_drafts);
 }

@@ -1,4 +1,4 @@
-"""Paged key-value cache: append, attention of new tokens, eviction (fp16 / bf16).
+"""Paged key-value cache: append, attention of new tokens, eviction, beams (16 or 4 bits).
 
 What generation with the tuned projections needs beside them; the reference trains only
 and has no counterpart.  Keys and values lie in pages ([pages, kv heads, page size, 128]); a
@@ -13,6 +13,14 @@ last cache rows: ``lengths`` counts them in.
                          weights=weights, weights_out=weights)
     lengths, weights = evict_kv(cache, block_table, lengths, weights, fresh, budget, max_length,
                                 sinks=4, recent=256)
+
+``PagedCache4`` holds the rows in 4 bits a value (136 bytes a row and head instead of 512) and
+stands wherever a ``PagedCache`` does, except in ``evict_kv`` and for attention weights.
+``read_kv`` gives rows back as a cache holds them.  ``fork_kv`` lets sequences continue others,
+as beams do (``kernels.beams.select_beams`` chooses them):
+
+    scores, parents, tokens = select_beams(logits, scores, beams)
+    table, lengths = fork_kv(caches, table, lengths, row_of(parents), spare_pages)
 
 Block tables, lengths and offsets are read on the device: no call waits for it, and all
 of them can be captured into a graph whose replays see the lengths of the moment
@@ -59,7 +67,7 @@ CACHE_RULES = (
 
 
 class PagedCache:
-    """Pages of keys and values: the tensors ``k`` and ``v`` [pages, kv_heads, page_size, 128]."""
+    """Pages of 16-bit keys and values: the tensors ``k`` and ``v`` [pages, kv_heads, page_size, 128]."""
 
     def __init__(self, k, v):
         enforce(CACHE_RULES, k=k, v=v)
@@ -86,8 +94,83 @@ class PagedCache:
         return self._v
 
     @property
+    def dtype(self):
+        return self._k.dtype
+
+    @property
+    def device(self):
+        return self._k.device
+
+    @property
+    def kv_heads(self):
+        return self._k.shape[1]
+
+    @property
     def page_size(self):
         return self._k.shape[2]
+
+
+GROUP_BYTES = 2176  # of 16 rows: key codes, value codes, key scales, value scales
+
+
+CACHE4_RULES = (
+    Rule("PagedCache4: data must be a uint8 [pages, kv_heads, page_size / 16, 2176] tensor",
+         lambda a: isinstance(a.data, torch.Tensor) and a.data.dtype == torch.uint8
+         and a.data.ndim == 4 and a.data.shape[3] == GROUP_BYTES),
+    Rule("PagedCache4: dtype must be torch.float16 or torch.bfloat16",
+         lambda a: a.dtype in (torch.float16, torch.bfloat16)),
+    Rule("PagedCache4: needs at least one page and head and a page size that is a multiple of 16",
+         lambda a: all(n > 0 for n in a.data.shape[:3])),
+    Rule("PagedCache4: data needs a 16-byte aligned base, a unit last stride and strides that "
+         "are multiples of 16", lambda a: _strided(a.data)),
+)
+
+
+class PagedCache4:
+    """Pages of keys and values in 4 bits: the bytes ``data`` [pages, kv_heads, page_size / 16, 2176].
+
+    Every 32 values of a row share a scale 2^e; a value is one of 0, 0.5, 1, 1.5, 2, 3, 4, 6 times
+    it, with a sign.  e is the least with which none is past 6 (-13 to 13 for fp16, -125 to 125
+    for bf16: beyond, values are held as 6 2^e); rounding is to nearest even.  A block with an
+    infinity or NaN reads as NaN.  ``dtype`` is the type of the tensors around the cache; the
+    bytes' layout is in include/soupsuck_amd.h.
+    """
+
+    def __init__(self, data, dtype=torch.float16):
+        enforce(CACHE4_RULES, data=data, dtype=dtype)
+        self._data, self._dtype = data, dtype
+        pages, heads, groups, _ = data.shape
+        self._struct = _lib.PagedCache4Struct(data.data_ptr(), *data.stride()[:3], pages,
+                                              16 * groups, heads, HEAD_DIM, _CODES[dtype])
+        self._pointer = ctypes.addressof(self._struct)
+
+    @classmethod
+    def empty(cls, pages, kv_heads, page_size, dtype=torch.float16, device="cuda"):
+        """A cache of uninitialised pages (``page_size`` a multiple of 16)."""
+        if not _whole(page_size, 16) or page_size % 16:
+            raise ValueError("PagedCache4: page_size must be a multiple of 16")
+        return cls(torch.empty((pages, kv_heads, page_size // 16, GROUP_BYTES), dtype=torch.uint8,
+                               device=device), dtype)
+
+    @property
+    def data(self):
+        return self._data
+
+    @property
+    def dtype(self):
+        return self._dtype
+
+    @property
+    def device(self):
+        return self._data.device
+
+    @property
+    def kv_heads(self):
+        return self._data.shape[1]
+
+    @property
+    def page_size(self):
+        return 16 * self._data.shape[2]
 
 
 def _table(t):
@@ -107,7 +190,7 @@ def _int32_line(t, n):
 
 
 def _packed(t, cache, heads=None):
-    return (isinstance(t, torch.Tensor) and t.ndim == 3 and t.dtype == cache.k.dtype
+    return (isinstance(t, torch.Tensor) and t.ndim == 3 and t.dtype == cache.dtype
             and t.shape[2] == HEAD_DIM and (heads is None or t.shape[1] == heads)
             and not t.requires_grad)
 
@@ -116,9 +199,18 @@ def _is_cache(cache):
     return isinstance(cache, PagedCache)
 
 
-def _rows_rules(name, with_offsets=True):
+def _is_cache4(cache):
+    return isinstance(cache, PagedCache4)
+
+
+def _any_cache(name):
+    return Rule(f"{name}: cache must be a PagedCache or a PagedCache4",
+                lambda a: _is_cache(a.cache) or _is_cache4(a.cache))
+
+
+def _rows_rules(name, with_offsets=True, cache_rule=None):
     rules = [
-        Rule(f"{name}: cache must be a PagedCache", lambda a: _is_cache(a.cache)),
+        cache_rule or _any_cache(name),
         Rule(f"{name}: block_table must be int32 [rows, pages a row] with a unit last stride",
              lambda a: _table(a.block_table)),
         Rule(f"{name}: lengths must be a contiguous int32 [rows]",
@@ -132,15 +224,20 @@ def _rows_rules(name, with_offsets=True):
 
 def _one_device(name):
     return Rule(f"{name}: all tensors must be CUDA tensors on the cache's device",
-                lambda a: a.cache.k.is_cuda and all(t is None or t.device == a.cache.k.device
-                                                    for t in a.tensors))
+                lambda a: a.cache.device.type == "cuda"
+                and all(t is None or t.device == a.cache.device for t in a.tensors))
+
+
+def _pages(cache):
+    """A tensor of the cache's memory."""
+    return cache._data if _is_cache4(cache) else cache._k
 
 
 APPEND_RULES = (
     *_rows_rules("append_kv"),
     Rule("append_kv: k and v must be [tokens, kv_heads, 128] of the cache's type, without "
-         "gradients", lambda a: _packed(a.k, a.cache, a.cache.k.shape[1])
-         and _packed(a.v, a.cache, a.cache.k.shape[1]) and a.k.shape[0] == a.v.shape[0]),
+         "gradients", lambda a: _packed(a.k, a.cache, a.cache.kv_heads)
+         and _packed(a.v, a.cache, a.cache.kv_heads) and a.k.shape[0] == a.v.shape[0]),
     Rule("append_kv: cos and sin go together, q only with them",
          lambda a: (a.cos is None) == (a.sin is None) and (a.q is None or a.cos is not None)),
     Rule("append_kv: q must be [tokens, q_heads, 128] of the cache's type, without gradients",
@@ -149,7 +246,7 @@ APPEND_RULES = (
     Rule("append_kv: cos and sin must be [tokens, 128], both of the cache's type or both fp32",
          lambda a: a.cos is None or all(
              isinstance(t, torch.Tensor) and t.shape == (a.k.shape[0], HEAD_DIM)
-             and t.dtype == a.cos.dtype and t.dtype in (a.cache.k.dtype, torch.float32)
+             and t.dtype == a.cos.dtype and t.dtype in (a.cache.dtype, torch.float32)
              for t in (a.cos, a.sin))),
     Rule("append_kv: q / k / v / cos / sin need 16-byte aligned bases, a unit last stride and "
          "strides that are multiples of 16 bytes",
@@ -164,12 +261,13 @@ def append_kv(cache, k, v, block_table, lengths, cu_seqlens, q=None, cos=None, s
 
     With ``cos`` / ``sin`` [T, 128] (a token's angles, as the model's rotary embedding gives
     them) k is rotated on its way and ``q`` [T, q_heads, 128] is rotated too: returns the
-    rotated q (None without q).  A token whose row the sequence does not hold is skipped.
+    rotated q (None without q).  A token whose row the sequence does not hold is skipped.  A 4-bit
+    cache takes its codes from the rotated key before any rounding (see ``read_kv``).
     """
-    nodes = native.nodes() if _is_cache(cache) else None
+    nodes = native.nodes() if _is_cache(cache) or _is_cache4(cache) else None
     if nodes is not None:
-        got = nodes.append_kv(cache._pointer, cache._k, k, v, block_table, lengths, cu_seqlens, q,
-                              cos, sin)
+        got = nodes.append_kv(cache._pointer, _pages(cache), _is_cache4(cache), k, v, block_table,
+                              lengths, cu_seqlens, q, cos, sin)
         if got is not None:
             return got if q is not None else None
     enforce(APPEND_RULES, cache=cache, k=k, v=v, block_table=block_table, lengths=lengths,
@@ -181,7 +279,7 @@ def append_kv(cache, k, v, block_table, lengths, cu_seqlens, q=None, cos=None, s
         return out
     device = k.device
     with torch.cuda.device(device):
-        _lib.call("ss_kv_append", cache._pointer, k.data_ptr(), k.stride(0), k.stride(1),
+        _lib.call("ss_kv_append4" if _is_cache4(cache) else "ss_kv_append", cache._pointer, k.data_ptr(), k.stride(0), k.stride(1),
                   v.data_ptr(), v.stride(0), v.stride(1),
                   *((None, 0, 0, 0) if q is None
                     else (q.data_ptr(), q.stride(0), q.stride(1), q.shape[1])),
@@ -198,7 +296,7 @@ def append_kv(cache, k, v, block_table, lengths, cu_seqlens, q=None, cos=None, s
 
 def _weights(t, table, cache):
     return (isinstance(t, torch.Tensor) and t.dtype == torch.float32 and t.is_contiguous()
-            and t.shape == (table.shape[0], cache.k.shape[1], table.shape[1] * cache.page_size))
+            and t.shape == (table.shape[0], cache.kv_heads, table.shape[1] * cache.page_size))
 
 
 ATTENTION_RULES = (
@@ -206,7 +304,7 @@ ATTENTION_RULES = (
     Rule("cached_attention: q must be [tokens, q_heads, 128] of the cache's type, without "
          "gradients", lambda a: _packed(a.q, a.cache)),
     Rule("cached_attention: q_heads must be a multiple of the cache's heads",
-         lambda a: a.q.shape[1] > 0 and a.q.shape[1] % a.cache.k.shape[1] == 0),
+         lambda a: a.q.shape[1] > 0 and a.q.shape[1] % a.cache.kv_heads == 0),
     Rule("cached_attention: q needs a 16-byte aligned base, a unit last stride and strides that "
          "are multiples of 8", lambda a: a.q.shape[0] == 0 or _strided(a.q)),
     Rule("cached_attention: max_new and max_length must be whole numbers, max_new from 1 up where "
@@ -222,6 +320,8 @@ ATTENTION_RULES = (
          lambda a: all(t is None or _weights(t, a.block_table, a.cache)
                        for t in (a.weights, a.weights_out))
          and (a.weights is None or a.weights_out is not None)),
+    Rule("cached_attention: a 4-bit cache gives no weights",
+         lambda a: _is_cache(a.cache) or a.weights_out is None),
     _one_device("cached_attention"),
 )
 
@@ -238,13 +338,14 @@ def cached_attention(q, cache, block_table, lengths, cu_seqlens, max_new, max_le
     zeros; may be the same tensor) plus every cache row's attention weight, summed over the new tokens
     and the q heads of its kv head: what ``evict_kv`` ranks by.  All of the call's tokens count. Drafted
     ones that may yet be refused are better left out: ask for the weights of the accepted ones in
-    a call of their own (their queries, ``lengths`` and offsets without the refused).
+    a call of their own (their queries, ``lengths`` and offsets without the refused).  A 4-bit
+    cache gives none.
     """
-    nodes = native.nodes() if _is_cache(cache) else None
+    nodes = native.nodes() if _is_cache(cache) or _is_cache4(cache) else None
     if nodes is not None:
-        got = nodes.cached_attention(cache._pointer, cache._k, q, block_table, lengths, cu_seqlens,
-                                     max_new, max_length, scale, window, sinks, weights,
-                                     weights_out)
+        got = nodes.cached_attention(cache._pointer, _pages(cache), _is_cache4(cache), q,
+                                     block_table, lengths, cu_seqlens, max_new, max_length, scale,
+                                     window, sinks, weights, weights_out)
         if got is not None:
             return got
     enforce(ATTENTION_RULES, q=q, cache=cache, block_table=block_table, lengths=lengths,
@@ -255,21 +356,26 @@ def cached_attention(q, cache, block_table, lengths, cu_seqlens, max_new, max_le
     device = q.device
     out = torch.empty(q.shape, dtype=q.dtype, device=device)
     rows = block_table.shape[0]
-    size = _lib.load().ss_cached_attention_workspace_size(
-        rows, tokens, heads, cache.k.shape[1], max_new, max_length, weights_out is not None)
+    four = _is_cache4(cache)
+    size = (_lib.load().ss_cached_attention4_workspace_size(
+                rows, tokens, heads, cache.kv_heads, max_new, max_length) if four else
+            _lib.load().ss_cached_attention_workspace_size(
+                rows, tokens, heads, cache.kv_heads, max_new, max_length, weights_out is not None))
     with torch.cuda.device(device):
         scratch = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-        _lib.call("ss_cached_attention", cache._pointer, q.data_ptr(), q.stride(0), q.stride(1),
-                  heads, block_table.data_ptr(), _line_stride(block_table), block_table.shape[1],
-                  lengths.data_ptr(), cu_seqlens.data_ptr(), rows, tokens, max_new, max_length,
-                  scale, window or 0, sinks, _lib.ptr(weights), _lib.ptr(weights_out),
+        _lib.call("ss_cached_attention4" if four else "ss_cached_attention", cache._pointer,
+                  q.data_ptr(), q.stride(0), q.stride(1), heads, block_table.data_ptr(),
+                  _line_stride(block_table), block_table.shape[1], lengths.data_ptr(),
+                  cu_seqlens.data_ptr(), rows, tokens, max_new, max_length, scale, window or 0,
+                  sinks, *(() if four else (_lib.ptr(weights), _lib.ptr(weights_out))),
                   out.data_ptr(), out.stride(0), out.stride(1), _lib.ptr(scratch), size,
                   _lib.stream(device))
     return out
 
 
 EVICT_RULES = (
-    *_rows_rules("evict_kv", with_offsets=False),
+    *_rows_rules("evict_kv", with_offsets=False, cache_rule=Rule(
+        "evict_kv: cache must be a PagedCache", lambda a: _is_cache(a.cache))),
     Rule("evict_kv: weights must be contiguous fp32 [rows, kv_heads, pages a row * page_size]",
          lambda a: _weights(a.weights, a.block_table, a.cache)),
     Rule("evict_kv: out_table must be int32 [rows, pages a row] with a unit last stride",
@@ -320,3 +426,123 @@ def evict_kv(cache, block_table, lengths, weights, out_table, budget, max_length
                   out_table.shape[1], budget, sinks, recent, out_lengths.data_ptr(),
                   out_weights.data_ptr(), scratch.data_ptr(), size, _lib.stream(device))
     return out_lengths, out_weights
+
+
+def _caches(value):
+    """The caches of a call as a tuple (one cache, or a list of them), None if they are none."""
+    caches = (value,) if _is_cache(value) or _is_cache4(value) else value
+    if not isinstance(caches, (list, tuple)) or not caches:
+        return None
+    first = caches[0]
+    kind = _is_cache if _is_cache(first) else _is_cache4
+    return tuple(caches) if all(kind(c) for c in caches) else None
+
+
+def _alike(caches):
+    """One shape, strides, type and device: what a launch over all of them takes for granted."""
+    def key(c):
+        tensors = (c.data,) if _is_cache4(c) else (c.k, c.v)
+        return (c.dtype, c.device, *((t.shape, t.stride()) for t in tensors))
+
+    first = key(caches[0])
+    return all(key(c) == first for c in caches[1:])
+
+
+def _caches_rules(name):
+    return (
+        Rule(f"{name}: caches must be a PagedCache, a PagedCache4, or a list of either",
+             lambda a: a.caches is not None),
+        Rule(f"{name}: the caches must have one shape, strides, dtype and device",
+             lambda a: _alike(a.caches)),
+    )
+
+
+def _pointers(caches):
+    return (ctypes.c_void_p * len(caches))(*(c._pointer for c in caches))
+
+
+READ_RULES = (
+    *_caches_rules("read_kv"),
+    *_rows_rules("read_kv"),
+    Rule("read_kv: tokens must be a whole number", lambda a: _whole(a.tokens, 0)
+         and a.tokens < 2 ** 31),
+    _one_device("read_kv"),
+)
+
+
+def read_kv(caches, block_table, lengths, cu_seqlens, tokens):
+    """k and v [tokens, kv_heads, 128] of the sequences' last rows, as a cache holds them.
+
+    The rows are those that ``append_kv`` writes when it is given the same ``block_table``,
+    ``lengths`` and ``cu_seqlens``; offsets as long as the sequences read them whole.  With a
+    list of caches (one a layer, alike) both are [caches, tokens, kv_heads, 128].  Rows that a
+    sequence does not hold are zeros.
+    """
+    several = isinstance(caches, (list, tuple))
+    caches = _caches(caches)
+    nodes = native.nodes() if caches is not None else None
+    if nodes is not None:
+        got = nodes.read_kv([c._pointer for c in caches], _pages(caches[0]),
+                            _is_cache4(caches[0]), [_pages(c) for c in caches], block_table,
+                            lengths, cu_seqlens, tokens, several)
+        if got is not None:
+            return got
+    enforce(READ_RULES, caches=caches, cache=caches and caches[0], block_table=block_table,
+            lengths=lengths, cu_seqlens=cu_seqlens, tokens=tokens,
+            tensors=(block_table, lengths, cu_seqlens))
+    cache = caches[0]
+    shape = (len(caches), tokens, cache.kv_heads, HEAD_DIM)
+    k, v = (torch.empty(shape, dtype=cache.dtype, device=cache.device) for _ in range(2))
+    if tokens:
+        with torch.cuda.device(cache.device):
+            _lib.call("ss_kv_read4" if _is_cache4(cache) else "ss_kv_read", _pointers(caches),
+                      len(caches), block_table.data_ptr(), _line_stride(block_table),
+                      block_table.shape[1], lengths.data_ptr(), cu_seqlens.data_ptr(),
+                      block_table.shape[0], tokens, k.data_ptr(), v.data_ptr(),
+                      _lib.stream(cache.device))
+    return (k, v) if several else (k[0], v[0])
+
+
+FORK_RULES = (
+    *_caches_rules("fork_kv"),
+    *_rows_rules("fork_kv", with_offsets=False),
+    Rule("fork_kv: parents and spare must be contiguous int32 [new rows]",
+         lambda a: isinstance(a.parents, torch.Tensor) and a.parents.ndim == 1
+         and all(_int32_line(t, a.parents.shape[0]) for t in (a.parents, a.spare))),
+    _one_device("fork_kv"),
+)
+
+
+def fork_kv(caches, block_table, lengths, parents, spare):
+    """Sequences that continue others: (block table, lengths) with a row for each of ``parents``.
+
+    Row i continues row ``parents[i]`` (int32 [new rows]; any number of rows may continue
+    one, and a parent that is no row counts as an empty sequence): it shares the parent's full
+    pages, and page ``spare[i]`` becomes the one that its next tokens go to, with the
+    rows that the parent has beyond its full pages copied there in every cache of the list (one a
+    layer, alike).  The entries behind are -1.  Spare pages must be nobody's: not in
+    ``block_table`` and not named twice.  The parents' own last pages are free again once no
+    row of ``block_table`` is used further, unless they are full.
+    """
+    caches = _caches(caches)
+    nodes = native.nodes() if caches is not None else None
+    if nodes is not None:
+        got = nodes.fork_kv([c._pointer for c in caches], _pages(caches[0]),
+                            _is_cache4(caches[0]), [_pages(c) for c in caches], block_table,
+                            lengths, parents, spare)
+        if got is not None:
+            return got
+    enforce(FORK_RULES, caches=caches, cache=caches and caches[0], block_table=block_table,
+            lengths=lengths, parents=parents, spare=spare,
+            tensors=(block_table, lengths, parents, spare))
+    cache, rows = caches[0], parents.shape[0]
+    out_table = torch.empty((rows, block_table.shape[1]), dtype=torch.int32, device=cache.device)
+    out_lengths = torch.empty(rows, dtype=torch.int32, device=cache.device)
+    if rows:
+        with torch.cuda.device(cache.device):
+            _lib.call("ss_kv_fork4" if _is_cache4(cache) else "ss_kv_fork", _pointers(caches),
+                      len(caches), block_table.data_ptr(), _line_stride(block_table),
+                      block_table.shape[1], lengths.data_ptr(), block_table.shape[0],
+                      parents.data_ptr(), spare.data_ptr(), rows, out_table.data_ptr(),
+                      out_lengths.data_ptr(), _lib.stream(cache.device))
+    return out_table, out_lengths
