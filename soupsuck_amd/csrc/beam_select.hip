@@ -6,14 +6,23 @@
 // order of v is that of the logits, so no v is needed before the few that can win are
 // known, and one pass over the logits does:
 //
-// beam_slice_kernel: a workgroup holds a slice of one beam's logits in registers (at most
-// kVectors loads of 16 bytes a thread, all on their way at once), takes its maximum, the sum of
-// exp(l - maximum) and its `count` first.  Exponentials are fp32 (a difference next to the
-// maximum, where it counts, is exact or off by 2^-24), sums of them fp64: log-sums are good to
-// some 1e-8.  The first: the count-th greatest of 64 maxima over disjoint parts is a bound that
-// count candidates reach and few more do; those go to LDS and are ranked by counting.
+// beam_slice_kernel: a workgroup goes through a slice of one beam's logits, sums exp(l) and
+// takes its `count` first.  Exponentials are fp32 (arguments off by 2^-22 at most at the top,
+// where they count), sums of 16 of them fp32 and of those fp64: log-sums are good to some 1e-8,
+// and to 1e-6 in any case.  The first: the count-th greatest of 64 maxima over disjoint parts is
+// a bound that count candidates reach and few more do; the rounds that hold one are loaded
+// again (each round's maximum is kept), and what reaches the bound goes to LDS and is ranked
+// by counting.  Keys in registers for all of it, with the code for each, left room for two waves
+// a SIMD: 104 us instead of 51 for 155 MB.
 // beam_join_kernel: a workgroup a sequence.  A wave joins a beam's sums and its slices' firsts in
-// the same way, then every candidate finds its rank by a binary search in each beam's line.
+// the same way, then every candidate finds its rank by counting, or by a binary search in each
+// beam's line.
+//
+// 64 sequences x 8 beams x 151936 bf16 logits (155 MB): 36 us and 7 for the join.  It loads at 4.3
+// TB/s with the VALUs busy 55 of 100 cycles (an exponential is a quarter as fast as an addition);
+// the start and the ranking, when nothing is loaded, are the rest.  All workgroups are there at
+// once, eight a CU: 12, 16 and 24 a CU took 37.3, 38.0 and 38.3 us, slices held in registers with
+// a barrier between maxima and sums 36.4 to 42.7.  One sequence is two latencies, 5.9 and 5.6 us.
 //
 // Keys are 64 bits and unique, the logit ordered as an integer over the complement of its
 // token, so that results do not depend on the order in which LDS slots are handed out.
@@ -30,10 +39,12 @@ constexpr int kThreads = 256;
 constexpr int kMostCount = 64;
 constexpr int kMostBeams = 64;
 constexpr int kMostFirsts = 2048;  // beams * count: 32 KiB of LDS
-constexpr int kVectors = 8;      // 16-byte loads of a thread at most
-constexpr int kRoom = 1024;      // candidates ranked at once
+constexpr int kRounds = 16;      // of a slice at most: their maxima are kept, 1 KiB each
+constexpr int kRoom = 512;       // candidates ranked at once
 constexpr int kJoinWaves = 8;
 constexpr int kJoinRoom = 256;   // of a wave there
+constexpr int kJoinLoads = 10;   // of a lane on their way
+constexpr int kJoinCounted = 256;  // candidates up to which ranks are counted: independent reads
 
 struct SelectArgs {
   const char* logits;
@@ -42,8 +53,9 @@ struct SelectArgs {
   int64_t vocab;
   int slices;
   const float* scores;
-  float* top;      // [sequences][beams][slices]
-  double* sums;    // [sequences][beams][slices]
+  int rounds;      // of a slice at most
+  double* base;    // [sequences][beams][slices]: the slice's sum of exp(l) is sums e^base
+  double* sums;
   uint64_t* best;  // [sequences][beams][slices][count]: keys, 0 for none
   float* out_scores;
   int32_t* parents;
@@ -65,17 +77,54 @@ __device__ __forceinline__ float value(const u32x4& v, int e) {
   else return (float)__builtin_bit_cast(T, (uint16_t)(v[e >> 1] >> 16 * (e & 1)));
 }
 
-// The n-th greatest (from 1) of the 64 lanes' numbers.
-__device__ __forceinline__ uint32_t nth_of_lanes(uint32_t mine, int n) {
-  const int lane = threadIdx.x & 63;
-  int rank = 0;  // equal ones in the order of their lanes
-#pragma unroll 16
-  for (int i = 0; i < 64; ++i) {
-    const uint32_t other = (uint32_t)__builtin_amdgcn_readlane((int)mine, i);
-    rank += (other > mine) | ((other == mine) & (i < lane));
+// Lane exchanges without LDS: rotations within rows of 16, then rows and halves side by side.
+template <int CTRL>
+__device__ __forceinline__ uint32_t moved(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false);
+}
+template <int CTRL>
+__device__ __forceinline__ float moved(float v) {
+  return __builtin_bit_cast(float, moved<CTRL>(__builtin_bit_cast(uint32_t, v)));
+}
+template <int CTRL>
+__device__ __forceinline__ double moved(double v) {
+  const u32x2 u = __builtin_bit_cast(u32x2, v);
+  return __builtin_bit_cast(double, u32x2{moved<CTRL>((uint32_t)u[0]), moved<CTRL>((uint32_t)u[1])});
+}
+template <class V>
+__device__ __forceinline__ V lane_of(V v, int lane) {
+  if constexpr (sizeof(V) == 8) {
+    const u32x2 u = __builtin_bit_cast(u32x2, v);
+    return __builtin_bit_cast(V, u32x2{(uint32_t)__builtin_amdgcn_readlane((int)u[0], lane),
+                                       (uint32_t)__builtin_amdgcn_readlane((int)u[1], lane)});
+  } else {
+    return __builtin_bit_cast(
+        V, (uint32_t)__builtin_amdgcn_readlane((int)__builtin_bit_cast(uint32_t, v), lane));
   }
-  const int at = __ffsll((long long)__ballot(rank == n - 1)) - 1;
-  return (uint32_t)__builtin_amdgcn_readlane((int)mine, at);
+}
+// f over the wave's lanes, the same in all of them (f commutes; the order is fixed).
+template <class V, class F>
+__device__ __forceinline__ V over_lanes(V v, F f) {
+  v = f(v, moved<0x121>(v));  // row_ror 1, 2, 4, 8
+  v = f(v, moved<0x122>(v));
+  v = f(v, moved<0x124>(v));
+  v = f(v, moved<0x128>(v));
+  return f(f(lane_of(v, 0), lane_of(v, 16)), f(lane_of(v, 32), lane_of(v, 48)));
+}
+__device__ __forceinline__ float greatest(float v) {
+  return over_lanes(v, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ double total(double v) {
+  return over_lanes(v, [](double a, double b) { return a + b; });
+}
+
+// The n-th greatest (from 1) of the 64 lanes' numbers: the least of those that fewer than n are
+// greater than.
+__device__ __forceinline__ uint32_t nth_of_lanes(uint32_t mine, int n) {
+  int rank = 0;
+#pragma unroll 16
+  for (int i = 0; i < 64; ++i) rank += (uint32_t)__builtin_amdgcn_readlane((int)mine, i) > mine;
+  return over_lanes(rank < n ? mine : ~0u, [](uint32_t a, uint32_t b) { return min(a, b); });
 }
 
 // The least key of a logit's order, or of any key.
@@ -109,103 +158,199 @@ __device__ __forceinline__ int gather(uint64_t* room, int* used, uint64_t bound,
   }
 }
 
-template <class T, int V>
+// 16 bytes of a line from token `at` on; at the line's end those before it, with -inf for the
+// tokens that are another thread's.  Lines of an odd vocabulary begin at any element.
+template <class T>
+struct Piece {
+  static constexpr int kEach = 16 / sizeof(T);
+  u32x4 x;
+  __device__ __forceinline__ static int from(int at, int vocab) { return min(at, vocab - kEach); }
+  __device__ __forceinline__ void load(const char* line, int at, int vocab) {
+    struct __attribute__((packed, aligned(sizeof(T)))) Loose {
+      u32x4 v;
+    };
+    x = reinterpret_cast<const Loose*>(line + (int64_t)from(at, vocab) * sizeof(T))->v;
+  }
+  __device__ __forceinline__ void mask(int at, int vocab) {
+#pragma unroll
+    for (int e = 0; e < kEach; ++e)
+      if (from(at, vocab) + e < at) none(e);
+  }
+  // Of a line shorter than a piece.
+  __device__ __forceinline__ void load_short(const char* line, int at, int vocab) {
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      none(e);
+      if (at + e < vocab) {
+        if constexpr (sizeof(T) == 4) put(e, reinterpret_cast<const uint32_t*>(line)[at + e]);
+        else put(e, reinterpret_cast<const uint16_t*>(line)[at + e]);
+      }
+    }
+  }
+  __device__ __forceinline__ float operator[](int e) const { return value<T>(x, e); }
+
+ private:
+  __device__ __forceinline__ void put(int e, uint32_t u) {
+    if constexpr (sizeof(T) == 4) x[e] = u;
+    else x[e >> 1] = (x[e >> 1] & (e & 1 ? 0xffffu : 0xffff0000u)) | u << 16 * (e & 1);
+  }
+  __device__ __forceinline__ void none(int e) {
+    put(e, sizeof(T) == 4 ? 0xff800000u : std::is_same<T, half_t>::value ? 0xfc00u : 0xff80u);
+  }
+};
+
+// A wave's running sums of exp(l), each lane's own `sum` times 2^shift, which stands for
+// e^(shift / c).  The shift is the wave's, a whole number next to the greatest logit so far (up to 4
+// below: a term's argument is then off by 2^-22 at most), so that a greater one costs no
+// rounding, and a term is 2^(l c - shift) by one fma.  Past 2^30 (`far`), where floats lie 64
+// apart and more, the sum is how many are the top.
+struct Terms {
+  static constexpr float c = 1.4426950408889634f;
+  double sum = 0.0;
+  float top = -INFINITY, shift = 0.f, limit = -INFINITY;
+  bool far = false;
+  // For logits up to `to`, the same in all lanes.
+  __device__ __forceinline__ void raise(float to) {
+    if (to <= top) return;
+    const bool was_far = far;
+    far = fabsf(to) >= 0x1p30f;
+    const float next = far ? 0.f : rintf(to * c);
+    if (far || was_far) sum *= 0.0;  // a NaN stays one
+    else if (top != -INFINITY) sum = __builtin_ldexp(sum, (int)fmaxf(shift - next, -4096.f));
+    top = to;
+    shift = next;
+    limit = far ? to : (next + 4.f) / c;
+  }
+  __device__ __forceinline__ void see(float mine) {
+    if (__any(mine > limit)) raise(greatest(mine));
+  }
+  template <class T, int P>
+  __device__ __forceinline__ void add(const Piece<T> (&x)[P]) {
+    constexpr int kEach = Piece<T>::kEach;
+    float part[P * kEach];
+    auto each = [&](auto term) {
+#pragma unroll
+      for (int i = 0; i < P; ++i)
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) part[i * kEach + e] = term(x[i][e]);
+    };
+    if (far) each([&](float l) { return l == top ? 1.f : l == l ? 0.f : l; });
+    else each([&](float l) { return __builtin_amdgcn_exp2f(__builtin_fmaf(l, c, -shift)); });
+#pragma unroll
+    for (int d = P * kEach / 2; d >= 1; d /= 2)
+#pragma unroll
+      for (int e = 0; e < d; ++e) part[e] += part[e + d];
+    sum += part[0];
+  }
+  // What is factored out, as a natural logarithm.
+  __device__ __forceinline__ double base() const {
+    return top == -INFINITY ? -INFINITY : far ? (double)top : shift / (double)c;
+  }
+};
+
+// P pieces a thread and round, the next round's on their way meanwhile (behind the last round
+// the line's end once more).  SHORT: lines of fewer tokens than a piece has.
+template <class T, int P, bool SHORT>
 __global__ __launch_bounds__(kThreads) void beam_slice_kernel(SelectArgs a) {
-  constexpr int kEach = 16 / sizeof(T);
+  constexpr int kEach = Piece<T>::kEach, kPass = kThreads * kEach;
   __shared__ uint64_t room[kRoom];
   __shared__ int used_slots;
+  __shared__ uint64_t shared_bound;
   __shared__ float tops[4][64];
   __shared__ double sums[4];
+  extern __shared__ float round_tops[];  // [rounds][threads]
   const int slice = blockIdx.x, beam = blockIdx.y, seq = blockIdx.z;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const char* line = a.logits + seq * a.seq + beam * a.beam;
-  const int64_t first = (int64_t)slice * (kThreads * kEach * V) + threadIdx.x * kEach;
-  // Rows of an odd vocabulary begin at any element.
-  struct __attribute__((packed, aligned(sizeof(T)))) Loose {
-    u32x4 v;
+  const int vocab = (int)a.vocab, start = slice * a.rounds * (kPass * P);
+  const int rounds = min(a.rounds, (vocab - start + kPass * P - 1) / (kPass * P));
+  const int first = start + threadIdx.x * kEach;
+  auto load = [&](Piece<T>& x, int at) {
+    if constexpr (SHORT) x.load_short(line, at, vocab);
+    else x.load(line, at, vocab);
   };
-  u32x4 x[V];
+  Piece<T> next[P];
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const int64_t i = first + (int64_t)v * kThreads * kEach;
-    if (i + kEach <= a.vocab) {
-      x[v] = reinterpret_cast<const Loose*>(line + i * sizeof(T))->v;
-    } else {
-      // -inf behind the last token, where key_of knows no candidate.
-      constexpr uint32_t none = sizeof(T) == 4 ? 0xff800000u
-                                : std::is_same<T, half_t>::value ? 0xfc00fc00u : 0xff80ff80u;
-      x[v] = u32x4{none, none, none, none};
+  for (int i = 0; i < P; ++i) load(next[i], first + i * kPass);
+  Terms terms;
+  float top = -INFINITY;
+#pragma unroll 1
+  for (int r = 0; r < rounds; ++r) {
+    Piece<T> x[P];
 #pragma unroll
-      for (int e = 0; e < kEach; ++e)
-        if (i + e < a.vocab) {
-          if constexpr (sizeof(T) == 4) {
-            x[v][e] = reinterpret_cast<const uint32_t*>(line)[i + e];
-          } else {
-            const uint32_t u = reinterpret_cast<const uint16_t*>(line)[i + e];
-            const uint32_t keep = e & 1 ? 0x0000ffffu : 0xffff0000u;
-            x[v][e >> 1] = (x[v][e >> 1] & keep) | u << 16 * (e & 1);
-          }
-        }
+    for (int i = 0; i < P; ++i) x[i] = next[i];
+    const int at = first + r * (kPass * P);
+#pragma unroll
+    for (int i = 0; i < P; ++i) load(next[i], at + (P + i) * kPass);
+    if (!SHORT && start + (r + 1) * (kPass * P) > vocab) {
+#pragma unroll
+      for (int i = 0; i < P; ++i) x[i].mask(at + i * kPass, vocab);
     }
-  }
-  float tops_of[V], top = -INFINITY;  // NaN is never greater
+    float here = -INFINITY;  // NaN is never greater
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    tops_of[v] = -INFINITY;
+    for (int i = 0; i < P; ++i)
 #pragma unroll
-    for (int e = 0; e < kEach; ++e) tops_of[v] = fmaxf(tops_of[v], value<T>(x[v], e));
-    top = fmaxf(top, tops_of[v]);
+      for (int e = 0; e < kEach; ++e) here = fmaxf(here, x[i][e]);
+    round_tops[r * kThreads + threadIdx.x] = here;
+    top = fmaxf(top, here);
+    terms.see(here);
+    terms.add(x);
   }
   tops[wave][lane] = top;
   __syncthreads();
   const float lane_top = fmaxf(fmaxf(tops[0][lane], tops[1][lane]),
                                fmaxf(tops[2][lane], tops[3][lane]));
-  // Lanes without a token of the slice have them behind its last one.
-  const bool some = (int64_t)slice * (kThreads * kEach * V) + lane * kEach < a.vocab;
-  const uint64_t bound = bound_from(nth_of_lanes(some ? ordered(lane_top) : 0u, a.count));
-  top = lane_top;
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, kWave));
-  // A NaN logit makes the sum NaN, and so does one of +inf.
-  const float base = top == -INFINITY ? 0.f : top;
-  double sum = 0.0;
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    float part = 0.f;
-#pragma unroll
-    for (int e = 0; e < kEach; ++e)
-      part += __builtin_amdgcn_exp2f((value<T>(x[v], e) - base) * 1.4426950408889634f);
-    sum += part;
+  if (wave == 0) {
+    // Lanes without a token of the slice have theirs behind its last one.
+    const bool some = start + lane * kEach < vocab;
+    const uint32_t nth = nth_of_lanes(some ? ordered(lane_top) : 0u, a.count);
+    if (lane == 0) shared_bound = bound_from(nth);
   }
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) sum += __shfl_xor(sum, d, kWave);
+  terms.raise(greatest(lane_top));
+  const double sum = total(terms.sum);
   if (lane == 0) sums[wave] = sum;
+  __syncthreads();
+  // The few rounds that reach the bound are loaded again.
   const int used = gather<kRoom>(
-      room, &used_slots, bound, a.count, threadIdx.x == 0,
+      room, &used_slots, shared_bound, a.count, threadIdx.x == 0,
       [&](uint64_t from, auto f) {
         const float least = unordered(max((uint32_t)(from >> 32), 0x007fffffu));
+        // Lanes go through their own rounds side by side, hardly ever more than one.
+        uint32_t those = 0;
+        for (int r = 0; r < rounds; ++r)
+          those |= (uint32_t)(round_tops[r * kThreads + threadIdx.x] >= least) << r;
+        while (those) {
+          const int at = first + (__ffs((int)those) - 1) * (kPass * P);
+          those &= those - 1;
+          Piece<T> x[P];
 #pragma unroll
-        for (int v = 0; v < V; ++v)
-          if (tops_of[v] >= least) {
+          for (int i = 0; i < P; ++i) load(x[i], at + i * kPass);
+#pragma unroll
+          for (int i = 0; i < P; ++i) {
+            const int from_here = at + i * kPass;
+            const int token = SHORT ? from_here : Piece<T>::from(from_here, vocab);
 #pragma unroll
             for (int e = 0; e < kEach; ++e) {
-              const int64_t i = first + (int64_t)v * kThreads * kEach + e;
-              const uint64_t key = (uint64_t)ordered(fmaxf(value<T>(x[v], e), -INFINITY)) << 32 |
-                                   (uint32_t)~(uint32_t)i;
-              if (i < a.vocab && key >= from) f(key);
+              const float l = fmaxf(x[i][e], -INFINITY);
+              if (l < least) continue;
+              const int t = token + e;
+              const uint64_t key = (uint64_t)ordered(l) << 32 | (uint32_t)~(uint32_t)t;
+              if (t >= from_here && t < vocab && key >= from) f(key);
             }
           }
+        }
       },
       [] { __syncthreads(); });
   const int64_t unit = ((int64_t)seq * a.beams + beam) * a.slices + slice;
   if (threadIdx.x == 0) {
-    a.top[unit] = top;
+    a.base[unit] = terms.base();
     a.sums[unit] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
   }
   uint64_t* out = a.best + unit * a.count;
   for (int c = threadIdx.x; c < used; c += kThreads) {
     const uint64_t key = room[c];
     int rank = 0;
+#pragma unroll 8
     for (int o = 0; o < used; ++o) rank += room[o] > key;
     if (rank < a.count) out[rank] = key;
   }
@@ -234,38 +379,54 @@ __global__ __launch_bounds__(64 * kJoinWaves) void beam_join_kernel(SelectArgs a
   };
   for (int b = wave; b < a.beams; b += kJoinWaves) {
     const int64_t unit = ((int64_t)seq * a.beams + b) * a.slices;
-    float top = -INFINITY;
-    for (int s = lane; s < a.slices; s += 64) top = fmaxf(top, a.top[unit + s]);
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, kWave));
-    double sum = 0.0;
-    for (int s = lane; s < a.slices; s += 64) {
-      const float t = a.top[unit + s];
-      const double part = a.sums[unit + s];
-      sum += t == -INFINITY ? part : part * exp((double)t - (double)top);  // 0 (or NaN) of -inf
-    }
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) sum += __shfl_xor(sum, d, kWave);
-    const double whole = (double)top + log(sum);
-    const double score = a.scores[(int64_t)seq * a.beams + b];
     const uint64_t* best = a.best + unit * a.count;
     const int n = a.slices * a.count;
+    const double score = a.scores[(int64_t)seq * a.beams + b];
+    // The first keys of a lane stay with it; the others are loaded as often as they are wanted.
+    uint64_t mine[kJoinLoads];
+#pragma unroll
+    for (int i = 0; i < kJoinLoads; ++i) mine[i] = lane + 64 * i < n ? best[lane + 64 * i] : 0;
+    auto each_key = [&](auto f) {
+#pragma unroll
+      for (int i = 0; i < kJoinLoads; ++i) f(mine[i]);
+      for (int c = lane + 64 * kJoinLoads; c < n; c += 64 * kJoinLoads) {
+        uint64_t key[kJoinLoads];
+#pragma unroll
+        for (int i = 0; i < kJoinLoads; ++i) key[i] = c + 64 * i < n ? best[c + 64 * i] : 0;
+#pragma unroll
+        for (int i = 0; i < kJoinLoads; ++i) f(key[i]);
+      }
+    };
+    // The first 64 slices' sums at once with all the rest.
+    const double my_base = lane < a.slices ? a.base[unit + lane] : -INFINITY;
+    const double my_sum = lane < a.slices ? a.sums[unit + lane] : 0.0;
     uint64_t most = 0;
-    for (int c = lane; c < n; c += 64) most = max(most, best[c]);
+    each_key([&](uint64_t key) { most = max(most, key); });
+    double base = my_base;
+    for (int s = 64 + lane; s < a.slices; s += 64) base = fmax(base, a.base[unit + s]);
+    base = over_lanes(base, [](double u, double w) { return fmax(u, w); });
+    auto scaled = [&](double of, double part) {  // 0 (or NaN) of a slice of -inf
+      return of == -INFINITY ? part : part * exp(of - base);
+    };
+    double sum = scaled(my_base, my_sum);
+    for (int s = 64 + lane; s < a.slices; s += 64)
+      sum += scaled(a.base[unit + s], a.sums[unit + s]);
+    sum = total(sum);
+    const double whole = base + log(sum);
     const uint64_t bound = bound_from(nth_of_lanes((uint32_t)(most >> 32), a.count));
     uint64_t* room = rooms[wave];
     const int used = gather<kJoinRoom>(
         room, &used_slots[wave], bound, a.count, lane == 0,
         [&](uint64_t from, auto f) {
-          for (int c = lane; c < n; c += 64) {
-            const uint64_t key = best[c];
+          each_key([&](uint64_t key) {
             if (key >= from) f(key);
-          }
+          });
         },
         wave_sync);
     for (int c = lane; c < used; c += 64) {
       const uint64_t key = room[c];
       int rank = 0;
+#pragma unroll 8
       for (int o = 0; o < used; ++o) rank += room[o] > key;
       if (rank >= a.count) continue;
       const double l = unordered((uint32_t)(key >> 32));
@@ -276,7 +437,31 @@ __global__ __launch_bounds__(64 * kJoinWaves) void beam_join_kernel(SelectArgs a
     wave_sync();
   }
   __syncthreads();
-  for (int c = threadIdx.x; c < a.beams * a.count; c += 64 * kJoinWaves) {
+  // Candidates in the order of beam and place there: equal ones stand in the order wanted.
+  const int all = a.beams * a.count;
+  auto place = [&](int c, uint64_t v, int rank) {
+    if (rank >= a.count) return;
+    const int64_t at = (int64_t)seq * a.count + rank;
+    const uint64_t u = v >> 63 ? v & ~((uint64_t)1 << 63) : ~v;
+    a.out_scores[at] = (float)__builtin_bit_cast(double, u);
+    a.parents[at] = c / a.count;
+    a.tokens[at] = (int64_t)(uint32_t)~(uint32_t)keys[c];
+  };
+  if (all <= kJoinCounted) {
+    // Four threads count for one.
+    const int part = threadIdx.x & 3;
+    for (int c = threadIdx.x >> 2; c < all; c += 16 * kJoinWaves) {
+      const uint64_t v = vs[c];
+      uint32_t rank = 0;
+#pragma unroll 8
+      for (int o = part; o < all; o += 4) rank += (vs[o] > v) | ((vs[o] == v) & (o < c));
+      rank += moved<0xb1>(rank);  // quad_perm: the neighbour, then the other two
+      rank += moved<0x4e>(rank);
+      if (part == 0 && v) place(c, v, rank);
+    }
+    return;
+  }
+  for (int c = threadIdx.x; c < all; c += 64 * kJoinWaves) {
     const uint64_t v = vs[c];
     if (!v) continue;
     const int b = c / a.count;
@@ -293,25 +478,23 @@ __global__ __launch_bounds__(64 * kJoinWaves) void beam_join_kernel(SelectArgs a
       }
       rank += lo;
     }
-    if (rank >= a.count) continue;
-    const int64_t at = (int64_t)seq * a.count + rank;
-    const uint64_t u = v >> 63 ? v & ~((uint64_t)1 << 63) : ~v;
-    a.out_scores[at] = (float)__builtin_bit_cast(double, u);
-    a.parents[at] = b;
-    a.tokens[at] = (int64_t)(uint32_t)~(uint32_t)keys[c];
+    place(c, v, rank);
   }
 }
 
 struct SelectLayout {
-  int vectors, slices;
-  size_t top, sums, best, bytes;
+  int pieces, rounds, slices;  // 16-byte loads of a thread and round
+  size_t base, sums, best, bytes;
   SelectLayout(int sequences, int beams, int64_t vocab, int count, int width) {
     const int64_t lines = (int64_t)sequences * beams;
-    // As many loads a thread as leave every CU four workgroups.
-    vectors = kVectors;
-    auto cut = [&](int v) { return cdiv(vocab, (int64_t)kThreads * (16 / width) * v); };
-    while (vectors > 1 && lines * cut(vectors) < 4 * (int64_t)device_cu_count()) vectors /= 2;
-    slices = (int)cut(vectors);
+    const int64_t all = cdiv(vocab, (int64_t)kThreads * (16 / width));
+    // Slices for eight workgroups a CU, of one round of one load as long as there are fewer.
+    const int64_t wanted = cdiv(8 * (int64_t)device_cu_count(), lines);
+    const int64_t each = cdiv(all, wanted < all ? wanted : all);
+    pieces = each > 1 ? 2 : 1;
+    rounds = (int)cdiv(each, pieces);
+    if (rounds > kRounds) rounds = kRounds;
+    slices = (int)cdiv(all, (int64_t)rounds * pieces);
     bytes = 0;
     auto take = [&](size_t n) {
       const size_t at = bytes;
@@ -320,19 +503,20 @@ struct SelectLayout {
     };
     best = take((size_t)lines * slices * count * 8);
     sums = take((size_t)lines * slices * 8);
-    top = take((size_t)lines * slices * 4);
+    base = take((size_t)lines * slices * 8);
   }
 };
 
 template <class T>
 int launch(const SelectArgs& a, const SelectLayout& p, int sequences, hipStream_t st) {
   const dim3 grid((unsigned)p.slices, (unsigned)a.beams, (unsigned)sequences), block(kThreads);
-  switch (p.vectors) {
-    case 1: hipLaunchKernelGGL((beam_slice_kernel<T, 1>), grid, block, 0, st, a); break;
-    case 2: hipLaunchKernelGGL((beam_slice_kernel<T, 2>), grid, block, 0, st, a); break;
-    case 4: hipLaunchKernelGGL((beam_slice_kernel<T, 4>), grid, block, 0, st, a); break;
-    default: hipLaunchKernelGGL((beam_slice_kernel<T, 8>), grid, block, 0, st, a); break;
-  }
+  const unsigned lds = p.rounds * kThreads * 4;
+  if (a.vocab < Piece<T>::kEach)
+    hipLaunchKernelGGL((beam_slice_kernel<T, 1, true>), grid, block, lds, st, a);
+  else if (p.pieces == 1)
+    hipLaunchKernelGGL((beam_slice_kernel<T, 1, false>), grid, block, lds, st, a);
+  else
+    hipLaunchKernelGGL((beam_slice_kernel<T, 2, false>), grid, block, lds, st, a);
   SS_CHECK_LAUNCH("beam_slice_kernel");
   hipLaunchKernelGGL(beam_join_kernel, dim3((unsigned)sequences), dim3(64 * kJoinWaves),
                      (unsigned)(a.beams * a.count * 16), st, a);
@@ -377,7 +561,7 @@ extern "C" int ss_select_beams(const void* logits, int64_t l_seq, int64_t l_beam
                "%s: workspace of %zu bytes, needs %zu", who, workspace_bytes, p.bytes);
   char* ws = (char*)workspace;
   SelectArgs a{(const char*)logits, l_seq * width, l_beam * width, beams, count, vocab, p.slices,
-               scores, (float*)(ws + p.top), (double*)(ws + p.sums), (uint64_t*)(ws + p.best),
+               scores, p.rounds, (double*)(ws + p.base), (double*)(ws + p.sums), (uint64_t*)(ws + p.best),
                out_scores, parents, tokens};
   const hipStream_t st = (hipStream_t)stream;
   return dtype == SS_F32   ? launch<float>(a, p, sequences, st)
