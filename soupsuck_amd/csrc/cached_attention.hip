@@ -351,7 +351,7 @@ __global__ __launch_bounds__(64 * W) void cached_attention_kernel(CachedAttnArgs
                   bool whole, int slot) {
     attend<T, QT, W, RW, SCORES, ONCE>(a, lds, b, block, kv, seq, span, x0, x1, whole, slot);
   };
-  if constexpr (SPLIT) for_ranges<QT, W, RW>(a, lds, unit);
+  if constexpr (SPLIT) for_ranges<QT, W, RW, false>(a, lds, unit);
   else for_unit<QT, RW>(a, unit);
   if (blockIdx.x == 0) clear_outside<W>(a);
 }

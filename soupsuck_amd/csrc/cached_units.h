@@ -336,34 +336,107 @@ __global__ __launch_bounds__(256) void cached_zeros_kernel(CachedAttnArgs a) {
       u32x4{0, 0, 0, 0};
 }
 
-// The workgroup's range of the line of all units' tiles, as calls of unit_of.
-template <int QT, int W, int RW, class F>
+// A workgroup's tiles [x0, x1) of a unit.
+struct Segment {
+  int line, kv, x0, x1, slot;
+  bool whole;
+  Sequence seq;
+};
+
+// Units cut into equal parts, each a workgroup's (`mine`, with x1 0 where there is none left):
+// true where that is done.  A range that holds the end of one unit and the start of another goes through
+// both one after the other, 5 us more than the others take.  Parts of up to as many tiles as
+// a range has places (its units' starts counted) are therefore better, if there are workgroups
+// for all of them; with few units there are.  Every wave finds its part by itself.
+template <int QT, int RW>
+__device__ __forceinline__ bool equal_parts(const CachedAttnArgs& a, Segment& mine) {
+  const int hk = a.cache.kv_heads, lane = threadIdx.x & 63;
+  const int lines = a.sequences * a.blocks;
+  if (lines > 64 || 2 * lines * hk > a.workers) return false;
+  Sequence seq{};
+  int tiles = 0;
+  if (lane < lines) {
+    const int b = lane / a.blocks;
+    seq = Sequence(a, b);
+    tiles = Span(a, seq, lane - b * a.blocks, 16 * QT * RW).tiles;
+  }
+  auto all = [&](int64_t v) {
+    return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)v, 63) |
+                     (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), 63) << 32);
+  };
+  const int64_t total = all(lanes_upto(tiles)) * hk;
+  const int64_t starts = (int64_t)__popcll(__ballot(tiles > 0)) * hk * kStart;
+  if (total > INT32_MAX / 2) return false;
+  const int least = (int)quotient(total + a.workers - 1, a.workers);
+  const int most = max((int)quotient(total + starts + a.workers - 1, a.workers), kMinRange);
+  int parts = 0;
+  int64_t upto = 0;
+  bool fits = false;
+#pragma unroll 1
+  for (int i = 0; i < 4 && !fits; ++i) {
+    const int size = max(least + (most - least) * i / 3, 1);
+    parts = (tiles + size - 1) / size;
+    upto = lanes_upto((int64_t)parts) * hk;
+    fits = all(upto) <= a.workers;
+  }
+  if (!fits) return false;
+  mine.x1 = 0;
+  if ((int64_t)blockIdx.x >= all(upto)) return true;
+  const int at = uniform(__ffsll((long long)__ballot(upto > (int64_t)blockIdx.x)) - 1);
+  auto of_line = [&](int v) { return __builtin_amdgcn_readlane(v, at); };
+  parts = of_line(parts);
+  tiles = of_line(tiles);
+  const int within = (int)blockIdx.x - of_line((int)upto) + parts * hk;
+  const int part = within % parts;
+  mine.line = at;
+  mine.kv = within / parts;
+  mine.x0 = (int)((int64_t)tiles * part / parts);
+  mine.x1 = (int)((int64_t)tiles * (part + 1) / parts);
+  mine.whole = parts == 1;
+  mine.slot = 2 * (int)blockIdx.x;
+  mine.seq.start = of_line(seq.start);
+  mine.seq.n = of_line(seq.n);
+  mine.seq.len = of_line(seq.len);
+  mine.seq.at = (int64_t)((uint64_t)(uint32_t)of_line((int)seq.at) |
+                          (uint64_t)(uint32_t)of_line((int)(seq.at >> 32)) << 32);
+  if (part == 0 && threadIdx.x == 0)
+    a.units[(int64_t)at * hk + mine.kv] = int4{(int)blockIdx.x, (int)blockIdx.x + parts - 1, 0, 0};
+  return true;
+}
+
+// The workgroup's range of the line of all units' tiles (PARTS: or its equal part), as calls of
+// unit_of.
+template <int QT, int W, int RW, bool PARTS, class F>
 __device__ __forceinline__ void for_ranges(const CachedAttnArgs& a, Results<QT, W>& lds, F unit_of) {
   const int hk = a.cache.kv_heads;
+  Segment mine;
+  const bool equal = PARTS && equal_parts<QT, RW>(a, mine);
   // Lines (sequence, block), 64 at a time: the places of each, and up to and with it.
   const int lane = threadIdx.x & 63;
   const int lines = a.sequences * a.blocks;
   auto scan = [&](int first) {
     __syncthreads();
     if (threadIdx.x < 64) {
-      uint32_t mine = 0;
+      uint32_t places = 0;
       if (first + lane < lines) {
         const int b = (first + lane) / a.blocks;
         const Sequence seq(a, b);
-        mine = Span(a, seq, first + lane - b * a.blocks, 16 * QT * RW).tiles;
+        places = Span(a, seq, first + lane - b * a.blocks, 16 * QT * RW).tiles;
         lds.seq[lane] = seq;
-        lds.tiles[lane] = mine;
-        if (mine) mine += kStart;
+        lds.tiles[lane] = places;
+        if (places) places += kStart;
       }
-      lds.upto[lane] = lanes_upto(mine);
+      lds.upto[lane] = lanes_upto(places);
     }
     __syncthreads();
   };
   int64_t total = 0;
+  if (!equal) {
 #pragma unroll 1
-  for (int first = (lines - 1) / 64 * 64; first >= 0; first -= 64) {
-    scan(first);
-    total += lds.upto[63];
+    for (int first = (lines - 1) / 64 * 64; first >= 0; first -= 64) {
+      scan(first);
+      total += lds.upto[63];
+    }
   }
   total = uniform(total) * hk;
   const int64_t range = max(uniform(quotient(total + a.workers - 1, a.workers)),
@@ -372,31 +445,38 @@ __device__ __forceinline__ void for_ranges(const CachedAttnArgs& a, Results<QT, 
   const int64_t end = min(begin + range, total);
   int base = 0;
   int64_t before = 0;  // places (of one kv head) of the lines before these 64
-  for (int64_t pos = begin; pos < end;) {
-    while (pos >= (before + uniform(lds.upto[63])) * hk) {
-      before += uniform(lds.upto[63]);
-      base += 64;
-      scan(base);
+  for (int64_t pos = begin; equal || pos < end;) {
+    if (equal) {
+      if (!mine.x1) break;
+    } else {
+      while (pos >= (before + uniform(lds.upto[63])) * hk) {
+        before += uniform(lds.upto[63]);
+        base += 64;
+        scan(base);
+      }
+      const int at =
+          uniform(__ffsll((long long)__ballot((before + lds.upto[lane]) * hk > pos)) - 1);
+      const int tiles = uniform(lds.tiles[at]);
+      const int64_t line_start = (before + uniform(lds.upto[at]) - tiles - kStart) * hk;
+      mine.kv = uniform((int)quotient(pos - line_start, tiles + kStart));
+      const int64_t unit = line_start + (int64_t)mine.kv * (tiles + kStart);
+      mine.x0 = max((int)(pos - unit) - kStart, 0);
+      mine.x1 = (int)min((int64_t)tiles, end - unit - kStart);
+      mine.line = base + at;
+      pos = unit + kStart + mine.x1;
+      if (mine.x1 <= mine.x0) break;  // the range ends before the unit's first tile
+      mine.whole = mine.x0 == 0 && mine.x1 == tiles;
+      mine.slot = (int)(2 * blockIdx.x + (unit > begin));
+      if (mine.x0 == 0 && threadIdx.x == 0)
+        a.units[(int64_t)mine.line * hk + mine.kv] =
+            int4{(int)blockIdx.x, (int)quotient(unit + kStart + tiles - 1, range), unit > begin, 0};
+      mine.seq = lds.seq[at];
+      mine.seq.settle();
     }
-    const int at = uniform(__ffsll((long long)__ballot((before + lds.upto[lane]) * hk > pos)) - 1);
-    const int tiles = uniform(lds.tiles[at]);
-    const int64_t line_start = (before + uniform(lds.upto[at]) - tiles - kStart) * hk;
-    const int kv = uniform((int)quotient(pos - line_start, tiles + kStart));
-    const int64_t unit = line_start + (int64_t)kv * (tiles + kStart);
-    const int x0 = max((int)(pos - unit) - kStart, 0);
-    const int x1 = (int)min((int64_t)tiles, end - unit - kStart);
-    const int line = base + at;
-    const int b = uniform(line / a.blocks), block = line - b * a.blocks;
-    pos = unit + kStart + x1;
-    if (x1 <= x0) break;  // the range ends before the unit's first tile
-    const bool whole = x0 == 0 && x1 == tiles;
-    if (x0 == 0 && threadIdx.x == 0)
-      a.units[(int64_t)line * hk + kv] =
-          int4{(int)blockIdx.x, (int)quotient(unit + kStart + tiles - 1, range), unit > begin, 0};
-    Sequence seq = lds.seq[at];
-    seq.settle();
-    Span span(a, seq, block, 16 * QT * RW);
-    unit_of(b, block, kv, seq, span, x0, x1, whole, (int)(2 * blockIdx.x + (unit > begin)));
+    const int b = uniform(mine.line / a.blocks), block = mine.line - b * a.blocks;
+    const Span span(a, mine.seq, block, 16 * QT * RW);
+    unit_of(b, block, mine.kv, mine.seq, span, mine.x0, mine.x1, mine.whole, mine.slot);
+    if (equal) break;
     if (pos < end) __syncthreads();  // the waves' results are read before the next ones come
   }
 }
@@ -479,8 +559,9 @@ struct Layout {
   int score_rows;           // 0: no scores kept
   int64_t score_keys;
   size_t stats, list, ml, o, scores, bytes;  // workspace offsets
+  // ranges: workgroups of a CU that a block of at most 16 rows has room for.
   Layout(int rows, int64_t tokens, int q_heads, int kv_heads, int new_bound, int64_t max_length,
-         bool weights) {
+         bool weights, int ranges = 1) {
     max_new = (int)(new_bound < tokens ? new_bound : tokens);
     const int64_t of_sequence = (int64_t)(max_new > 0 ? max_new : 1) * (q_heads / kv_heads);
     // A wave takes 16 rows, or 32, and up to four waves of 32 share a tile: 33 new tokens of 4
@@ -489,7 +570,8 @@ struct Layout {
     blocks = (int)cdiv(of_sequence, block_rows);
     units = (int64_t)rows * blocks * kv_heads;
     const int stripes = kWaves / (block_rows <= 32 ? 1 : block_rows / 32);
-    workers = max_length <= kWholeTiles * kKeys * stripes ? 0 : device_cu_count();
+    workers = max_length <= kWholeTiles * kKeys * stripes
+                  ? 0 : device_cu_count() * (block_rows == 16 ? ranges : 1);
     score_keys = cdiv(max_length > 0 ? max_length : 1, kKeys) * kKeys;
     score_rows = 0;
     if (weights && of_sequence <= kScoreRows &&
