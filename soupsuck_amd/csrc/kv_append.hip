@@ -29,6 +29,7 @@ struct AppendArgs {
   const int32_t* cu;
   int sequences;
   uint32_t items;  // tokens * heads
+  uint32_t query_items;  // 4-bit cache: tokens * sets of query heads, the first of the items
   const char* k; int64_t k_tok, k_head;  // bytes
   const char* v; int64_t v_tok, v_head;
   const char* q; int64_t q_tok, q_head;
@@ -37,6 +38,8 @@ struct AppendArgs {
   char* qo; int64_t qo_tok, qo_head;
   int hq, heads;  // q heads (0: none); q + 2 kv heads
 };
+
+constexpr int kQueryHeads = 4;  // of a set
 
 template <class T>
 using Vec8 = T __attribute__((ext_vector_type(8)));
@@ -97,14 +100,58 @@ __device__ __forceinline__ int page_of(const AppendArgs& a, uint32_t t, int64_t*
   return a.rows.page(b, entry, a.cache.pages);
 }
 
+// Some heads of a token's queries by eight threads, which load its angles once.
+template <class T, class CS>
+__device__ __forceinline__ void turn_queries(const AppendArgs& a, uint32_t item, int c) {
+  const uint32_t sets = (uint32_t)(a.hq + kQueryHeads - 1) / kQueryHeads, t = item / sets;
+  const int first = (int)(item - t * sets) * kQueryHeads;
+  Vec8<T> lo[kQueryHeads], hi[kQueryHeads];
+#pragma unroll
+  for (int i = 0; i < kQueryHeads; ++i) {
+    const char* from = a.q + t * a.q_tok + min(first + i, a.hq - 1) * a.q_head;
+    lo[i] = reinterpret_cast<const Vec8<T>*>(from)[c / 8];
+    hi[i] = reinterpret_cast<const Vec8<T>*>(from)[c / 8 + 8];
+  }
+  float c1[8], c2[8], s1[8], s2[8];
+  load_angles<CS>(a.cos + t * a.cos_tok, c, c1);
+  load_angles<CS>(a.cos + t * a.cos_tok, c + 64, c2);
+  load_angles<CS>(a.sin + t * a.sin_tok, c, s1);
+  load_angles<CS>(a.sin + t * a.sin_tok, c + 64, s2);
+#pragma unroll
+  for (int i = 0; i < kQueryHeads; ++i) {
+    if (first + i >= a.hq) break;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x = (float)lo[i][e], y = (float)hi[i][e];
+      lo[i][e] = (T)(x * c1[e] - y * s1[e]);
+      hi[i][e] = (T)(y * c2[e] + x * s2[e]);
+    }
+    char* to = a.qo + t * a.qo_tok + (first + i) * a.qo_head;
+    reinterpret_cast<Vec8<T>*>(to)[c / 8] = lo[i];
+    reinterpret_cast<Vec8<T>*>(to)[c / 8 + 8] = hi[i];
+  }
+}
+
 template <class T, class CS, bool FOUR>
 __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
   const uint32_t item = blockIdx.x * 32 + (threadIdx.x >> 3);
   if (item >= a.items) return;
   const int c = (threadIdx.x & 7) * 8;
-  const uint32_t t = item / (uint32_t)a.heads;
-  const int head = (int)(item - t * (uint32_t)a.heads);
   const int hk = a.cache.kv_heads;
+  uint32_t t;
+  int head;
+  if constexpr (FOUR) {
+    if (item < a.query_items) {
+      turn_queries<T, CS>(a, item, c);
+      return;
+    }
+    const uint32_t row = item - a.query_items;
+    t = row / (2 * (uint32_t)hk);
+    head = (int)(row - t * 2 * (uint32_t)hk) + a.hq;
+  } else {
+    t = item / (uint32_t)a.heads;
+    head = (int)(item - t * (uint32_t)a.heads);
+  }
   const bool is_q = head < a.hq, is_k = !is_q && head < a.hq + hk;
   const int h = is_q ? head : is_k ? head - a.hq : head - a.hq - hk;
   const char* from = is_q   ? a.q + t * a.q_tok + h * a.q_head
@@ -117,13 +164,13 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = (float)lo[e], y[e] = (float)hi[e];
   }
-  if (a.cos && (is_q || is_k)) {
+  if (a.cos && (is_k || (!FOUR && is_q))) {
     float c1[8], c2[8], s1[8], s2[8];
     load_angles<CS>(a.cos + t * a.cos_tok, c, c1);
     load_angles<CS>(a.cos + t * a.cos_tok, c + 64, c2);
     load_angles<CS>(a.sin + t * a.sin_tok, c, s1);
     load_angles<CS>(a.sin + t * a.sin_tok, c + 64, s2);
-    if (FOUR && is_k) {
+    if constexpr (FOUR) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const double u = x[e], w = y[e];
@@ -140,7 +187,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
     }
   }
   char* to;
-  if (is_q) {
+  if (!FOUR && is_q) {
     to = a.qo + t * a.qo_tok + h * a.qo_head;
   } else {
     int64_t r = 0;
@@ -200,13 +247,15 @@ int append(const char* who, const Cache* cache, const void* k, int64_t k_tok, in
   SS_CHECK_ARG(heads <= INT32_MAX && tokens <= (int64_t)INT32_MAX / heads,
                "%s: too many rows in one call", who);
   const int cs = cs_dtype == SS_F32 ? 4 : 2;
+  const int64_t sets = FOUR ? cdiv(hq, kQueryHeads) : 0;
+  const int64_t items = tokens * (FOUR ? sets + 2 * (int64_t)cache->kv_heads : heads);
   AppendArgs a{cache_view(cache), TableView{table, table_stride, row_pages, lengths},
-               cu_seqlens, rows, (uint32_t)(tokens * heads),
+               cu_seqlens, rows, (uint32_t)items, (uint32_t)(tokens * sets),
                (const char*)k, k_tok * 2, k_head * 2, (const char*)v, v_tok * 2, v_head * 2,
                (const char*)q, q_tok * 2, q_head * 2, (const char*)cos, cos_tok * cs,
                (const char*)sin, sin_tok * cs, (char*)q_out, qo_tok * 2, qo_head * 2, hq,
                (int)heads};
-  const dim3 grid((unsigned)cdiv(tokens * heads, 32)), block(256);
+  const dim3 grid((unsigned)cdiv(items, 32)), block(256);
   const hipStream_t st = (hipStream_t)stream;
   const bool wide = cos && cs_dtype == SS_F32;
   if (cache->dtype == SS_F16) {

@@ -7,9 +7,12 @@
 // kv_fork: new row i continues old row p = parents[i].  Its full pages are p's own (shared from
 // then on: nothing is appended to them), the page that p's next token goes to is spare[i], and
 // the rows that p has there already are copied, for all layers in one launch: a workgroup
-// takes 16 rows of one head of one layer, 8 KiB (16 bits) or a group (4 bits) in one round of
-// 16-byte loads.  Offsets, length and table entry are three dependent loads, and that
-// latency is what a small fork costs.
+// takes 16 rows of one head, 8 KiB (16 bits) or a group (4 bits), in some of the layers.
+// Parent, length and table entry are three dependent loads, and that latency is what a small
+// fork costs: 28 layers of 4 beams 4.0 us; 32 beams of 4 heads (43 MB) 14.4 us, 20.7 with a
+// workgroup for every layer.  Reading those rows back (98 MB) takes 21 us, 4.7 TB/s, in a
+// workgroup for every layer: two of them one after the other took the same, and one
+// layer's read longer.
 #include "paged4.h"
 
 namespace ss {
@@ -97,7 +100,8 @@ struct ForkArgs {
 };
 
 template <bool FOUR>
-__global__ __launch_bounds__(256) void kv_fork_kernel(ForkArgs a, bool tables) {
+__global__ __launch_bounds__(256) void kv_fork_kernel(ForkArgs a, int caches, int each,
+                                                      bool tables) {
   const int pieces = a.cache.page_size / kGroupRows, hk = a.cache.kv_heads;
   const uint32_t unit = blockIdx.x / (uint32_t)pieces;
   const int piece = (int)(blockIdx.x - unit * pieces);
@@ -117,20 +121,29 @@ __global__ __launch_bounds__(256) void kv_fork_kernel(ForkArgs a, bool tables) {
     if (threadIdx.x == 0) a.out_lengths[i] = length;
   }
   if (from < 0 || spare < 0 || spare >= a.cache.pages || piece * kGroupRows >= open) return;
+  const int first = blockIdx.y * each, last = min(first + each, caches);
   if constexpr (FOUR) {
-    char* base = a.bases.k[blockIdx.y] + h * a.cache.k_head + piece * a.cache.k_row;
-    if (threadIdx.x < kGroupBytes / 16)
-      reinterpret_cast<u32x4*>(base + spare * a.cache.k_page)[threadIdx.x] =
-          reinterpret_cast<const u32x4*>(base + from * a.cache.k_page)[threadIdx.x];
+    constexpr int kParts = kGroupBytes / 16;
+    const int64_t at = h * a.cache.k_head + piece * a.cache.k_row;
+    const int64_t source = at + from * a.cache.k_page, target = at + spare * a.cache.k_page;
+#pragma unroll 4
+    for (int item = threadIdx.x; item < (last - first) * kParts; item += 256) {
+      char* base = a.bases.k[first + item / kParts] + item % kParts * 16;
+      *reinterpret_cast<u32x4*>(base + target) = *reinterpret_cast<const u32x4*>(base + source);
+    }
   } else {
-    const int r = piece * kGroupRows + (threadIdx.x >> 4), c = threadIdx.x & 15;
+    const int r = piece * kGroupRows + (threadIdx.x >> 4), c = (threadIdx.x & 15) * 16;
     if (r >= open) return;
-    char* k = a.bases.k[blockIdx.y] + h * a.cache.k_head + r * a.cache.k_row;
-    char* v = a.bases.v[blockIdx.y] + h * a.cache.v_head + r * a.cache.v_row;
-    const u32x4 x = reinterpret_cast<const u32x4*>(k + from * a.cache.k_page)[c];
-    const u32x4 y = reinterpret_cast<const u32x4*>(v + from * a.cache.v_page)[c];
-    reinterpret_cast<u32x4*>(k + spare * a.cache.k_page)[c] = x;
-    reinterpret_cast<u32x4*>(v + spare * a.cache.v_page)[c] = y;
+    const int64_t at_k = h * a.cache.k_head + r * a.cache.k_row + c;
+    const int64_t at_v = h * a.cache.v_head + r * a.cache.v_row + c;
+#pragma unroll 4
+    for (int cache = first; cache < last; ++cache) {
+      char *k = a.bases.k[cache] + at_k, *v = a.bases.v[cache] + at_v;
+      const u32x4 x = *reinterpret_cast<const u32x4*>(k + from * a.cache.k_page);
+      const u32x4 y = *reinterpret_cast<const u32x4*>(v + from * a.cache.v_page);
+      *reinterpret_cast<u32x4*>(k + spare * a.cache.k_page) = x;
+      *reinterpret_cast<u32x4*>(v + spare * a.cache.v_page) = y;
+    }
   }
 }
 
@@ -216,8 +229,11 @@ int fork(const char* who, const Cache* const* caches, int count, const int32_t* 
   return in_launches(caches, count, [&](const Bases& bases, int first, int n) -> int {
     ForkArgs a{cache_view(cache), TableView{table, table_stride, row_pages, lengths}, rows,
                parents, spare, out_table, out_lengths, new_rows, bases};
-    hipLaunchKernelGGL((kv_fork_kernel<FOUR>), dim3((unsigned)units, (unsigned)n), dim3(256), 0, st,
-                       a, first == 0);
+    // As many caches a workgroup as leave every CU eight.
+    const int64_t most = units * n / (8 * (int64_t)device_cu_count());
+    const int each = (int)(most < 1 ? 1 : most < 8 ? most : 8);
+    hipLaunchKernelGGL((kv_fork_kernel<FOUR>), dim3((unsigned)units, (unsigned)cdiv(n, each)),
+                       dim3(256), 0, st, a, n, each, first == 0);
     SS_CHECK_LAUNCH("kv_fork_kernel");
     return SS_OK;
   });

@@ -276,43 +276,78 @@ py::object evict_kv(int64_t cache_pointer, const Tensor& pages, py::handle table
   return py::make_tuple(out_lengths, out_weights);
 }
 
-// The caches of a call: alike, on one device, by their structs' addresses.
+// The caches of a call, a list or tuple of one class: their structs' addresses (`_pointer`) and
+// devices (`_index`) by attribute, as a call for each layer's cache would cost more than its kernel.
 struct Caches {
   std::vector<int64_t> pointers;
-  bool ok = true;
-  Caches(const py::list& addresses, const py::list& memory, bool is_four, const Tensor& first) {
-    for (size_t i = 0; i < addresses.size(); ++i) {
-      pointers.push_back(addresses[i].cast<int64_t>());
-      const Argument pages(memory[i]);
-      ok = ok && pages.ok && pages.t.defined() && pages.t.device() == first.device();
-      if (is_four) same<ss_paged_cache4>(offsetof(ss_paged_cache4, page), i);
-      else same<ss_paged_cache>(offsetof(ss_paged_cache, k_page), i);
+  bool ok = false, four = false;
+  int64_t index = -1;
+  Caches(py::handle caches, py::handle wide_type, py::handle four_type) {
+    static PyObject* const pointer_name = PyUnicode_InternFromString("_pointer");
+    static PyObject* const index_name = PyUnicode_InternFromString("_index");
+    const bool list = PyList_Check(caches.ptr());
+    if (!list && !PyTuple_Check(caches.ptr())) return;
+    const Py_ssize_t n = list ? PyList_GET_SIZE(caches.ptr()) : PyTuple_GET_SIZE(caches.ptr());
+    if (n == 0 || n >= INT32_MAX) return;
+    pointers.reserve(n);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+      PyObject* cache = list ? PyList_GET_ITEM(caches.ptr(), i) : PyTuple_GET_ITEM(caches.ptr(), i);
+      const bool is_four = (PyObject*)Py_TYPE(cache) == four_type.ptr();
+      if (!is_four && (PyObject*)Py_TYPE(cache) != wide_type.ptr()) return;
+      int64_t pointer, device;
+      if (!number_of(cache, pointer_name, &pointer) || !number_of(cache, index_name, &device))
+        return;
+      if (i == 0) four = is_four, index = device;
+      if (is_four != four || device != index || device < 0) return;
+      pointers.push_back(pointer);
+      if (!(four ? alike<ss_paged_cache4>(offsetof(ss_paged_cache4, page), 3)
+                 : alike<ss_paged_cache>(offsetof(ss_paged_cache, k_page), 3)))
+        return;
     }
-    ok = ok && !pointers.empty();
+    ok = true;
+  }
+  static bool number_of(PyObject* of, PyObject* name, int64_t* out) {
+    PyObject* value = PyObject_GetAttr(of, name);
+    const bool good = value && PyLong_CheckExact(value);
+    if (good) *out = PyLong_AsLongLong(value);
+    Py_XDECREF(value);
+    PyErr_Clear();
+    return good;
   }
   // Everything but the bases (the C entries compare the strides of v).
   template <class C>
-  void same(size_t from, size_t i) {
+  bool alike(size_t from, size_t strides) const {
     const auto *a = reinterpret_cast<const C*>(pointers[0]),
-               *b = reinterpret_cast<const C*>(pointers[i]);
-    ok = ok && a->pages == b->pages && a->page_size == b->page_size &&
-         a->kv_heads == b->kv_heads && a->dtype == b->dtype &&
-         !memcmp((const char*)a + from, (const char*)b + from, 3 * sizeof(int64_t));
+               *b = reinterpret_cast<const C*>(pointers.back());
+    return a->pages == b->pages && a->page_size == b->page_size && a->kv_heads == b->kv_heads &&
+           a->dtype == b->dtype &&
+           !memcmp((const char*)a + from, (const char*)b + from, strides * sizeof(int64_t));
   }
   template <class C>
   const C* const* all() const {
     return reinterpret_cast<const C* const*>(pointers.data());
   }
   int count() const { return (int)pointers.size(); }
+  bool on(const Tensor& t) const { return t.is_cuda() && t.device().index() == index; }
 };
 
-py::object read_kv(const py::list& addresses, const Tensor& pages, bool is_four,
-                   const py::list& memory, py::handle table_arg, py::handle lengths_arg,
-                   py::handle cu_arg, py::handle tokens_arg, bool several) {
+// The block table of a call, whose device the others are checked against.
+bool table_of(py::handle arg, Tensor* out) {
+  const Argument a(arg);
+  *out = a.t;
+  return a.ok && a.t.defined();
+}
+
+py::object read_kv(py::handle caches_arg, py::handle wide_type, py::handle four_type,
+                   py::handle table_arg, py::handle lengths_arg, py::handle cu_arg,
+                   py::handle tokens_arg, bool several) {
   int64_t tokens;
-  const Caches caches(addresses, memory, is_four, pages);
-  if (!caches.ok || !whole(tokens_arg, 1, (int64_t)1 << 31, &tokens)) return py::none();
-  const Cache cache(caches.pointers[0], is_four);
+  Tensor pages;
+  const Caches caches(caches_arg, wide_type, four_type);
+  if (!caches.ok || !whole(tokens_arg, 1, (int64_t)1 << 31, &tokens) ||
+      !table_of(table_arg, &pages) || !caches.on(pages))
+    return py::none();
+  const Cache cache(caches.pointers[0], caches.four);
   Checked c(pages);
   const Table rows(c, table_arg, lengths_arg);
   const Tensor cu = c.take(cu_arg, at::kInt, 1);
@@ -330,17 +365,18 @@ py::object read_kv(const py::list& addresses, const Tensor& pages, bool is_four,
                  ptr<void>(k), ptr<void>(v), stream_of(pages)),
             name);
     };
-    if (is_four) read(&ss_kv_read4, caches.all<ss_paged_cache4>(), "ss_kv_read4");
+    if (caches.four) read(&ss_kv_read4, caches.all<ss_paged_cache4>(), "ss_kv_read4");
     else read(&ss_kv_read, caches.all<ss_paged_cache>(), "ss_kv_read");
   }
   return py::make_tuple(k, v);
 }
 
-py::object fork_kv(const py::list& addresses, const Tensor& pages, bool is_four,
-                   const py::list& memory, py::handle table_arg, py::handle lengths_arg,
-                   py::handle parents_arg, py::handle spare_arg) {
-  const Caches caches(addresses, memory, is_four, pages);
-  if (!caches.ok) return py::none();
+py::object fork_kv(py::handle caches_arg, py::handle wide_type, py::handle four_type,
+                   py::handle table_arg, py::handle lengths_arg, py::handle parents_arg,
+                   py::handle spare_arg) {
+  Tensor pages;
+  const Caches caches(caches_arg, wide_type, four_type);
+  if (!caches.ok || !table_of(table_arg, &pages) || !caches.on(pages)) return py::none();
   Checked c(pages);
   const Table rows(c, table_arg, lengths_arg);
   const Tensor parents = c.take(parents_arg, at::kInt, 1), spare = c.take(spare_arg, at::kInt, 1);
@@ -360,7 +396,7 @@ py::object fork_kv(const py::list& addresses, const Tensor& pages, bool is_four,
                  ptr<int32_t>(lengths), stream_of(pages)),
             name);
     };
-    if (is_four) fork(&ss_kv_fork4, caches.all<ss_paged_cache4>(), "ss_kv_fork4");
+    if (caches.four) fork(&ss_kv_fork4, caches.all<ss_paged_cache4>(), "ss_kv_fork4");
     else fork(&ss_kv_fork, caches.all<ss_paged_cache>(), "ss_kv_fork");
   }
   return py::make_tuple(table, lengths);

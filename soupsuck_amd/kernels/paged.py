@@ -51,6 +51,11 @@ def _whole(value, minimum):
     return isinstance(value, int) and not isinstance(value, bool) and value >= minimum
 
 
+def _index(t):
+    """The tensor's GPU, -1 where it is on none."""
+    return t.device.index if t.is_cuda else -1
+
+
 CACHE_RULES = (
     Rule("PagedCache: k and v must be [pages, kv_heads, page_size, 128] fp16 or bf16 tensors of "
          "one shape, dtype and device, without gradients",
@@ -77,6 +82,7 @@ class PagedCache:
             k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], pages, size, heads, dim,
             _CODES[k.dtype])
         self._pointer = ctypes.addressof(self._struct)
+        self._index = _index(k)
 
     @classmethod
     def empty(cls, pages, kv_heads, page_size, dtype=torch.float16, device="cuda"):
@@ -143,6 +149,7 @@ class PagedCache4:
         self._struct = _lib.PagedCache4Struct(data.data_ptr(), *data.stride()[:3], pages,
                                               16 * groups, heads, HEAD_DIM, _CODES[dtype])
         self._pointer = ctypes.addressof(self._struct)
+        self._index = _index(data)
 
     @classmethod
     def empty(cls, pages, kv_heads, page_size, dtype=torch.float16, device="cuda"):
@@ -479,14 +486,13 @@ def read_kv(caches, block_table, lengths, cu_seqlens, tokens):
     sequence does not hold are zeros.
     """
     several = isinstance(caches, (list, tuple))
-    caches = _caches(caches)
-    nodes = native.nodes() if caches is not None else None
+    nodes = native.nodes()
     if nodes is not None:
-        got = nodes.read_kv([c._pointer for c in caches], _pages(caches[0]),
-                            _is_cache4(caches[0]), [_pages(c) for c in caches], block_table,
+        got = nodes.read_kv(caches if several else (caches,), PagedCache, PagedCache4, block_table,
                             lengths, cu_seqlens, tokens, several)
         if got is not None:
             return got
+    caches = _caches(caches)
     enforce(READ_RULES, caches=caches, cache=caches and caches[0], block_table=block_table,
             lengths=lengths, cu_seqlens=cu_seqlens, tokens=tokens,
             tensors=(block_table, lengths, cu_seqlens))
@@ -524,14 +530,13 @@ def fork_kv(caches, block_table, lengths, parents, spare):
     ``block_table`` and not named twice.  The parents' own last pages are free again once no
     row of ``block_table`` is used further, unless they are full.
     """
-    caches = _caches(caches)
-    nodes = native.nodes() if caches is not None else None
+    nodes = native.nodes()
     if nodes is not None:
-        got = nodes.fork_kv([c._pointer for c in caches], _pages(caches[0]),
-                            _is_cache4(caches[0]), [_pages(c) for c in caches], block_table,
-                            lengths, parents, spare)
+        got = nodes.fork_kv(caches if isinstance(caches, (list, tuple)) else (caches,), PagedCache,
+                            PagedCache4, block_table, lengths, parents, spare)
         if got is not None:
             return got
+    caches = _caches(caches)
     enforce(FORK_RULES, caches=caches, cache=caches and caches[0], block_table=block_table,
             lengths=lengths, parents=parents, spare=spare,
             tensors=(block_table, lengths, parents, spare))
