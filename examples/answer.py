@@ -1,6 +1,7 @@
 """Answering with a tuned model: NF4 weights with LoRA adapters, a paged cache, drafted tokens.
 
     python examples/answer.py [--layers 2] [--tokens 64] [--budget 256]
+    python examples/answer.py --beams 4 [--bits 4]
 
 A Qwen2.5 1.5B-shaped model (random weights here; the layers are ``soupsuck_amd.layer``'s)
 answers a batch of prompts of different lengths.  Each step the next tokens are guessed from the
@@ -10,6 +11,10 @@ made.  In that pass ``append_kv`` puts the rotated keys and the values into the 
 pages, ``cached_attention`` reads them and adds up every row's attention weight (again for the
 tokens that stay where some were refused: a weight is a vote of the text's own tokens), and when a
 sequence is well past its budget ``evict_kv`` moves each head's heaviest rows to fresh pages.
+
+With ``--bits 4`` the cache holds its rows in 4 bits (no budget then: it gives no weights).  With
+``--beams`` the best of several texts at a time is kept: ``select_beams`` chooses their
+continuations and ``fork_kv`` lets the caches' sequences follow.
 """
 
 import argparse
@@ -22,9 +27,10 @@ sys.path.insert(0, str(Path(__file__).resolve().parents[1]))
 
 from soupsuck_amd.kernels.add_rmsnorm import add_rms_norm  # noqa: E402
 from soupsuck_amd.kernels.attention import row_offsets  # noqa: E402
+from soupsuck_amd.kernels.beams import select_beams  # noqa: E402
 from soupsuck_amd.kernels.nf4_gemm import gemm_f16  # noqa: E402
-from soupsuck_amd.kernels.paged import (PagedCache, append_kv, cached_attention,  # noqa: E402
-                                        evict_kv)
+from soupsuck_amd.kernels.paged import (PagedCache, PagedCache4, append_kv,  # noqa: E402
+                                        cached_attention, evict_kv, fork_kv)
 from soupsuck_amd.kernels.rmsnorm import rms_norm  # noqa: E402
 from soupsuck_amd.kernels.swiglu import swiglu  # noqa: E402
 from soupsuck_amd.kernels.verify import verify_drafts  # noqa: E402
@@ -74,17 +80,27 @@ def rotation(positions):
 
 
 class Session:
-    """A batch of texts and their pages; one table serves the caches of all layers."""
+    """A batch of texts and their pages; one table serves the caches of all layers.
 
-    def __init__(self, model, rows, longest, page=16, budget=None, sinks=4, recent=32):
+    ``beams`` texts may come to continue each row (``fork``; 0 for none); ``bits`` is 16 or 4.
+    """
+
+    def __init__(self, model, rows, longest, page=16, budget=None, sinks=4, recent=32, bits=16,
+                 beams=0):
+        if bits not in (4, 16):
+            raise ValueError("Session: a cache has 16 or 4 bits")
+        if budget and (bits == 4 or beams):
+            raise ValueError("Session: a budget needs the weights of a 16-bit cache, without beams")
         device = model.embedding.device
         self.model, self.page, self.budget = model, page, budget
         self.sinks, self.recent = sinks, recent
         self.slack = budget // 4 if budget else 0   # rows past the budget before it is cut
         width = -(-longest // page)
         kept = -(-budget // page) if budget else 0
-        self.free = list(range(rows * (width + kept)))
-        self.caches = [PagedCache.empty(len(self.free), model.kv_heads, page, device=device)
+        # Beams need a page each beside those that they had.
+        self.free = list(range(rows * beams * (width + 1) if beams else rows * (width + kept)))
+        kind = PagedCache4 if bits == 4 else PagedCache
+        self.caches = [kind.empty(len(self.free), model.kv_heads, page, device=device)
                        for _ in model.layers]
         self.pages = [[] for _ in range(rows)]        # as the table has them, on the host
         self.table = torch.full((rows, width), -1, dtype=torch.int32, device=device)
@@ -152,6 +168,19 @@ class Session:
                 self._attend(i, q[index], lengths, cu, max(stay))
         self.weights, self.voted = self.voted, self.weights
 
+    def fork(self, parents):
+        """Row i goes on with the text of old row ``parents[i]``."""
+        spare = [self.free.pop() for _ in parents]
+        held = {page for line in self.pages for page in line}
+        self.table, _ = fork_kv(self.caches, self.table, self._int32(self.lengths),
+                                self._int32(parents), self._int32(spare))
+        # As the table has it: full pages are shared, the last one is a row's own.
+        self.pages = [self.pages[p][:self.lengths[p] // self.page] + [page]
+                      for p, page in zip(parents, spare)]
+        self.lengths = [self.lengths[p] for p in parents]
+        self.positions = [self.positions[p] for p in parents]
+        self.free += sorted(held - {page for line in self.pages for page in line})
+
     def tidy(self):
         """Sequences well past the budget are cut to it."""
         if not self.weights or max(self.lengths) <= self.budget + self.slack:
@@ -185,14 +214,15 @@ def guess(text, most):
     return []
 
 
-def answer(model, prompts, tokens, drafts=4, temperature=0.0, budget=None, page=16, seed=0):
+def answer(model, prompts, tokens, drafts=4, temperature=0.0, budget=None, page=16, seed=0,
+           bits=16):
     """(texts, forward passes, evictions): each prompt with ``tokens`` more tokens."""
     if not prompts or not all(prompts):
         raise ValueError("answer: needs prompts of at least one token")
     device = model.embedding.device
     gen = torch.Generator(device=device).manual_seed(seed)
     longest = max(len(p) for p in prompts) + tokens + 2 * drafts + 2
-    session = Session(model, len(prompts), longest, page, budget)
+    session = Session(model, len(prompts), longest, page, budget, bits=bits)
     texts = [list(p) for p in prompts]
     pending = [list(p) for p in prompts]      # tokens that the cache does not hold yet
     passes = 0
@@ -230,6 +260,39 @@ def answer(model, prompts, tokens, drafts=4, temperature=0.0, budget=None, page=
     return [t[:len(p) + tokens] for t, p in zip(texts, prompts)], passes, session.evictions
 
 
+def beam_answer(model, prompts, tokens, beams=4, bits=16, page=16, session=None):
+    """(texts, scores): each prompt with the ``tokens`` more tokens that are the best of ``beams``
+    texts kept at a time, and the sum of their log-probabilities."""
+    if not prompts or not all(prompts):
+        raise ValueError("beam_answer: needs prompts of at least one token")
+    if tokens < 1 or beams < 1:
+        raise ValueError("beam_answer: needs at least one token and one beam")
+    rows = len(prompts)
+    device = model.embedding.device
+    longest = max(len(p) for p in prompts) + tokens + 1
+    session = session or Session(model, rows, longest, page, bits=bits, beams=beams)
+    logits = session.forward(prompts)
+    ends = torch.tensor([sum(session.counts[:row + 1]) - 1 for row in range(rows)], device=device)
+    # The first step: one text a row, and as many continuations of it as there are beams.
+    scores, parents, chosen = select_beams(logits[ends][:, None],
+                                           torch.zeros((rows, 1), device=device), beams)
+    texts = [list(p) for p in prompts for _ in range(beams)]
+    before = list(range(rows))                       # the session's row of each row's first text
+    for step in range(tokens):
+        follows = [before[row] + p for row, line in enumerate(parents.tolist()) for p in line]
+        if step:
+            texts = [list(texts[p]) for p in follows]
+        for text, token in zip(texts, chosen.flatten().tolist()):
+            text.append(token)
+        if step == tokens - 1:
+            break
+        session.fork(follows)
+        before = list(range(0, rows * beams, beams))
+        logits = session.forward([text[-1:] for text in texts])
+        scores, parents, chosen = select_beams(logits.view(rows, beams, -1), scores, beams)
+    return texts[::beams], scores[:, 0].tolist()
+
+
 def main():
     parser = argparse.ArgumentParser(description=__doc__.splitlines()[0])
     parser.add_argument("--layers", type=int, default=2)
@@ -237,13 +300,21 @@ def main():
     parser.add_argument("--budget", type=int, default=256)
     parser.add_argument("--temperature", type=float, default=0.0)
     parser.add_argument("--vocab", type=int, default=32000)
+    parser.add_argument("--bits", type=int, default=16, choices=(4, 16))
+    parser.add_argument("--beams", type=int, default=1)
     args = parser.parse_args()
     device = torch.device("cuda", torch.cuda.current_device())
     model = Model(device, args.layers, args.vocab)
     gen = torch.Generator().manual_seed(1)
     prompts = [torch.randint(0, args.vocab, (n,), generator=gen).tolist() for n in (300, 37, 180)]
-    texts, passes, evictions = answer(model, prompts, args.tokens, budget=args.budget,
-                                      temperature=args.temperature)
+    if args.beams > 1:
+        texts, scores = beam_answer(model, prompts, args.tokens, args.beams, args.bits)
+        for prompt, text, score in zip(prompts, texts, scores):
+            print(f"{len(prompt)} tokens, then {text[len(prompt):][:12]} ... ({score:.2f})")
+        return
+    texts, passes, evictions = answer(model, prompts, args.tokens, temperature=args.temperature,
+                                      budget=args.budget if args.bits == 16 else None,
+                                      bits=args.bits)
     for prompt, text in zip(prompts, texts):
         print(f"{len(prompt)} tokens, then {text[len(prompt):][:12]} ...")
     print(f"{args.tokens} tokens each in {passes} passes, {evictions} evictions")
