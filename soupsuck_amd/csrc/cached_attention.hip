@@ -45,6 +45,12 @@ namespace ss {
 namespace {
 
 constexpr int kRowBytes = kCacheDim * 2;
+// Tiles of a wave up to which a unit is one workgroup's.  So and cut, one sequence and eight, us:
+// 6 query rows a kv head (4 tiles are 1024 keys) 1000 keys 11.9 / 12.5 and 12.4 / 14.7, 2000 keys
+// 16.5 / 13.9 and 20.8 / 15.0; 30 rows, 500 keys 13.0 / 15.4 and 13.4 / 17.1, 1100 keys 16.2 / 15.8
+// and 16.4 / 17.3; 54 rows (512 keys) 500 keys 16.0 / 16.3 and 16.3 / 18.7, 700 keys 17.5 / 16.4 and
+// 17.8 / 18.7; 198 rows (256 keys) 250 keys 16.6 / 20.0 and 17.4 / 25.3.
+constexpr int kWholeTiles = 4;
 constexpr int kSteps = 31;      // tiles of a wave whose pages are looked up at once
 
 template <class T, int QT, int W, int RW>
@@ -483,6 +489,12 @@ __global__ __launch_bounds__(256) void cached_weights_again_kernel(CachedAttnArg
   }
 }
 
+Layout layout(int rows, int64_t tokens, int q_heads, int kv_heads, int max_new, int64_t max_length,
+              bool weights) {
+  return Layout(rows, tokens, q_heads, kv_heads, max_new, max_length, weights,
+                [](int, int64_t, int, int64_t tiles) { return tiles <= kWholeTiles; });
+}
+
 template <class T, int QT, int RW, bool SCORES, bool ONCE>
 int launch_attention(const CachedAttnArgs& a, const Layout& p, hipStream_t st) {
   const dim3 block(64 * kWaves);
@@ -559,7 +571,7 @@ extern "C" size_t ss_cached_attention_workspace_size(int rows, int64_t tokens, i
   if (rows <= 0 || tokens <= 0 || q_heads <= 0 || kv_heads <= 0 || max_new < 0 ||
       max_length < 0 || q_heads % kv_heads)
     return 0;
-  return ss::Layout(rows, tokens, q_heads, kv_heads, max_new, max_length, weights != 0).bytes;
+  return ss::layout(rows, tokens, q_heads, kv_heads, max_new, max_length, weights != 0).bytes;
 }
 
 extern "C" int ss_cached_attention(const ss_paged_cache* cache, const void* q, int64_t q_tok,
@@ -587,7 +599,8 @@ extern "C" int ss_cached_attention(const ss_paged_cache* cache, const void* q, i
   SS_CHECK_ARG(cache->k_row >= 0 && cache->k_row < (1 << 26) && cache->v_row >= 0 &&
                    cache->v_row < (1 << 26),
                "%s: cache rows must lie less than 2^26 elements apart", who);
-  const Layout p(rows, tokens, q_heads, cache->kv_heads, max_new, max_length, weights_out != 0);
+  const Layout p =
+      layout(rows, tokens, q_heads, cache->kv_heads, max_new, max_length, weights_out != 0);
   const int64_t cap = (int64_t)row_pages * cache->page_size;
   SS_CHECK_ARG(tokens <= (int64_t)INT32_MAX / q_heads && p.units <= kMaxGrid / 4 &&
                    (!weights_out || rows * (int64_t)cache->kv_heads * cdiv(cap, 4 * kKeys) <= kMaxGrid),

@@ -17,7 +17,6 @@
 namespace ss {
 namespace {
 
-constexpr int kRanges = 1;     // workgroups of a CU (blocks of 16 rows)
 constexpr int kDeep = 3;       // tiles of a wave on their way
 constexpr int kSteps = 27;     // tiles of a wave whose pages are looked up at once
 static_assert(kSteps % kDeep == 0 && 2 * (kSteps + kDeep) <= kWave, "a lane for every half tile");
@@ -281,6 +280,24 @@ __global__ __launch_bounds__(64 * W) void cached_attention4_kernel(CachedAttnArg
   if (blockIdx.x == 0) clear_outside<W>(a);
 }
 
+// One workgroup a unit, or the split: whole, the units that there are leave the other CUs without
+// work, a tile of a wave 0.9 us long (16 rows) or 1.5; split, the join comes after, 5.5 us and
+// one more for 1100 rows.  Past 16 tiles the lengths, which the bound says little of, matter more.
+// So and so, whole and split, us: 28 / 4 heads, one token, 1 / 8 / 32 sequences of 1500 keys 11.7
+// 12.7 / 11.8 13.1 / 12.8 16.8, of 3000 17.5 12.7 / 17.6 13.7 / 18.8 19.9; 12 / 2 heads, 5 tokens,
+// of 1500 15.9 13.5 / 16.0 14.4 / 16.3 17.0; 28 / 4 heads, 8 tokens, of 600 14.7 15.4 / 15.0 16.9 /
+// 15.6 29.5, of 1500 24.1 15.4 / 24.3 19.4 / 25.0 33.4.
+bool whole(int unit_rows, int64_t units, int cus, int64_t tiles) {
+  const double idle = units < cus ? 1.0 - (double)units / cus : 0.0;
+  const double tile = unit_rows <= 16 ? 0.9 : 1.5;
+  return tiles <= 16 && tiles * tile * idle <= 5.5 + (double)units * unit_rows / 1100;
+}
+
+Layout layout4(int rows, int64_t tokens, int q_heads, int kv_heads, int max_new,
+               int64_t max_length) {
+  return Layout(rows, tokens, q_heads, kv_heads, max_new, max_length, false, whole);
+}
+
 template <class T, int QT, int RW, bool ONCE>
 int launch_attention4(const CachedAttnArgs& a, const Layout& p, hipStream_t st) {
   constexpr int kW = kWaves;
@@ -338,8 +355,7 @@ extern "C" size_t ss_cached_attention4_workspace_size(int rows, int64_t tokens, 
   if (rows <= 0 || tokens <= 0 || q_heads <= 0 || kv_heads <= 0 || max_new < 0 ||
       max_length < 0 || q_heads % kv_heads)
     return 0;
-  return ss::Layout(rows, tokens, q_heads, kv_heads, max_new, max_length, false,
-                    ss::kRanges).bytes;
+  return ss::layout4(rows, tokens, q_heads, kv_heads, max_new, max_length).bytes;
 }
 
 extern "C" int ss_cached_attention4(const ss_paged_cache4* cache, const void* q, int64_t q_tok,
@@ -363,7 +379,7 @@ extern "C" int ss_cached_attention4(const ss_paged_cache4* cache, const void* q,
   SS_CHECK_ARG(aligned16(q) && aligned16(o) && ((q_tok | q_head | o_tok | o_head) & 7) == 0,
                "%s: needs 16-byte aligned bases and strides that are multiples of 8", who);
   SS_CHECK_ARG(max_new > 0, "%s: tokens, but max_new is 0", who);
-  const Layout p(rows, tokens, q_heads, cache->kv_heads, max_new, max_length, false, kRanges);
+  const Layout p = layout4(rows, tokens, q_heads, cache->kv_heads, max_new, max_length);
   SS_CHECK_ARG(tokens <= (int64_t)INT32_MAX / q_heads && p.units <= kMaxGrid / 4,
                "%s: too many tokens in one call", who);
   const size_t need = ss_cached_attention4_workspace_size(rows, tokens, q_heads, cache->kv_heads,

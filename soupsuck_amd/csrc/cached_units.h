@@ -26,12 +26,6 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kKeys = 32;       // of a tile
 constexpr int kPadDim = kCacheDim + 4;  // fp32 row of the waves' results in LDS
-// Tiles of a wave up to which a unit is one workgroup's.  So and cut, one sequence and eight, us:
-// 6 query rows a kv head (4 tiles are 1024 keys) 1000 keys 11.9 / 12.5 and 12.4 / 14.7, 2000 keys
-// 16.5 / 13.9 and 20.8 / 15.0; 30 rows, 500 keys 13.0 / 15.4 and 13.4 / 17.1, 1100 keys 16.2 / 15.8
-// and 16.4 / 17.3; 54 rows (512 keys) 500 keys 16.0 / 16.3 and 16.3 / 18.7, 700 keys 17.5 / 16.4 and
-// 17.8 / 18.7; 198 rows (256 keys) 250 keys 16.6 / 20.0 and 17.4 / 25.3.
-constexpr int kWholeTiles = 4;
 // Query rows of a kv head up to which their scores are kept (those of one 16-row block): kept
 // and with the keys again, 64 sequences of 7000 keys with 7 rows 196 and 249 us, 14 rows 215 and
 // 252, 16 rows (two kv heads) 117 and 135; 4 of them 27.9 / 32.4, 32.7 / 33.6, 25.2 / 26.8; 4 of
@@ -559,9 +553,11 @@ struct Layout {
   int score_rows;           // 0: no scores kept
   int64_t score_keys;
   size_t stats, list, ml, o, scores, bytes;  // workspace offsets
-  // ranges: workgroups of a CU that a block of at most 16 rows has room for.
+  // whole: whether the units are a workgroup's each, from the query rows of a unit, the units, the
+  // CUs and the tiles that a wave then has.
+  template <class Whole>
   Layout(int rows, int64_t tokens, int q_heads, int kv_heads, int new_bound, int64_t max_length,
-         bool weights, int ranges = 1) {
+         bool weights, Whole whole) {
     max_new = (int)(new_bound < tokens ? new_bound : tokens);
     const int64_t of_sequence = (int64_t)(max_new > 0 ? max_new : 1) * (q_heads / kv_heads);
     // A wave takes 16 rows, or 32, and up to four waves of 32 share a tile: 33 new tokens of 4
@@ -570,8 +566,9 @@ struct Layout {
     blocks = (int)cdiv(of_sequence, block_rows);
     units = (int64_t)rows * blocks * kv_heads;
     const int stripes = kWaves / (block_rows <= 32 ? 1 : block_rows / 32);
-    workers = max_length <= kWholeTiles * kKeys * stripes
-                  ? 0 : device_cu_count() * (block_rows == 16 ? ranges : 1);
+    const int unit_rows = (int)(of_sequence < block_rows ? of_sequence : block_rows);
+    workers = whole(unit_rows, units, device_cu_count(), cdiv(max_length, kKeys * stripes))
+                  ? 0 : device_cu_count();
     score_keys = cdiv(max_length > 0 ? max_length : 1, kKeys) * kKeys;
     score_rows = 0;
     if (weights && of_sequence <= kScoreRows &&

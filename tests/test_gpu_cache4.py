@@ -282,11 +282,16 @@ def test_attention_bounds_below_what_is_there(device):
     cache = PagedCache4(c.data, F16)
     q = tokens(9, 6, F16, device, 1)
     cu = offsets([6, 3], device)
+    # (Other bounds may lay a call out in another way, whose sums come in another order.)
+    k, v = values(c.data)
+    ref, reach_of, reach, _ = ocache.attention(host(q), k, v, c.table.tolist(),
+                                               c.lengths.tolist(), cu.tolist(), SCALE)
+    bound = attention_bound(F16, ref, reach_of, reach, 300)
     got = cached_attention(q, cache, c.table, c.lengths, cu, 4, 1000, SCALE)
     all_of = cached_attention(q, cache, c.table, c.lengths, cu, 6, 1000, SCALE)
-    assert (got[4:6] == 0).all() and torch.equal(got[:4], all_of[:4])
-    assert torch.equal(got[6:], all_of[6:])
-    k, v = values(c.data)
+    assert (got[4:6] == 0).all() and (np.abs(host(all_of) - ref) <= bound).all()
+    seen = [0, 1, 2, 3, 6, 7, 8]
+    assert (np.abs(host(got) - ref) <= bound)[seen].all()
     k[c.table[0, 16:].tolist()], v[c.table[0, 16:].tolist()] = np.nan, np.nan
     short = cached_attention(q, cache, c.table, c.lengths, cu, 6, 256, SCALE)
     assert not torch.isnan(short).any()
