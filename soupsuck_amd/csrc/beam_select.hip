@@ -15,8 +15,8 @@
 // by counting.  Keys in registers for all of it, with the code for each, left room for two waves
 // a SIMD: 104 us instead of 51 for 155 MB.
 // beam_join_kernel: a workgroup a sequence.  A wave joins a beam's sums and its slices' firsts in
-// the same way, then every candidate finds its rank by counting, or by a binary search in each
-// beam's line.
+// the same way, then the beams' firsts are ranked by counting, those that reach a bound where they
+// are many.
 //
 // 64 sequences x 8 beams x 151936 bf16 logits (155 MB): 36 us and 7 for the join.  It loads at 4.3
 // TB/s with the VALUs busy 55 of 100 cycles (an exponential is a quarter as fast as an addition);
@@ -41,10 +41,9 @@ constexpr int kMostBeams = 64;
 constexpr int kMostFirsts = 2048;  // beams * count: 32 KiB of LDS
 constexpr int kRounds = 16;      // of a slice at most: their maxima are kept, 1 KiB each
 constexpr int kRoom = 512;       // candidates ranked at once
-constexpr int kJoinWaves = 8;
 constexpr int kJoinRoom = 256;   // of a wave there
 constexpr int kJoinLoads = 10;   // of a lane on their way
-constexpr int kJoinCounted = 256;  // candidates up to which ranks are counted: independent reads
+constexpr int kJoinCounted = 128;  // candidates up to which ranks are counted
 
 struct SelectArgs {
   const char* logits;
@@ -86,10 +85,18 @@ template <int CTRL>
 __device__ __forceinline__ float moved(float v) {
   return __builtin_bit_cast(float, moved<CTRL>(__builtin_bit_cast(uint32_t, v)));
 }
+template <int CTRL, class V>
+__device__ __forceinline__ V moved_pair(V v) {
+  const u32x2 u = __builtin_bit_cast(u32x2, v);
+  return __builtin_bit_cast(V, u32x2{moved<CTRL>((uint32_t)u[0]), moved<CTRL>((uint32_t)u[1])});
+}
 template <int CTRL>
 __device__ __forceinline__ double moved(double v) {
-  const u32x2 u = __builtin_bit_cast(u32x2, v);
-  return __builtin_bit_cast(double, u32x2{moved<CTRL>((uint32_t)u[0]), moved<CTRL>((uint32_t)u[1])});
+  return moved_pair<CTRL>(v);
+}
+template <int CTRL>
+__device__ __forceinline__ uint64_t moved(uint64_t v) {
+  return moved_pair<CTRL>(v);
 }
 template <class V>
 __device__ __forceinline__ V lane_of(V v, int lane) {
@@ -126,6 +133,22 @@ __device__ __forceinline__ uint32_t nth_of_lanes(uint32_t mine, int n) {
   for (int i = 0; i < 64; ++i) rank += (uint32_t)__builtin_amdgcn_readlane((int)mine, i) > mine;
   return over_lanes(rank < n ? mine : ~0u, [](uint32_t a, uint32_t b) { return min(a, b); });
 }
+
+// The n-th greatest of the lanes' 128 numbers, two each.  Of 64 maxima over disjoint parts the
+// least is a poor bound: some 300 keys reach it.
+__device__ __forceinline__ uint32_t nth_of_pairs(uint32_t a, uint32_t b, int n) {
+  int rank_a = 0, rank_b = 0;
+#pragma unroll 8
+  for (int i = 0; i < 64; ++i) {
+    const uint32_t x = (uint32_t)__builtin_amdgcn_readlane((int)a, i);
+    const uint32_t y = (uint32_t)__builtin_amdgcn_readlane((int)b, i);
+    rank_a += (x > a) + (y > a);
+    rank_b += (x > b) + (y > b);
+  }
+  const uint32_t least = min(rank_a < n ? a : ~0u, rank_b < n ? b : ~0u);
+  return over_lanes(least, [](uint32_t u, uint32_t w) { return min(u, w); });
+}
+constexpr int kLanesBound = 32;  // counts up to which 64 maxima give the bound
 
 // The least key of a logit's order, or of any key.
 __device__ __forceinline__ uint64_t bound_from(uint32_t order) {
@@ -302,8 +325,14 @@ __global__ __launch_bounds__(kThreads) void beam_slice_kernel(SelectArgs a) {
                                fmaxf(tops[2][lane], tops[3][lane]));
   if (wave == 0) {
     // Lanes without a token of the slice have theirs behind its last one.
-    const bool some = start + lane * kEach < vocab;
-    const uint32_t nth = nth_of_lanes(some ? ordered(lane_top) : 0u, a.count);
+    auto order_of = [&](float l, int thread) {
+      return start + thread * kEach < vocab ? ordered(l) : 0u;
+    };
+    const uint32_t nth =
+        a.count <= kLanesBound
+            ? nth_of_lanes(order_of(lane_top, lane), a.count)
+            : nth_of_pairs(order_of(fmaxf(tops[0][lane], tops[1][lane]), lane),
+                           order_of(fmaxf(tops[2][lane], tops[3][lane]), 128 + lane), a.count);
     if (lane == 0) shared_bound = bound_from(nth);
   }
   terms.raise(greatest(lane_top));
@@ -346,15 +375,18 @@ __global__ __launch_bounds__(kThreads) void beam_slice_kernel(SelectArgs a) {
     a.base[unit] = terms.base();
     a.sums[unit] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
   }
+  // Turned by slice, so that a lane of the join has some of each rank: the maxima of lanes that
+  // held the slices' bests, and of others that held their lasts, gave a bound that most reached.
   uint64_t* out = a.best + unit * a.count;
+  auto turned = [&](int c) { return (c + 11 * slice) % a.count; };
   for (int c = threadIdx.x; c < used; c += kThreads) {
     const uint64_t key = room[c];
     int rank = 0;
 #pragma unroll 8
     for (int o = 0; o < used; ++o) rank += room[o] > key;
-    if (rank < a.count) out[rank] = key;
+    if (rank < a.count) out[turned(rank)] = key;
   }
-  for (int c = used + threadIdx.x; c < a.count; c += kThreads) out[c] = 0;
+  for (int c = used + threadIdx.x; c < a.count; c += kThreads) out[turned(c)] = 0;
 }
 
 // v ordered as an integer, 1 at least.
@@ -364,11 +396,13 @@ __device__ __forceinline__ uint64_t ordered(double v) {
   return u >> 63 ? ~u : u | (uint64_t)1 << 63;
 }
 
-__global__ __launch_bounds__(64 * kJoinWaves) void beam_join_kernel(SelectArgs a) {
-  __shared__ uint64_t rooms[kJoinWaves][kJoinRoom];
-  __shared__ int used_slots[kJoinWaves];
+// W waves: as many as there are beams, 16 at most.
+template <int W>
+__global__ __launch_bounds__(64 * W) void beam_join_kernel(SelectArgs a) {
+  __shared__ uint64_t rooms[W][kJoinRoom];
+  __shared__ int used_slots[W];
   // The beams' firsts in order: v (0 where there is none) and key.
-  extern __shared__ uint64_t lines[];
+  extern __shared__ __attribute__((aligned(16))) uint64_t lines[];
   uint64_t* vs = lines;
   uint64_t* keys = lines + a.beams * a.count;
   const int seq = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -377,7 +411,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void beam_join_kernel(SelectArgs a
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
   };
-  for (int b = wave; b < a.beams; b += kJoinWaves) {
+  for (int b = wave; b < a.beams; b += W) {
     const int64_t unit = ((int64_t)seq * a.beams + b) * a.slices;
     const uint64_t* best = a.best + unit * a.count;
     const int n = a.slices * a.count;
@@ -400,20 +434,29 @@ __global__ __launch_bounds__(64 * kJoinWaves) void beam_join_kernel(SelectArgs a
     // The first 64 slices' sums at once with all the rest.
     const double my_base = lane < a.slices ? a.base[unit + lane] : -INFINITY;
     const double my_sum = lane < a.slices ? a.sums[unit + lane] : 0.0;
-    uint64_t most = 0;
-    each_key([&](uint64_t key) { most = max(most, key); });
+    uint64_t most = 0, second = 0;
+    each_key([&](uint64_t key) {
+      second = max(second, min(most, key));
+      most = max(most, key);
+    });
     double base = my_base;
     for (int s = 64 + lane; s < a.slices; s += 64) base = fmax(base, a.base[unit + s]);
     base = over_lanes(base, [](double u, double w) { return fmax(u, w); });
+    // Bases are whole numbers over c, or (far) as good as 0 or nothing apart.
     auto scaled = [&](double of, double part) {  // 0 (or NaN) of a slice of -inf
-      return of == -INFINITY ? part : part * exp(of - base);
+      if (of == -INFINITY) return part;
+      return __builtin_ldexp(part, (int)fmax(rint((of - base) * (double)Terms::c), -4096.0));
     };
     double sum = scaled(my_base, my_sum);
     for (int s = 64 + lane; s < a.slices; s += 64)
       sum += scaled(a.base[unit + s], a.sums[unit + s]);
     sum = total(sum);
     const double whole = base + log(sum);
-    const uint64_t bound = bound_from(nth_of_lanes((uint32_t)(most >> 32), a.count));
+    const uint32_t nth =
+        a.count <= kLanesBound
+            ? nth_of_lanes((uint32_t)(most >> 32), a.count)
+            : nth_of_pairs((uint32_t)(most >> 32), (uint32_t)(second >> 32), a.count);
+    const uint64_t bound = bound_from(nth);
     uint64_t* room = rooms[wave];
     const int used = gather<kJoinRoom>(
         room, &used_slots[wave], bound, a.count, lane == 0,
@@ -448,37 +491,63 @@ __global__ __launch_bounds__(64 * kJoinWaves) void beam_join_kernel(SelectArgs a
     a.tokens[at] = (int64_t)(uint32_t)~(uint32_t)keys[c];
   };
   if (all <= kJoinCounted) {
-    // Four threads count for one.
+    // Four threads count for one, two candidates at a time (the one behind the last is there: a
+    // key, and not counted).
     const int part = threadIdx.x & 3;
-    for (int c = threadIdx.x >> 2; c < all; c += 16 * kJoinWaves) {
+    for (int c = threadIdx.x >> 2; c < all; c += 16 * W) {
       const uint64_t v = vs[c];
       uint32_t rank = 0;
 #pragma unroll 8
-      for (int o = part; o < all; o += 4) rank += (vs[o] > v) | ((vs[o] == v) & (o < c));
+      for (int o = 2 * part; o < all; o += 8) {
+        const u32x4 two = *reinterpret_cast<const u32x4*>(vs + o);
+        const uint64_t x = (uint64_t)two[1] << 32 | two[0], y = (uint64_t)two[3] << 32 | two[2];
+        rank += (x > v) | ((x == v) & (o < c));
+        rank += ((y > v) | ((y == v) & (o + 1 < c))) & (o + 1 < all);
+      }
       rank += moved<0xb1>(rank);  // quad_perm: the neighbour, then the other two
       rank += moved<0x4e>(rank);
       if (part == 0 && v) place(c, v, rank);
     }
     return;
   }
-  for (int c = threadIdx.x; c < all; c += 64 * kJoinWaves) {
-    const uint64_t v = vs[c];
-    if (!v) continue;
-    const int b = c / a.count;
-    int rank = c - b * a.count;
-    for (int o = 0; o < a.beams && rank < a.count; ++o) {
-      if (o == b) continue;
-      // Those of line o that come before: v' > v, and the equal ones of a lower beam.
-      const uint64_t least = v + (o > b);
-      int lo = 0, hi = a.count;
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (vs[o * a.count + mid] >= least) lo = mid + 1;
-        else hi = mid;
+  if (wave) return;
+  // Many: 64 of them, the first of each line in equal numbers, give a bound again.
+  const int each = 64 / a.beams, of_line = lane / each, in_line = lane - of_line * each;
+  const uint64_t mine =
+      of_line < a.beams && in_line < a.count ? vs[of_line * a.count + in_line] : 0;
+  const uint64_t bound = bound_from(nth_of_lanes((uint32_t)(mine >> 32), a.count));
+  uint32_t* those = reinterpret_cast<uint32_t*>(rooms);  // in order
+  int n = 0;
+  for (int c = lane; c - lane < all; c += 64) {
+    const bool reaches = c < all && vs[c] >= bound;
+    const uint64_t lanes = __ballot(reaches);
+    const int at = n + __popcll(lanes & (((uint64_t)1 << lane) - 1));
+    if (reaches && at < kJoinRoom) those[at] = c;
+    n += __popcll(lanes);
+  }
+  wave_sync();
+  if (n <= kJoinRoom) {
+    for (int i = lane; i < n; i += 64) {
+      const uint64_t v = vs[those[i]];
+      int rank = 0;
+#pragma unroll 8
+      for (int o = 0; o < n; ++o) {
+        const uint64_t x = vs[those[o]];
+        rank += (x > v) | ((x == v) & (o < i));
       }
-      rank += lo;
+      place(those[i], v, rank);
     }
-    place(c, v, rank);
+    return;
+  }
+  // Equal ones, -inf for instance: the lines are merged, of which a lane has one each.
+  const int first = lane * a.count;
+  uint64_t v = lane < a.beams ? vs[first] : 0;
+  for (int i = 0, at = 0; i < a.count; ++i) {
+    const uint64_t top = over_lanes(v, [](uint64_t x, uint64_t y) { return x > y ? x : y; });
+    if (lane != __ffsll((long long)__ballot(v == top)) - 1) continue;
+    place(first + at, v, i);
+    ++at;
+    v = at < a.count ? vs[first + at] : 0;
   }
 }
 
@@ -488,8 +557,12 @@ struct SelectLayout {
   SelectLayout(int sequences, int beams, int64_t vocab, int count, int width) {
     const int64_t lines = (int64_t)sequences * beams;
     const int64_t all = cdiv(vocab, (int64_t)kThreads * (16 / width));
-    // Slices for eight workgroups a CU, of one round of one load as long as there are fewer.
-    const int64_t wanted = cdiv(8 * (int64_t)device_cu_count(), lines);
+    // Slices for eight workgroups a CU, of one round of one load as long as there are fewer; not
+    // more than the join's lanes hold the firsts of at once (one sequence of 16 beams and 32
+    // each 34 us without).
+    int64_t wanted = cdiv(8 * (int64_t)device_cu_count(), lines);
+    const int64_t most = 64 * kJoinLoads / count;
+    wanted = wanted < most ? wanted : most;
     const int64_t each = cdiv(all, wanted < all ? wanted : all);
     pieces = each > 1 ? 2 : 1;
     rounds = (int)cdiv(each, pieces);
@@ -518,8 +591,10 @@ int launch(const SelectArgs& a, const SelectLayout& p, int sequences, hipStream_
   else
     hipLaunchKernelGGL((beam_slice_kernel<T, 2, false>), grid, block, lds, st, a);
   SS_CHECK_LAUNCH("beam_slice_kernel");
-  hipLaunchKernelGGL(beam_join_kernel, dim3((unsigned)sequences), dim3(64 * kJoinWaves),
-                     (unsigned)(a.beams * a.count * 16), st, a);
+  const dim3 sequence((unsigned)sequences);
+  const unsigned firsts = (unsigned)(a.beams * a.count * 16);
+  if (a.beams <= 8) hipLaunchKernelGGL(beam_join_kernel<8>, sequence, dim3(512), firsts, st, a);
+  else hipLaunchKernelGGL(beam_join_kernel<16>, sequence, dim3(1024), firsts, st, a);
   SS_CHECK_LAUNCH("beam_join_kernel");
   return SS_OK;
 }
