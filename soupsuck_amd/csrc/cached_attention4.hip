@@ -11,6 +11,19 @@
 // dimensions of one block, the operands of four products as they stand (the queries' dimensions
 // are taken in the same order: lane group g has 32 g + 8 s .. + 7 of product s), and 16 bytes
 // are four keys' values in eight columns, which permutes pair by key.
+//
+// What bounds it: 136 bytes a key and head leave the VALUs 1500 cycles for a tile of 32 keys at
+// HBM's rate, and 16 query rows take them 243 instructions (64 conversions, 32 permutes, 16 for the
+// values' scales, some 60 for the softmax), so a large batch is near both: 64 sequences of 5860
+// .. 8191 keys (245 MB) 51 us, 4.8 TB/s, the VALUs busy 60 of 100 cycles and the matrix cores 15.
+// Tiles on their way in the loop's order count more than their number: with the first ones' loads
+// in another order the loop's first wait was for all of them (53.7 us); 2, 3 and 4 tiles 51.5
+// (12 waves), 50.0 and 51.9 us; two workgroups a CU 60.2 (128 registers, some spilled).  Longer
+// blocks are bound by conversions, which every wave does for itself: 64 tokens of 4 sequences
+// (13.7 GFLOP) 39 us; decoded by one wave for four of 32 rows, through LDS with a barrier for
+// two tiles, 45.4.  One sequence is latency: 518 keys 7.7 us, 131071 keys (71 MB) 19 us, of which
+// 5 pass before the first tile is there and 2 to 3 after the last one, and 5 for the join.
+
 #include "cached_units.h"
 #include "paged4.h"
 
@@ -273,9 +286,7 @@ __global__ __launch_bounds__(64 * W) void cached_attention4_kernel(CachedAttnArg
                   bool whole, int slot) {
     attend4<T, QT, W, RW, ONCE>(a, lds, b, block, kv, seq, span, x0, x1, whole, slot);
   };
-  // Blocks of more than 32 rows are bound by their products, and equal parts are no better: 64
-  // tokens of 4 sequences 48.4 us against 45.7.
-  if constexpr (SPLIT) for_ranges<QT, W, RW, RW == 1>(a, lds, unit);
+  if constexpr (SPLIT) for_ranges<QT, W, RW, true>(a, lds, unit);
   else for_unit<QT, RW>(a, unit);
   if (blockIdx.x == 0) clear_outside<W>(a);
 }
@@ -293,9 +304,11 @@ bool whole(int unit_rows, int64_t units, int cus, int64_t tiles) {
   return tiles <= 16 && tiles * tile * idle <= 5.5 + (double)units * unit_rows / 1100;
 }
 
+// Blocks of 64 rows at most: 64 tokens of 4 sequences (448 rows a kv head) 42.9 us, in blocks of
+// 128 45.7 and of 32 54.7.
 Layout layout4(int rows, int64_t tokens, int q_heads, int kv_heads, int max_new,
                int64_t max_length) {
-  return Layout(rows, tokens, q_heads, kv_heads, max_new, max_length, false, whole);
+  return Layout(rows, tokens, q_heads, kv_heads, max_new, max_length, false, whole, 64);
 }
 
 template <class T, int QT, int RW, bool ONCE>
@@ -331,9 +344,7 @@ int launch4(const CachedAttnArgs& a, const Layout& p, hipStream_t st) {
     SS_CHECK_LAUNCH("cached_zeros_kernel");
     return SS_OK;
   }
-  if (p.block_rows > 32)
-    return p.block_rows == 64 ? launch_attention4<T, 2, 2, false>(a, p, st)
-                              : launch_attention4<T, 2, 4, false>(a, p, st);
+  if (p.block_rows > 32) return launch_attention4<T, 2, 2, false>(a, p, st);
   int64_t keys = a.max_length;
   if (a.window && a.window < keys && a.sinks < keys)
     keys = std::min(keys, a.window + a.sinks + a.max_new);

@@ -363,17 +363,18 @@ __device__ __forceinline__ bool equal_parts(const CachedAttnArgs& a, Segment& mi
   if (total > INT32_MAX / 2) return false;
   const int least = (int)quotient(total + a.workers - 1, a.workers);
   const int most = max((int)quotient(total + starts + a.workers - 1, a.workers), kMinRange);
+  // The largest parts first, which fit if any do, then the smallest that do.
   int parts = 0;
   int64_t upto = 0;
-  bool fits = false;
-#pragma unroll 1
-  for (int i = 0; i < 4 && !fits; ++i) {
-    const int size = max(least + (most - least) * i / 3, 1);
+  auto fit = [&](int size) {
     parts = (tiles + size - 1) / size;
     upto = lanes_upto((int64_t)parts) * hk;
-    fits = all(upto) <= a.workers;
-  }
-  if (!fits) return false;
+    return all(upto) <= a.workers;
+  };
+  if (!fit(max(most, 1))) return false;
+#pragma unroll 1
+  for (int i = 0; i < 4; ++i)
+    if (fit(max(least + (most - least) * i / 3, 1))) break;
   mine.x1 = 0;
   if ((int64_t)blockIdx.x >= all(upto)) return true;
   const int at = uniform(__ffsll((long long)__ballot(upto > (int64_t)blockIdx.x)) - 1);
@@ -557,12 +558,12 @@ struct Layout {
   // CUs and the tiles that a wave then has.
   template <class Whole>
   Layout(int rows, int64_t tokens, int q_heads, int kv_heads, int new_bound, int64_t max_length,
-         bool weights, Whole whole) {
+         bool weights, Whole whole, int widest = 128) {
     max_new = (int)(new_bound < tokens ? new_bound : tokens);
     const int64_t of_sequence = (int64_t)(max_new > 0 ? max_new : 1) * (q_heads / kv_heads);
     // A wave takes 16 rows, or 32, and up to four waves of 32 share a tile: 33 new tokens of 4
     // sequences (231 rows) 36 us in blocks of 128, 39 in blocks of 64.
-    block_rows = of_sequence <= 16 ? 16 : of_sequence <= 32 ? 32 : of_sequence <= 64 ? 64 : 128;
+    block_rows = of_sequence <= 16 ? 16 : of_sequence <= 32 ? 32 : of_sequence <= 64 ? 64 : widest;
     blocks = (int)cdiv(of_sequence, block_rows);
     units = (int64_t)rows * blocks * kv_heads;
     const int stripes = kWaves / (block_rows <= 32 ? 1 : block_rows / 32);

@@ -17,7 +17,9 @@
 // borders, half way between two steps, so the rotated key is taken without a rounding before
 // its own: products of 24 and 11 bits are exact in fp64, their sum is rounded to odd in fp32
 // (a last bit of 1 stands for whatever was cut off), which orders against every border as the
-// sum itself does.  The queries' rotation stays in fp32.
+// sum in fp64 does.  The queries' rotation stays in fp32.  6042 tokens (108 MB) 23.4 us, 4.6 TB/s.
+// Queries are sets of four heads for eight threads, which load the angles once for them: a head at
+// a time 25.4 us, its angles four times its own bytes; with heads of both kinds in a wave 24.9.
 #include "paged4.h"
 
 namespace ss {
