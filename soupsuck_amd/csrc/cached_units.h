@@ -119,6 +119,18 @@ __device__ __forceinline__ int64_t lanes_upto(int64_t v) {
   v = add_moved<0x142, 0xa>(v);  // the last lane of rows 0 and 2 to rows 1 and 3
   return add_moved<0x143, 0xc>(v);  // and of row 1 to rows 2 and 3
 }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t add_moved(uint32_t v) {
+  return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ uint32_t lanes_upto(uint32_t v) {
+  v = add_moved<0x111, 0xf>(v);
+  v = add_moved<0x112, 0xf>(v);
+  v = add_moved<0x114, 0xf>(v);
+  v = add_moved<0x118, 0xf>(v);
+  v = add_moved<0x142, 0xa>(v);
+  return add_moved<0x143, 0xc>(v);
+}
 // a / b of numbers from 0 and 1 up: seldom more than 32 bits.
 __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
   return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
@@ -202,6 +214,13 @@ __device__ __forceinline__ LateArgs* late_args() {
   return p;
 }
 
+// A workgroup's tiles [x0, x1) of a unit.
+struct Segment {
+  int line, kv, x0, x1, slot;
+  bool whole;
+  Sequence seq;
+};
+
 // What the workgroup's waves leave for each other, and 64 lines (sequence, block) of the split.
 template <int QT, int W>
 struct Results {
@@ -209,6 +228,8 @@ struct Results {
   int64_t upto[64];
   int tiles[64];
   Sequence seq[64];
+  Segment mine;
+  bool equal;
 };
 
 typedef __amdgpu_buffer_rsrc_t Rsrc;
@@ -255,43 +276,47 @@ __device__ __forceinline__ void finish_unit(const Results<QT, W>& lds, const Wav
 
   LateArgs* late = late_args();
   const int group = late->group;
-  for (int item = thread; item < 16 * QT * RW * 16; item += 64 * W) {
-    const int line = item >> 4, c = (item & 15) * 8;
+  // Columns of a thread and row: fewer where threads would have none.
+  constexpr int kCols = 16 * QT * RW * 16 <= 32 * W ? 4 : 8;
+  constexpr int kPieces = kCacheDim / kCols;
+  typedef T Out __attribute__((ext_vector_type(kCols)));
+  for (int item = thread; item < 16 * QT * RW * kPieces; item += 64 * W) {
+    const int line = item / kPieces, c = item % kPieces * kCols;
     if (block_row + line >= rows) continue;
     const int half = line / (16 * QT), r = line % (16 * QT);
     float top = -INFINITY;
 #pragma unroll
     for (int w = half; w < W; w += RW) top = fmaxf(top, lds.m[w][r]);
     const float base = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, o[8] = {};
+    float sum = 0.f, o[kCols] = {};
 #pragma unroll
     for (int w = half; w < W; w += RW) {
       const float f = __builtin_amdgcn_exp2f((lds.m[w][r] - base) * late->scale_log2);
       sum += f * lds.l[w][r];
-      const float4v x = *reinterpret_cast<const float4v*>(&waves[w].o[r][c]);
-      const float4v y = *reinterpret_cast<const float4v*>(&waves[w].o[r][c + 4]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        o[i] += f * x[i];
-        o[4 + i] += f * y[i];
+      for (int q = 0; q < kCols; q += 4) {
+        const float4v x = *reinterpret_cast<const float4v*>(&waves[w].o[r][c + q]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[q + i] += f * x[i];
       }
     }
     if (whole) {
       const int i = (block_row + line) / group;
       const int head = kv * group + block_row + line - i * group;
       const float inverse = sum == 0.f ? 0.f : 1.f / sum;
-      Vec8<T> out;
+      Out out;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) out[e] = (T)(sum == 0.f ? 0.f : o[e] * inverse);
-      *reinterpret_cast<Vec8<T>*>(late->o + (int64_t)(seq.start + i) * late->o_tok + head * late->o_head +
-                                  c * 2) = out;
+      for (int e = 0; e < kCols; ++e) out[e] = (T)(sum == 0.f ? 0.f : o[e] * inverse);
+      *reinterpret_cast<Out*>(late->o + (int64_t)(seq.start + i) * late->o_tok + head * late->o_head +
+                              c * 2) = out;
       if (late->stats && c == 0)
         late->stats[(int64_t)(seq.start + i) * late->hq + head] = row_stats<T>(base, sum, inverse);
     } else {
       const int64_t part = (int64_t)slot * 16 * QT * RW + line;
       float* out = late->part_o + part * kCacheDim + c;
-      *reinterpret_cast<float4v*>(out) = float4v{o[0], o[1], o[2], o[3]};
-      *reinterpret_cast<float4v*>(out + 4) = float4v{o[4], o[5], o[6], o[7]};
+#pragma unroll
+      for (int q = 0; q < kCols; q += 4)
+        *reinterpret_cast<float4v*>(out + q) = float4v{o[q], o[q + 1], o[q + 2], o[q + 3]};
       if (c == 0) *reinterpret_cast<float2v*>(late->part_ml + part * 2) = float2v{top, sum};
     }
   }
@@ -330,72 +355,61 @@ __global__ __launch_bounds__(256) void cached_zeros_kernel(CachedAttnArgs a) {
       u32x4{0, 0, 0, 0};
 }
 
-// A workgroup's tiles [x0, x1) of a unit.
-struct Segment {
-  int line, kv, x0, x1, slot;
-  bool whole;
-  Sequence seq;
-};
-
 // Units cut into equal parts, each a workgroup's (`mine`, with x1 0 where there is none left):
 // true where that is done.  A range that holds the end of one unit and the start of another goes through
 // both one after the other, 5 us more than the others take.  Parts of up to as many tiles as
 // a range has places (its units' starts counted) are therefore better, if there are workgroups
-// for all of them; with few units there are.  Every wave finds its part by itself.
+// for all of them; with few units there are.  For one wave.
 template <int QT, int RW>
 __device__ __forceinline__ bool equal_parts(const CachedAttnArgs& a, Segment& mine) {
+  constexpr int kMostTiles = 1 << 22;  // of a unit: sums over 128 units are 32-bit numbers
   const int hk = a.cache.kv_heads, lane = threadIdx.x & 63;
   const int lines = a.sequences * a.blocks;
-  if (lines > 64 || 2 * lines * hk > a.workers) return false;
   Sequence seq{};
-  int tiles = 0;
+  uint32_t tiles = 0;
   if (lane < lines) {
     const int b = lane / a.blocks;
     seq = Sequence(a, b);
     tiles = Span(a, seq, lane - b * a.blocks, 16 * QT * RW).tiles;
   }
-  auto all = [&](int64_t v) {
-    return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)v, 63) |
-                     (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), 63) << 32);
-  };
-  const int64_t total = all(lanes_upto(tiles)) * hk;
-  const int64_t starts = (int64_t)__popcll(__ballot(tiles > 0)) * hk * kStart;
-  if (total > INT32_MAX / 2) return false;
-  const int least = (int)quotient(total + a.workers - 1, a.workers);
-  const int most = max((int)quotient(total + starts + a.workers - 1, a.workers), kMinRange);
+  if (__any(tiles > kMostTiles)) return false;
+  auto all = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, 63); };
+  const uint32_t workers = a.workers, total = all(lanes_upto(tiles)) * hk;
+  const uint32_t starts = (uint32_t)__popcll(__ballot(tiles > 0)) * hk * kStart;
+  const uint32_t least = (total + workers - 1) / workers;
+  const uint32_t most = max((total + starts + workers - 1) / workers, (uint32_t)kMinRange);
   // The largest parts first, which fit if any do, then the smallest that do.
-  int parts = 0;
-  int64_t upto = 0;
-  auto fit = [&](int size) {
+  uint32_t parts = 0, upto = 0;
+  auto fit = [&](uint32_t size) {
     parts = (tiles + size - 1) / size;
-    upto = lanes_upto((int64_t)parts) * hk;
-    return all(upto) <= a.workers;
+    upto = lanes_upto(parts) * hk;
+    return all(upto) <= workers;
   };
-  if (!fit(max(most, 1))) return false;
+  if (!fit(most)) return false;
 #pragma unroll 1
-  for (int i = 0; i < 4; ++i)
-    if (fit(max(least + (most - least) * i / 3, 1))) break;
+  for (uint32_t i = 0; i < 4; ++i)
+    if (fit(max(least + (most - least) * i / 3, 1u))) break;
   mine.x1 = 0;
-  if ((int64_t)blockIdx.x >= all(upto)) return true;
-  const int at = uniform(__ffsll((long long)__ballot(upto > (int64_t)blockIdx.x)) - 1);
-  auto of_line = [&](int v) { return __builtin_amdgcn_readlane(v, at); };
+  if (blockIdx.x >= all(upto)) return true;
+  const int at = uniform(__ffsll((long long)__ballot(upto > blockIdx.x)) - 1);
+  auto of_line = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, at); };
   parts = of_line(parts);
   tiles = of_line(tiles);
-  const int within = (int)blockIdx.x - of_line((int)upto) + parts * hk;
-  const int part = within % parts;
+  const uint32_t within = blockIdx.x - of_line(upto) + parts * hk;
+  const uint32_t kv = within / parts, part = within - kv * parts;
   mine.line = at;
-  mine.kv = within / parts;
-  mine.x0 = (int)((int64_t)tiles * part / parts);
-  mine.x1 = (int)((int64_t)tiles * (part + 1) / parts);
+  mine.kv = kv;
+  mine.x0 = (int)((uint64_t)tiles * part / parts);
+  mine.x1 = (int)((uint64_t)tiles * (part + 1) / parts);
   mine.whole = parts == 1;
   mine.slot = 2 * (int)blockIdx.x;
   mine.seq.start = of_line(seq.start);
   mine.seq.n = of_line(seq.n);
   mine.seq.len = of_line(seq.len);
-  mine.seq.at = (int64_t)((uint64_t)(uint32_t)of_line((int)seq.at) |
-                          (uint64_t)(uint32_t)of_line((int)(seq.at >> 32)) << 32);
-  if (part == 0 && threadIdx.x == 0)
-    a.units[(int64_t)at * hk + mine.kv] = int4{(int)blockIdx.x, (int)blockIdx.x + parts - 1, 0, 0};
+  mine.seq.at = (int64_t)((uint64_t)of_line((uint32_t)seq.at) |
+                          (uint64_t)of_line((uint32_t)(seq.at >> 32)) << 32);
+  if (part == 0 && lane == 0)
+    a.units[(int64_t)at * hk + kv] = int4{(int)blockIdx.x, (int)(blockIdx.x + parts) - 1, 0, 0};
   return true;
 }
 
@@ -405,7 +419,28 @@ template <int QT, int W, int RW, bool PARTS, class F>
 __device__ __forceinline__ void for_ranges(const CachedAttnArgs& a, Results<QT, W>& lds, F unit_of) {
   const int hk = a.cache.kv_heads;
   Segment mine;
-  const bool equal = PARTS && equal_parts<QT, RW>(a, mine);
+  bool equal = false;
+  if constexpr (PARTS) {
+    // (Where there are at most half as many units as workgroups.)
+    if (a.sequences * a.blocks <= 64 && 2 * a.sequences * a.blocks * hk <= a.workers) {
+      if (threadIdx.x < 64) {
+        equal = equal_parts<QT, RW>(a, mine);
+        if (threadIdx.x == 0) lds.equal = equal, lds.mine = mine;
+      }
+      __syncthreads();
+      equal = uniform((int)lds.equal);
+      if (equal) {
+        mine = lds.mine;
+        mine.line = uniform(mine.line);
+        mine.kv = uniform(mine.kv);
+        mine.x0 = uniform(mine.x0);
+        mine.x1 = uniform(mine.x1);
+        mine.slot = uniform(mine.slot);
+        mine.whole = uniform((int)mine.whole);
+        mine.seq.settle();
+      }
+    }
+  }
   // Lines (sequence, block), 64 at a time: the places of each, and up to and with it.
   const int lane = threadIdx.x & 63;
   const int lines = a.sequences * a.blocks;
@@ -421,7 +456,7 @@ __device__ __forceinline__ void for_ranges(const CachedAttnArgs& a, Results<QT, 
         lds.tiles[lane] = places;
         if (places) places += kStart;
       }
-      lds.upto[lane] = lanes_upto(places);
+      lds.upto[lane] = lanes_upto((int64_t)places);
     }
     __syncthreads();
   };
