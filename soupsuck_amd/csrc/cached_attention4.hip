@@ -12,10 +12,11 @@
 // are taken in the same order: lane group g has 32 g + 8 s .. + 7 of product s), and 16 bytes
 // are four keys' values in eight columns, which permutes pair by key.
 //
-// What bounds it: 136 bytes a key and head leave the VALUs 1500 cycles for a tile of 32 keys at
-// HBM's rate, and 16 query rows take them 243 instructions (64 conversions, 32 permutes, 16 for the
-// values' scales, some 60 for the softmax), so a large batch is near both: 64 sequences of 5860
-// .. 8191 keys (245 MB) 51 us, 4.8 TB/s, the VALUs busy 60 of 100 cycles and the matrix cores 15.
+// What bounds it: a tile of 32 keys and 16 query rows takes a SIMD 1400 cycles (170 vector
+// instructions, 64 of them conversions, 32 permutes, 12 for the values' scales, some 50 for the
+// softmax, and 16 MFMAs, which overlap little), and HBM's rate leaves 1500 for its 4352 bytes,
+// so a large batch is near both: 64 sequences of 5860 .. 8191 keys (245 MB) 50 us, 4.9 TB/s, the
+// vector units busy 60 of 100 cycles and the matrix cores 15.
 // Tiles on their way in the loop's order count more than their number: with the first ones' loads
 // in another order the loop's first wait was for all of them (53.7 us); 2, 3 and 4 tiles 51.5
 // (12 waves), 50.0 and 51.9 us; two workgroups a CU 60.2 (128 registers, some spilled).  Longer

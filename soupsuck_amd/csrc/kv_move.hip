@@ -9,10 +9,9 @@
 // the rows that p has there already are copied, for all layers in one launch: a workgroup
 // takes 16 rows of one head, 8 KiB (16 bits) or a group (4 bits), in some of the layers.
 // Parent, length and table entry are three dependent loads, and that latency is what a small
-// fork costs: 28 layers of 4 beams 4.0 us; 32 beams of 4 heads (43 MB) 14.4 us, 20.7 with a
-// workgroup for every layer.  Reading those rows back (98 MB) takes 21 us, 4.7 TB/s, in a
-// workgroup for every layer: two of them one after the other took the same, and one
-// layer's read longer.
+// fork costs: 28 layers of 4 beams 4.0 us; 32 beams of 4 heads (43 MB) 12 us.  Reading those
+// rows back (98 MB) takes 21 us, 4.7 TB/s, in a workgroup for every layer: two of them one after
+// the other took the same, and one layer's read longer.
 #include "paged4.h"
 
 namespace ss {
@@ -229,9 +228,10 @@ int fork(const char* who, const Cache* const* caches, int count, const int32_t* 
   return in_launches(caches, count, [&](const Bases& bases, int first, int n) -> int {
     ForkArgs a{cache_view(cache), TableView{table, table_stride, row_pages, lengths}, rows,
                parents, spare, out_table, out_lengths, new_rows, bases};
-    // As many caches a workgroup as leave every CU eight.
+    // Four caches a workgroup, whose loads are on their way at once, where that leaves every CU
+    // eight: 32 beams of 28 layers 20.7, 12.0, 13.8, 14.8 and 16.4 us with 1, 4, 7, 14 and 28.
     const int64_t most = units * n / (8 * (int64_t)device_cu_count());
-    const int each = (int)(most < 1 ? 1 : most < 8 ? most : 8);
+    const int each = (int)(most < 1 ? 1 : most < 4 ? most : 4);
     hipLaunchKernelGGL((kv_fork_kernel<FOUR>), dim3((unsigned)units, (unsigned)cdiv(n, each)),
                        dim3(256), 0, st, a, n, each, first == 0);
     SS_CHECK_LAUNCH("kv_fork_kernel");
