@@ -312,18 +312,34 @@ Layout layout4(int rows, int64_t tokens, int q_heads, int kv_heads, int max_new,
   return Layout(rows, tokens, q_heads, kv_heads, max_new, max_length, false, whole, 64);
 }
 
+template <class T, int QT, int W, int RW, bool ONCE>
+int launch_whole4(const CachedAttnArgs& a, const Layout& p, hipStream_t st) {
+  hipLaunchKernelGGL((cached_attention4_kernel<T, QT, W, RW, false, ONCE>),
+                     dim3((unsigned)p.units), dim3(64 * W), 0, st, a);
+  SS_CHECK_LAUNCH("cached_attention4_kernel");
+  return SS_OK;
+}
+
 template <class T, int QT, int RW, bool ONCE>
 int launch_attention4(const CachedAttnArgs& a, const Layout& p, hipStream_t st) {
-  constexpr int kW = kWaves;
-  const dim3 block(64 * kW);
   if (!p.workers) {
-    hipLaunchKernelGGL((cached_attention4_kernel<T, QT, kW, RW, false, ONCE>),
-                       dim3((unsigned)p.units), block, 0, st, a);
-    SS_CHECK_LAUNCH("cached_attention4_kernel");
-    return SS_OK;
+    // More units than CUs: smaller workgroups, of which a CU holds several, so that one's start
+    // and end pass while another multiplies.  With 8, 4 and 2 waves, us: 512 units of a row, 40
+    // keys 9.7 7.1 7.1, 600 15.7 13.1 16.8, 2000 31.5 27.9 40.4; 1024 of a row, 40 keys 16.8
+    // 11.6 7.3, 600 28.4 23.6 19.7, 2000 61.6 53.5 50.6; 512 of 24 rows, 100 keys 14.9 15.0 9.4,
+    // 1000 29.8 33.0 26.2, 2000 43.0 50.8 44.2; 800 of up to 64, 40 keys 31.6 31.1 20.1, 600
+    // 54.2 66.4 56.4.
+    const int64_t cus = device_cu_count();
+    if constexpr (QT == 1) {
+      if (p.units >= 4 * cus) return launch_whole4<T, QT, 2, RW, ONCE>(a, p, st);
+      if (p.units > cus) return launch_whole4<T, QT, 4, RW, ONCE>(a, p, st);
+    } else if (p.units >= 2 * cus && a.max_length <= 16 * kKeys * (2 / RW)) {
+      return launch_whole4<T, QT, 2, RW, ONCE>(a, p, st);
+    }
+    return launch_whole4<T, QT, kWaves, RW, ONCE>(a, p, st);
   }
-  hipLaunchKernelGGL((cached_attention4_kernel<T, QT, kW, RW, true, ONCE>),
-                     dim3((unsigned)p.workers), block, 0, st, a);
+  hipLaunchKernelGGL((cached_attention4_kernel<T, QT, kWaves, RW, true, ONCE>),
+                     dim3((unsigned)p.workers), dim3(64 * kWaves), 0, st, a);
   SS_CHECK_LAUNCH("cached_attention4_kernel");
   const int64_t rows = (int64_t)a.max_new * a.group;
   hipLaunchKernelGGL((cached_join_kernel<T, 16 * QT * RW>),

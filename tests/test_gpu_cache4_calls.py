@@ -113,6 +113,28 @@ def test_attention_over_many_ranges(device, rows, new, hq, hk):
     check_attention(device, lengths, (new,) * rows, hq, hk, 16, BF16, seed=rows)
 
 
+@pytest.mark.parametrize("rows,new,hq,hk,window", [
+    (70, 3, 64, 8, None), (70, 3, 64, 8, 40),          # blocks of 32 rows on two waves
+    (36, 7, 128, 16, None), (36, 7, 128, 16, 40),      # of 64 rows on two waves
+    (68, 1, 8, 8, None), (150, 1, 8, 8, 40),           # of 16 rows on four, and on two
+])
+def test_attention_of_many_short_units(device, rows, new, hq, hk, window):
+    rng = np.random.default_rng(rows)
+    lengths = rng.integers(1, 200, rows).tolist()
+    lengths[::9] = [0] * len(lengths[::9])
+    lengths[2] = 270
+
+    def change(c):
+        # NaN blocks of values in a row that the last token alone sees, and in one that all see
+        for b, row in ((2, 269), (4, 0)):
+            page = c.table[b, row // 16].item()
+            if page >= 0:
+                c.data[page, 0, 0, 2112 + 16 + row % 16] = 255
+
+    check_attention(device, lengths, (new,) * rows, hq, hk, 16, F16, window, 2, seed=rows,
+                    change=change)
+
+
 @pytest.mark.parametrize("window", [None, 500])
 def test_attention_of_equal_parts(device, window):
     """Eight sequences whose units are cut into as many parts each."""
