@@ -281,7 +281,7 @@ __device__ __forceinline__ void attend4(const CachedAttnArgs& a, Shared4<QT, W>&
 }
 
 template <class T, int QT, int W, int RW, bool SPLIT, bool ONCE>
-__global__ __launch_bounds__(64 * W) void cached_attention4_kernel(CachedAttnArgs a) {
+__global__ __launch_bounds__(64 * W, 2) void cached_attention4_kernel(CachedAttnArgs a) {
   __shared__ Shared4<QT, W> lds;
   auto unit = [&](int b, int block, int kv, const Sequence& seq, const Span& span, int x0, int x1,
                   bool whole, int slot) {
@@ -323,19 +323,17 @@ int launch_whole4(const CachedAttnArgs& a, const Layout& p, hipStream_t st) {
 template <class T, int QT, int RW, bool ONCE>
 int launch_attention4(const CachedAttnArgs& a, const Layout& p, hipStream_t st) {
   if (!p.workers) {
-    // More units than CUs: smaller workgroups, of which a CU holds several, so that one's start
-    // and end pass while another multiplies.  With 8, 4 and 2 waves, us: 512 units of a row, 40
-    // keys 9.7 7.1 7.1, 600 15.7 13.1 16.8, 2000 31.5 27.9 40.4; 1024 of a row, 40 keys 16.8
-    // 11.6 7.3, 600 28.4 23.6 19.7, 2000 61.6 53.5 50.6; 512 of 24 rows, 100 keys 14.9 15.0 9.4,
-    // 1000 29.8 33.0 26.2, 2000 43.0 50.8 44.2; 800 of up to 64, 40 keys 31.6 31.1 20.1, 600
-    // 54.2 66.4 56.4.
+    // More units than CUs: workgroups of four waves, of which a CU holds two, so that one's start
+    // and end pass while another multiplies.  More than those hold at once: of two waves, where
+    // the work of a unit is little.  With 8, 4 and 2 waves, us: 320 units of 24 rows, 40 keys
+    // 14.2 9.0, 600 20.7 16.7, 2000 38.7 32.2; 640 of 24 rows, 40 keys - 14.2 9.4, 600 - 24.2
+    // 23.0; 800 of up to 64 rows, 40 keys - 19.9 14.0, 600 - 42.5 42.0; 448 of 64 rows, 600 keys
+    // 77.7 57.5 63.3, 2000 164.5 136 175; 1024 of one row, 40 keys - 11.1 7.3, 600 - 20.6 18.8,
+    // 2000 - 48.8 49.9; 2000 of seven rows, 40 keys - 17.4 12.2, 2000 - 97.9 103.
     const int64_t cus = device_cu_count();
-    if constexpr (QT == 1) {
-      if (p.units >= 4 * cus) return launch_whole4<T, QT, 2, RW, ONCE>(a, p, st);
-      if (p.units > cus) return launch_whole4<T, QT, 4, RW, ONCE>(a, p, st);
-    } else if (p.units >= 2 * cus && a.max_length <= 16 * kKeys * (2 / RW)) {
-      return launch_whole4<T, QT, 2, RW, ONCE>(a, p, st);
-    }
+    const bool little = QT == 1 || a.max_length <= 16 * kKeys * (2 / RW);
+    if (p.units > 2 * cus && little) return launch_whole4<T, QT, 2, RW, ONCE>(a, p, st);
+    if (p.units > cus) return launch_whole4<T, QT, 4, RW, ONCE>(a, p, st);
     return launch_whole4<T, QT, kWaves, RW, ONCE>(a, p, st);
   }
   hipLaunchKernelGGL((cached_attention4_kernel<T, QT, kWaves, RW, true, ONCE>),

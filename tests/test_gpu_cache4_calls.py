@@ -116,7 +116,10 @@ def test_attention_over_many_ranges(device, rows, new, hq, hk):
 @pytest.mark.parametrize("rows,new,hq,hk,window", [
     (70, 3, 64, 8, None), (70, 3, 64, 8, 40),          # blocks of 32 rows on two waves
     (36, 7, 128, 16, None), (36, 7, 128, 16, 40),      # of 64 rows on two waves
-    (68, 1, 8, 8, None), (150, 1, 8, 8, 40),           # of 16 rows on four, and on two
+    (68, 1, 8, 8, None), (150, 1, 8, 8, 40),           # of 16 rows on two waves
+    (40, 3, 64, 8, None), (40, 3, 64, 8, 40),          # each on four
+    (40, 7, 64, 8, None), (40, 7, 64, 8, 40),
+    (40, 1, 8, 8, None), (40, 1, 64, 8, 40),
 ])
 def test_attention_of_many_short_units(device, rows, new, hq, hk, window):
     rng = np.random.default_rng(rows)
