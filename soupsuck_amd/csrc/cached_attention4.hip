@@ -292,6 +292,55 @@ __global__ __launch_bounds__(64 * W, 2) void cached_attention4_kernel(CachedAttn
   if (blockIdx.x == 0) clear_outside<W>(a);
 }
 
+// The join of long blocks where a unit has few parts: a workgroup takes eight rows at once, 32
+// lanes of 4 columns each, part by part, or, of a unit that has more (a long sequence among short
+// ones), one after the other.  112 units of 64 rows, two parts each (7.3 MB): 5.4 us, with a
+// workgroup a row 8.4 (7168 of them, most of whose threads have no part).  Of 16 rows it is no
+// faster (64 units, 15 rows, four parts: the call 19.0 us against 17.7).
+constexpr int kFewParts = 8, kJoinRows = 8;
+template <class T, int ROWS>
+__global__ __launch_bounds__(32 * kJoinRows) void cached_join_rows_kernel(CachedAttnArgs a) {
+  __shared__ JoinShared lds;
+  const int hk = a.cache.kv_heads;
+  const int line = (int)(blockIdx.x / hk), kv = (int)(blockIdx.x - line * hk);
+  const int b = line / a.blocks, block = line - b * a.blocks;
+  const int4 unit = a.units[blockIdx.x];
+  const Sequence seq(a, b);
+  const int first = blockIdx.y * kJoinRows;
+  const int rows = min(kJoinRows, min(seq.n, a.max_new) * a.group - block * ROWS - first);
+  if (rows <= 0 || unit.x == unit.y) return;
+  const int count = unit.y - unit.x + 1;
+  if (count > kFewParts) {
+    for (int r = 0; r < rows; ++r) {
+      join_row<T, ROWS>(a, lds, seq, unit, block, kv, first + r);
+      __syncthreads();
+    }
+    return;
+  }
+  const int c = threadIdx.x & 31, r = threadIdx.x >> 5;
+  if (r >= rows) return;
+  auto part = [&](int i) {
+    return (int64_t)(2 * (unit.x + i) + (i ? 0 : unit.z)) * ROWS + first + r;
+  };
+  float2v s{-INFINITY, 0.f};  // of the lane's part
+  if (c < count) s = *reinterpret_cast<const float2v*>(a.part_ml + part(c) * 2);
+  float m = s[0];
+#pragma unroll
+  for (int d = kFewParts / 2; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, kFewParts));
+  m = __shfl(m, 0, 32);
+  const float base = m == -INFINITY ? 0.f : m;
+  const float f = __builtin_amdgcn_exp2f((s[0] - base) * a.scale_log2);
+  float sum = 0.f;
+  float4v o{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int i = 0; i < count; ++i) {
+    const float fi = __shfl(f, i, 32);
+    sum += fi * __shfl(s[1], i, 32);
+    o += fi * *reinterpret_cast<const float4v*>(a.part_o + part(i) * kCacheDim + 4 * c);
+  }
+  store_joined<T>(a, seq, kv, block * ROWS + first + r, c, o, sum, base);
+}
+
 // One workgroup a unit, or the split: whole, the units that there are leave the other CUs without
 // work, a tile of a wave 0.9 us long (16 rows) or 1.5; split, the join comes after, 5.5 us and
 // one more for 1100 rows.  Past 16 tiles the lengths, which the bound says little of, matter more.
@@ -340,8 +389,17 @@ int launch_attention4(const CachedAttnArgs& a, const Layout& p, hipStream_t st) 
                      dim3((unsigned)p.workers), dim3(64 * kWaves), 0, st, a);
   SS_CHECK_LAUNCH("cached_attention4_kernel");
   const int64_t rows = (int64_t)a.max_new * a.group;
-  hipLaunchKernelGGL((cached_join_kernel<T, 16 * QT * RW>),
-                     dim3((unsigned)p.units, (unsigned)(rows < p.block_rows ? rows : p.block_rows)),
+  const unsigned block = (unsigned)(rows < p.block_rows ? rows : p.block_rows);
+  if constexpr (QT > 1) {
+    if (p.units * kFewParts >= p.workers) {
+      hipLaunchKernelGGL((cached_join_rows_kernel<T, 16 * QT * RW>),
+                         dim3((unsigned)p.units, (block + kJoinRows - 1) / kJoinRows), dim3(256), 0,
+                         st, a);
+      SS_CHECK_LAUNCH("cached_join_rows_kernel");
+      return SS_OK;
+    }
+  }
+  hipLaunchKernelGGL((cached_join_kernel<T, 16 * QT * RW>), dim3((unsigned)p.units, block),
                      dim3(256), 0, st, a);
   SS_CHECK_LAUNCH("cached_join_kernel");
   return SS_OK;

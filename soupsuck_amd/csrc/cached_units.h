@@ -524,25 +524,37 @@ __device__ __forceinline__ void for_unit(const CachedAttnArgs& a, F unit_of) {
     unit_of(b, block, kv, seq, span, 0, span.tiles, true, 0);
 }
 
-// Parts of units that cross ranges: one workgroup a query row, 32 lanes of 4 columns for every
+// Four columns of a query row, from its parts' sums under the maximum `base`.
+template <class T>
+__device__ __forceinline__ void store_joined(const CachedAttnArgs& a, const Sequence& seq, int kv,
+                                             int row, int c, float4v o, float sum, float base) {
+  const int i = row / a.group;
+  const int head = kv * a.group + row - i * a.group;
+  T* out = reinterpret_cast<T*>(a.o + (int64_t)(seq.start + i) * a.o_tok + head * a.o_head) + 4 * c;
+  const float inverse = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) out[e] = (T)(sum == 0.f ? 0.f : o[e] * inverse);
+  if (a.stats && c == 0)
+    a.stats[(int64_t)(seq.start + i) * a.hq + head] = row_stats<T>(base, sum, inverse);
+}
+
+struct JoinShared {
+  float4v sums[8][32];
+  float ml[8][2];
+};
+
+// Parts of a unit that crosses ranges, row `at` of its block: 32 lanes of 4 columns for every
 // eighth part, joined in the order of the ranges.
 template <class T, int ROWS>
-__global__ __launch_bounds__(256) void cached_join_kernel(CachedAttnArgs a) {
-  __shared__ float4v sums[8][32];
-  __shared__ float ml[8][2];
-  const int hk = a.cache.kv_heads;
-  const int line = (int)(blockIdx.x / hk), kv = (int)(blockIdx.x - line * hk);
-  const int b = line / a.blocks, block = line - b * a.blocks;
-  const int row = block * ROWS + blockIdx.y;
-  const int4 unit = a.units[blockIdx.x];
-  const Sequence seq(a, b);
-  if (row >= min(seq.n, a.max_new) * a.group || unit.x == unit.y) return;
+__device__ __forceinline__ void join_row(const CachedAttnArgs& a, JoinShared& lds,
+                                         const Sequence& seq, int4 unit, int block, int kv,
+                                         int at) {
   const int c = threadIdx.x & 31, g = threadIdx.x >> 5;
   float4v o{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
 #pragma unroll 4
   for (int w = unit.x + g; w <= unit.y; w += 8) {
-    const int64_t p = (int64_t)(2 * w + (w == unit.x ? unit.z : 0)) * ROWS + blockIdx.y;
+    const int64_t p = (int64_t)(2 * w + (w == unit.x ? unit.z : 0)) * ROWS + at;
     const float2v s = *reinterpret_cast<const float2v*>(a.part_ml + p * 2);
     const float4v x = *reinterpret_cast<const float4v*>(a.part_o + p * kCacheDim + 4 * c);
     const float top = fmaxf(m, s[0]), base = top == -INFINITY ? 0.f : top;
@@ -552,29 +564,34 @@ __global__ __launch_bounds__(256) void cached_join_kernel(CachedAttnArgs a) {
     l = l * f + s[1] * h;
     m = top;
   }
-  sums[g][c] = o;
-  if (c == 0) ml[g][0] = m, ml[g][1] = l;
+  lds.sums[g][c] = o;
+  if (c == 0) lds.ml[g][0] = m, lds.ml[g][1] = l;
   __syncthreads();
   if (g) return;
 #pragma unroll
-  for (int i = 1; i < 8; ++i) m = fmaxf(m, ml[i][0]);
+  for (int i = 1; i < 8; ++i) m = fmaxf(m, lds.ml[i][0]);
   const float base = m == -INFINITY ? 0.f : m;
   float sum = 0.f;
   o = float4v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float f = __builtin_amdgcn_exp2f((ml[i][0] - base) * a.scale_log2);
-    sum += f * ml[i][1];
-    o += f * sums[i][c];
+    const float f = __builtin_amdgcn_exp2f((lds.ml[i][0] - base) * a.scale_log2);
+    sum += f * lds.ml[i][1];
+    o += f * lds.sums[i][c];
   }
-  const int i = row / a.group;
-  const int head = kv * a.group + row - i * a.group;
-  T* out = reinterpret_cast<T*>(a.o + (int64_t)(seq.start + i) * a.o_tok + head * a.o_head) + 4 * c;
-  const float inverse = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) out[e] = (T)(sum == 0.f ? 0.f : o[e] * inverse);
-  if (a.stats && c == 0)
-    a.stats[(int64_t)(seq.start + i) * a.hq + head] = row_stats<T>(base, sum, inverse);
+  store_joined<T>(a, seq, kv, block * ROWS + at, c, o, sum, base);
+}
+
+template <class T, int ROWS>
+__global__ __launch_bounds__(256) void cached_join_kernel(CachedAttnArgs a) {
+  __shared__ JoinShared lds;
+  const int hk = a.cache.kv_heads;
+  const int line = (int)(blockIdx.x / hk), kv = (int)(blockIdx.x - line * hk);
+  const int b = line / a.blocks, block = line - b * a.blocks;
+  const int4 unit = a.units[blockIdx.x];
+  const Sequence seq(a, b);
+  if (block * ROWS + (int)blockIdx.y >= min(seq.n, a.max_new) * a.group || unit.x == unit.y) return;
+  join_row<T, ROWS>(a, lds, seq, unit, block, kv, blockIdx.y);
 }
 
 // Waves of a workgroup side by side on the query rows of a block: one as long as a sequence

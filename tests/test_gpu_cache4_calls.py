@@ -145,6 +145,16 @@ def test_attention_of_equal_parts(device, window):
                     seed=3)
 
 
+@pytest.mark.parametrize("new,hq,hk", [(5, 8, 2), (9, 8, 2), (11, 14, 2)])
+def test_attention_of_one_long_among_short_ones(device, new, hq, hk):
+    """Its units have more parts than are joined row by row; blocks of 20, 36, 64 and 13 rows."""
+    lengths = [70 + 5 * i for i in range(24)]
+    lengths[5], lengths[6], lengths[20] = 20000, 0, 900
+    news = [new] * 24
+    news[7], news[8] = 0, 1
+    check_attention(device, lengths, news, hq, hk, 16, BF16, seed=new)
+
+
 @pytest.mark.parametrize("new", [5, 12, 40, 90])
 def test_attention_bounds_far_above_the_lengths(device, new):
     """Bounds that ask for the split where the sequences are short, or have nothing."""
