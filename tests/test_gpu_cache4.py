@@ -265,6 +265,30 @@ def test_attention_scales(device, scale):
     check_attention(device, (200, 70), (3, 1), 12, 2, 16, F16, scale=scale, seed=8)
 
 
+@pytest.mark.parametrize("new,hq,hk", [(1, 6, 2), (9, 6, 2)])
+@pytest.mark.parametrize("dtype,rise", [(F16, 0.98), (F16, 1.0), (BF16, 7.9), (BF16, 8.1)])
+def test_attention_maxima_that_rise_by_little(device, new, hq, hk, dtype, rise):
+    """Every eighth tile the scores rise by a power of two next to the one that sums are kept to."""
+    length = 8 * 32 * 7 - 5
+    c = build4([length], hk, 16, device, seed=3)
+    for j in range(0, length, 16):
+        page = c.table[0, j // 16].item()
+        keys = c.data[page, :, 0, :1024].view(hk, 4, 16, 16)
+        keys.zero_()
+        keys[:, 0, :, :j // 256] = 0x11                    # a score of one each: 0.5 + 0.5
+        c.data[page, :, 0, 2048:2112] = 127
+    cu = offsets([new], device)
+    q = torch.ones(new, hq, DIM, dtype=dtype, device=device)
+    scale = rise * np.log(2.0)
+    k, v = values(c.data)
+    ref, reach_of, reach, _ = ocache.attention(host(q), k, v, c.table.tolist(),
+                                               c.lengths.tolist(), cu.tolist(), scale, None, 0)
+    got = host(cached_attention(q, PagedCache4(c.data, dtype), c.table, c.lengths, cu, new, length,
+                                scale))
+    bound = attention_bound(dtype, ref, reach_of, reach, length)
+    assert (np.abs(got - ref) / bound).max() <= 1
+
+
 def test_attention_pages_that_are_not_held(device):
     def change(c):
         c.table[0, 2] = -1
