@@ -279,19 +279,26 @@ py::object evict_kv(int64_t cache_pointer, const Tensor& pages, py::handle table
 // The caches of a call, a list or tuple of one class: their structs' addresses (`_pointer`) and
 // devices (`_index`) by attribute, as a call for each layer's cache would cost more than its kernel.
 struct Caches {
+  py::object held;  // while the call runs without the lock, whatever becomes of a list
   std::vector<int64_t> pointers;
   bool ok = false, four = false;
   int64_t index = -1;
   Caches(py::handle caches, py::handle wide_type, py::handle four_type) {
     static PyObject* const pointer_name = PyUnicode_InternFromString("_pointer");
     static PyObject* const index_name = PyUnicode_InternFromString("_index");
-    const bool list = PyList_Check(caches.ptr());
-    if (!list && !PyTuple_Check(caches.ptr())) return;
-    const Py_ssize_t n = list ? PyList_GET_SIZE(caches.ptr()) : PyTuple_GET_SIZE(caches.ptr());
+    if (PyList_Check(caches.ptr()))
+      held = py::reinterpret_steal<py::object>(PyList_AsTuple(caches.ptr()));
+    else if (PyTuple_Check(caches.ptr()))
+      held = py::reinterpret_borrow<py::object>(caches);
+    if (!held) {
+      PyErr_Clear();
+      return;
+    }
+    const Py_ssize_t n = PyTuple_GET_SIZE(held.ptr());
     if (n == 0 || n >= INT32_MAX) return;
     pointers.reserve(n);
     for (Py_ssize_t i = 0; i < n; ++i) {
-      PyObject* cache = list ? PyList_GET_ITEM(caches.ptr(), i) : PyTuple_GET_ITEM(caches.ptr(), i);
+      PyObject* cache = PyTuple_GET_ITEM(held.ptr(), i);
       const bool is_four = (PyObject*)Py_TYPE(cache) == four_type.ptr();
       if (!is_four && (PyObject*)Py_TYPE(cache) != wide_type.ptr()) return;
       int64_t pointer, device;

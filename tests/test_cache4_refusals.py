@@ -268,6 +268,17 @@ def test_c_read_and_fork(raw):
     assert read(tokens=0) == fork(new=0) == _lib.OK
 
 
+def test_c_reads_and_forks_past_a_grid(raw):
+    """Eight threads a row and head, 256 a new row, head and 16 rows: 2^32 of them are refused."""
+    lib, cache, at, _ = raw
+    tokens = 2 ** 32 // 8 // cache.kv_heads
+    _refused(lib, lib.ss_kv_read4(_pointers(cache), 1, at, 3, 3, at, at, 2, tokens, at, at, None),
+             "too many")
+    rows = 2 ** 32 // 256 // cache.kv_heads // (cache.page_size // 16)
+    _refused(lib, lib.ss_kv_fork4(_pointers(cache), 1, at, 3, 3, at, 2, at, at, rows, at, at, None),
+             "too many")
+
+
 @pytest.mark.parametrize("change,needle", [
     (dict(dtype=7), "dtype"), (dict(rows=-1), "sizes"), (dict(beams=0), "sizes"),
     (dict(beams=65), "sizes"), (dict(vocab=0), "sizes"), (dict(count=0), "sizes"),
