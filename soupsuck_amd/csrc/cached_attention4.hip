@@ -21,8 +21,8 @@
 // in another order the loop's first wait was for all of them (53.7 us); 2, 3 and 4 tiles 51.5
 // (12 waves), 50.0 and 51.9 us; two workgroups a CU 60.2 (128 registers, some spilled).  Longer
 // blocks are bound by conversions, which every wave does for itself: 64 tokens of 4 sequences
-// (13.7 GFLOP) 39 us; decoded by one wave for four of 32 rows, through LDS with a barrier for
-// two tiles, 45.4.  One sequence is latency: 518 keys 7.7 us, 131071 keys (71 MB) 19 us, of which
+// (13.7 GFLOP) 37 us; decoded by one wave for four of 32 rows, through LDS with a barrier for
+// two tiles, 45.4, when this took 39.  One sequence is latency: 518 keys 7.7 us, 131071 keys (71 MB) 19 us, of which
 // 5 pass before the first tile is there and 2 to 3 after the last one, and 5 for the join.
 
 #include "cached_units.h"
