@@ -43,12 +43,17 @@ struct Shared4 : Results<QT, W> {
 };
 
 // A row's sums stay where they are until a tile's maximum is more than this power of two above the
-// one that they refer to: P is then as much above its lift, which bf16 holds anyhow and fp16 up to
-// 65504 (2^15.99 is 65070).  (Sums of n values of bf16 pass fp32 from 2^120 / n on, not 2^128 / n.)
-// A wave of a long call has few tiles, and in most of the first ones some row has a new maximum: 4
-// sequences of 64 tokens (bf16) 38.9 us, without 40.2.
+// one that they refer to.  A wave of a long call has few tiles, and in most of the first ones some
+// row has a new maximum: 4 sequences of 64 tokens (bf16) 38.9 us, without 40.2.
 template <class T>
 constexpr float kRise = std::is_same<T, half_t>::value ? 0.99f : 8.f;
+
+// Powers of two that P is raised by.  fp16: as over a 16-bit cache, and P, up to 2^0.99 above its
+// lift then, stays below 65504 (2^15.99 is 65070).  bf16: lowered by what sums may rise, so that P
+// is 1 at most and sums of values next to fp32's end (the cache holds up to 6 2^125) do not pass
+// it; P of at least 2^-8 at the top leaves the least value, 2^-126, 15 bits in fp32's subnormals.
+template <class T>
+constexpr float kLift4 = std::is_same<T, half_t>::value ? kLift<T> : -kRise<T>;
 
 // 32 rows of one kv head: two groups' parts, as the lanes load them.
 struct Tile4 {
@@ -236,7 +241,7 @@ __device__ __forceinline__ void attend4(const CachedAttnArgs& a, Shared4<QT, W>&
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const float w =
-                __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][i] - base_score, scale, kLift<T>));
+                __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][i] - base_score, scale, kLift4<T>));
             l[t] += w;
             p[t][i] = (T)w;
           }
