@@ -251,6 +251,7 @@ int append(const char* who, const Cache* cache, const void* k, int64_t k_tok, in
   const int cs = cs_dtype == SS_F32 ? 4 : 2;
   const int64_t sets = FOUR ? cdiv(hq, kQueryHeads) : 0;
   const int64_t items = tokens * (FOUR ? sets + 2 * (int64_t)cache->kv_heads : heads);
+  SS_CHECK_ARG(fits_grid(items, 32, 256), "%s: too many rows in one call", who);
   AppendArgs a{cache_view(cache), TableView{table, table_stride, row_pages, lengths},
                cu_seqlens, rows, (uint32_t)items, (uint32_t)(tokens * sets),
                (const char*)k, k_tok * 2, k_head * 2, (const char*)v, v_tok * 2, v_head * 2,

@@ -18,7 +18,6 @@ namespace ss {
 namespace {
 
 constexpr int kCaches = 64;  // of a launch: their bases are arguments
-constexpr int64_t kMostThreads = (int64_t)1 << 32;  // a grid has fewer, in each direction
 
 struct Bases {
   char* k[kCaches];
@@ -194,8 +193,9 @@ int read(const char* who, const Cache* const* caches, int count, const int32_t* 
   if (tokens == 0) return SS_OK;
   SS_CHECK_ARG(k && v && (rows == 0 || cu_seqlens), "%s: null pointer", who);
   SS_CHECK_ARG(aligned16(k) && aligned16(v), "%s: needs 16-byte aligned outputs", who);
-  SS_CHECK_ARG(tokens <= (kMostThreads - 1) / 8 / cache->kv_heads, "%s: too many rows in one call",
-               who);
+  SS_CHECK_ARG(tokens <= INT64_MAX / cache->kv_heads &&
+                   fits_grid(tokens * cache->kv_heads, 32, 256),
+               "%s: too many rows in one call", who);
   const int64_t each = tokens * cache->kv_heads * kCacheDim * 2;
   const hipStream_t st = (hipStream_t)stream;
   return in_launches(caches, count, [&](const Bases& bases, int first, int n) -> int {
@@ -225,7 +225,7 @@ int fork(const char* who, const Cache* const* caches, int count, const int32_t* 
   if (new_rows == 0) return SS_OK;
   SS_CHECK_ARG(parents && spare && out_table && out_lengths, "%s: null pointer", who);
   const int64_t units = (int64_t)new_rows * cache->kv_heads * (cache->page_size / kGroupRows);
-  SS_CHECK_ARG(units <= (kMostThreads - 1) / 256, "%s: too many rows in one call", who);
+  SS_CHECK_ARG(fits_grid(units, 1, 256), "%s: too many rows in one call", who);
   const hipStream_t st = (hipStream_t)stream;
   return in_launches(caches, count, [&](const Bases& bases, int first, int n) -> int {
     ForkArgs a{cache_view(cache), TableView{table, table_stride, row_pages, lengths}, rows,

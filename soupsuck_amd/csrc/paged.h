@@ -52,6 +52,12 @@ __device__ __forceinline__ int sequence_of(const int32_t* cu, int rows, int64_t 
   return cu[lo] <= t && t < cu[lo + 1] ? lo : -1;
 }
 
+// Whether a launch of `threads` a workgroup, each workgroup with `each` of the items, has a grid: of
+// fewer than 2^32 threads.
+inline bool fits_grid(int64_t items, int64_t each, int64_t threads) {
+  return cdiv(items, each) <= (int64_t)UINT32_MAX / threads;
+}
+
 inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 inline CacheView cache_view(const ss_paged_cache* c) {
