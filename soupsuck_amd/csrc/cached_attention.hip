@@ -539,8 +539,8 @@ int launch_attention(const CachedAttnArgs& a, const Layout& p, hipStream_t st) {
 template <class T>
 int launch(const CachedAttnArgs& a, const Layout& p, hipStream_t st) {
   if (a.sequences == 0) {
-    hipLaunchKernelGGL(cached_zeros_kernel, dim3((unsigned)cdiv(a.tokens * a.hq, 16)), dim3(256), 0,
-                       st, a);
+    hipLaunchKernelGGL(cached_zeros_kernel, dim3((unsigned)cdiv(a.tokens * a.hq, kZeroRows)),
+                       dim3(256), 0, st, a);
     SS_CHECK_LAUNCH("cached_zeros_kernel");
     return SS_OK;
   }
@@ -603,6 +603,7 @@ extern "C" int ss_cached_attention(const ss_paged_cache* cache, const void* q, i
       layout(rows, tokens, q_heads, cache->kv_heads, max_new, max_length, weights_out != 0);
   const int64_t cap = (int64_t)row_pages * cache->page_size;
   SS_CHECK_ARG(tokens <= (int64_t)INT32_MAX / q_heads && p.units <= kMaxGrid / 4 &&
+                   (rows > 0 || fits_grid(tokens * q_heads, kZeroRows, 256)) &&
                    (!weights_out || rows * (int64_t)cache->kv_heads * cdiv(cap, 4 * kKeys) <= kMaxGrid),
                "%s: too many tokens in one call", who);
   const size_t need = ss_cached_attention_workspace_size(rows, tokens, q_heads, cache->kv_heads,

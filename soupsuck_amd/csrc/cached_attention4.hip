@@ -428,8 +428,8 @@ constexpr int64_t kOnceBytes = (int64_t)32 << 20;
 template <class T>
 int launch4(const CachedAttnArgs& a, const Layout& p, hipStream_t st) {
   if (a.sequences == 0) {
-    hipLaunchKernelGGL(cached_zeros_kernel, dim3((unsigned)cdiv(a.tokens * a.hq, 16)), dim3(256), 0,
-                       st, a);
+    hipLaunchKernelGGL(cached_zeros_kernel, dim3((unsigned)cdiv(a.tokens * a.hq, kZeroRows)),
+                       dim3(256), 0, st, a);
     SS_CHECK_LAUNCH("cached_zeros_kernel");
     return SS_OK;
   }
@@ -480,7 +480,8 @@ extern "C" int ss_cached_attention4(const ss_paged_cache4* cache, const void* q,
                "%s: needs 16-byte aligned bases and strides that are multiples of 8", who);
   SS_CHECK_ARG(max_new > 0, "%s: tokens, but max_new is 0", who);
   const Layout p = layout4(rows, tokens, q_heads, cache->kv_heads, max_new, max_length);
-  SS_CHECK_ARG(tokens <= (int64_t)INT32_MAX / q_heads && p.units <= kMaxGrid / 4,
+  SS_CHECK_ARG(tokens <= (int64_t)INT32_MAX / q_heads && p.units <= kMaxGrid / 4 &&
+                   (rows > 0 || fits_grid(tokens * q_heads, kZeroRows, 256)),
                "%s: too many tokens in one call", who);
   const size_t need = ss_cached_attention4_workspace_size(rows, tokens, q_heads, cache->kv_heads,
                                                           max_new, max_length);

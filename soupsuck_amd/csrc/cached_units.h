@@ -347,8 +347,9 @@ __device__ __forceinline__ void clear_outside(const CachedAttnArgs& a) {
 }
 
 // Zeros for every token of a call without sequences.
+constexpr int kZeroRows = 16;  // of a workgroup
 __global__ __launch_bounds__(256) void cached_zeros_kernel(CachedAttnArgs a) {
-  const int64_t item = (int64_t)blockIdx.x * 256 + threadIdx.x, row = item / 16;
+  const int64_t item = (int64_t)blockIdx.x * 256 + threadIdx.x, row = item / (256 / kZeroRows);
   if (row >= a.tokens * a.hq) return;
   const int64_t t = row / a.hq;
   *reinterpret_cast<u32x4*>(a.o + t * a.o_tok + (row - t * a.hq) * a.o_head + (item & 15) * 16) =

@@ -47,3 +47,17 @@ def test_read_of_whole_workgroups(raw4):  # noqa: F811
     caches = (ctypes.c_void_p * 1)(ctypes.addressof(cache))
     for tokens in (2 ** 32 // 8 - 1, 2 ** 32 // 8 - 31):
         _too_many(lib, lib.ss_kv_read4(caches, 1, at, 3, 3, at, at, 2, tokens, at, at, None))
+
+
+def _attention(call, cache, at, tokens, weights):
+    return call(ctypes.byref(cache), at, 256, 128, 2, at, 3, 3, None, None, 0, tokens, 1, 48, 0.1,
+                0, 0, *weights, at, 256, 128, None, 0, None)
+
+
+def test_attention_without_sequences(raw, raw4):  # noqa: F811
+    """Zeros are written by 16 threads a row of a head."""
+    lib, cache, at, _ = raw
+    _, cache4, at4, _ = raw4
+    for tokens in (2 ** 32 // 16 // 2, 2 ** 30 - 1, 2 ** 32 // 16 // 2 - 7):
+        _too_many(lib, _attention(lib.ss_cached_attention, cache, at, tokens, (None, None)))
+        _too_many(lib, _attention(lib.ss_cached_attention4, cache4, at4, tokens, ()))
