@@ -244,7 +244,8 @@ extern "C" int ss_kv_evict(const ss_paged_cache* cache, const int32_t* table,
                "%s: workspace of %zu bytes, needs %zu", who, workspace_bytes, need);
   const int64_t lines = (int64_t)rows * cache->kv_heads;
   const int64_t items = (int64_t)out_pages * cache->page_size * lines;
-  SS_CHECK_ARG(lines <= INT32_MAX && cdiv(items, 16) <= INT32_MAX, "%s: too many rows", who);
+  SS_CHECK_ARG(fits_grid(lines, 1, kWaves * 64) && fits_grid(items, 16, 256), "%s: too many rows",
+               who);
   EvictArgs a{cache_view(cache), TableView{table, table_stride, row_pages, lengths}, rows,
               max_length, weights, out_table, out_stride, out_pages, budget, sinks, recent,
               out_lengths, out_weights, (int32_t*)workspace};

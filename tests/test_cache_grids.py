@@ -61,3 +61,12 @@ def test_attention_without_sequences(raw, raw4):  # noqa: F811
     for tokens in (2 ** 32 // 16 // 2, 2 ** 30 - 1, 2 ** 32 // 16 // 2 - 7):
         _too_many(lib, _attention(lib.ss_cached_attention, cache, at, tokens, (None, None)))
         _too_many(lib, _attention(lib.ss_cached_attention4, cache4, at4, tokens, ()))
+
+
+@pytest.mark.parametrize("rows,out_pages", [(2 ** 21, 2), (2 ** 31 - 1, 1), (2 ** 20, 2 ** 3)])
+def test_evict(raw, rows, out_pages):  # noqa: F811
+    """1024 threads for each kv head of a sequence; 16 for each row that it may keep."""
+    lib, cache, at, _ = raw
+    rc = lib.ss_kv_evict(ctypes.byref(cache), at, 3, 3, at, rows, 48, at, at, out_pages, out_pages,
+                         16, 0, 0, at, at, at, 2 ** 62, None)
+    _too_many(lib, rc)
