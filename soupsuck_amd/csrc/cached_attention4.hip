@@ -4,7 +4,10 @@
 // their split over the keys as over a 16-bit cache (cached_units.h).  Keys and values
 // become 16-bit numbers in registers, exactly (two significant bits times a power of two), on
 // v_cvt_scalef32_pk, which takes the block's scale with it; all products are 16-bit MFMAs,
-// so that the result is that of a 16-bit cache with the same rows.
+// so that the result is that of a 16-bit cache with the same rows.  As there P is rounded to the
+// cache's type, its product's operand, while its sum is of what was not rounded: bf16 outputs
+// lie 2.0e-3 of their norm from 64 bits, 1.7e-3 of it their own rounding, fp16 ones 2.2e-4 and
+// 2.1e-4 of that.
 //
 // Products (v_mfma_f32_16x16x32): S^T = K Q^T and O^T += V^T P^T, operands as over a 16-bit
 // cache.  A group of 16 rows is laid out for it: 16 bytes a lane are one key's 32
@@ -20,9 +23,12 @@
 // Tiles on their way in the loop's order count more than their number: with the first ones' loads
 // in another order the loop's first wait was for all of them (53.7 us); 2, 3 and 4 tiles 51.5
 // (12 waves), 50.0 and 51.9 us; two workgroups a CU 60.2 (128 registers, some spilled).  Longer
-// blocks are bound by conversions, which every wave does for itself: 64 tokens of 4 sequences
-// (13.7 GFLOP) 37 us; decoded by one wave for four of 32 rows, through LDS with a barrier for
-// two tiles, 45.4, when this took 39.  One sequence is latency: 518 keys 7.7 us, 131071 keys (71 MB) 19 us, of which
+// blocks are bound by vector instructions (373 a tile of 32 rows, conversions for each wave by itself
+// among them) that its products do not run beside: 64 tokens of 4 sequences (13.7 GFLOP) 37 us, of
+// whose 73700 cycles the vector units are busy 41400 and the matrix cores 13200.  They go by ranges
+// (parts of 55 tiles would be 308), 92 of which hold the end of one unit and the start of another.
+// Decoded by one wave for four of 32 rows, through LDS with a barrier for two tiles, 45.4, when
+// this took 39.  One sequence is latency: 518 keys 7.7 us, 131071 keys (71 MB) 19 us, of which
 // 5 pass before the first tile is there and 2 to 3 after the last one, and 5 for the join.
 
 #include "cached_units.h"
@@ -310,7 +316,7 @@ __global__ __launch_bounds__(64 * W, 2) void cached_attention4_kernel(CachedAttn
 
 // The join of long blocks where a unit has few parts: a workgroup takes eight rows at once, 32
 // lanes of 4 columns each, part by part, or, of a unit that has more (a long sequence among short
-// ones), one after the other.  112 units of 64 rows, two parts each (7.3 MB): 5.4 us, with a
+// ones), one after the other.  112 units of 64 rows, up to five parts each (ranges): 5.4 us, with a
 // workgroup a row 8.4 (7168 of them, most of whose threads have no part).  Of 16 rows it is no
 // faster (64 units, 15 rows, four parts: the call 19.0 us against 17.7).
 constexpr int kFewParts = 8, kJoinRows = 8;
@@ -394,7 +400,8 @@ int launch_attention4(const CachedAttnArgs& a, const Layout& p, hipStream_t st) 
     // 14.2 9.0, 600 20.7 16.7, 2000 38.7 32.2; 640 of 24 rows, 40 keys - 14.2 9.4, 600 - 24.2
     // 23.0; 800 of up to 64 rows, 40 keys - 19.9 14.0, 600 - 42.5 42.0; 448 of 64 rows, 600 keys
     // 77.7 57.5 63.3, 2000 164.5 136 175; 1024 of one row, 40 keys - 11.1 7.3, 600 - 20.6 18.8,
-    // 2000 - 48.8 49.9; 2000 of seven rows, 40 keys - 17.4 12.2, 2000 - 97.9 103.
+    // 2000 - 48.8 49.9; 2000 of seven rows, 40 keys - 17.4 12.2, 2000 - 97.9 103.  (Blocks of 16
+    // rows take two at any length, which costs those 2 and 5 % where sequences are long.)
     const int64_t cus = device_cu_count();
     const bool little = QT == 1 || a.max_length <= 16 * kKeys * (2 / RW);
     if (p.units > 2 * cus && little) return launch_whole4<T, QT, 2, RW, ONCE>(a, p, st);

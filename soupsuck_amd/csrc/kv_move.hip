@@ -11,7 +11,8 @@
 // Parent, length and table entry are three dependent loads, and that latency is what a small
 // fork costs: 28 layers of 4 beams 4.0 us; 32 beams of 4 heads (43 MB) 12 us.  Reading those
 // rows back (98 MB) takes 21 us, 4.7 TB/s, in a workgroup for every layer: two of them one after
-// the other took the same, and one layer's read longer.
+// the other took the same, and one layer's read longer.  Of 16 bits: four layers of 42976 tokens (704
+// MB) 124 us, 5.7 TB/s; one of 6042 tokens (25 MB) 6.3.
 #include "paged4.h"
 
 namespace ss {

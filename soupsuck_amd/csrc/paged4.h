@@ -3,7 +3,7 @@
 // A row has 128 keys and 128 values of one kv head, in blocks of 32 that share a scale 2^e.  A
 // value is a code of 4 bits (sign, two bits exponent, one mantissa: 0, 0.5, 1, 1.5, 2, 3, 4, 6)
 // times that scale, so two significant bits: exact in fp16 and bf16 as long as e keeps away
-// from the ends of their range (kLowest .. kHighest; past 6 2^kHighest codes saturate).  The
+// from the ends of their range (Exponents' lowest .. highest; past 6 2^highest codes saturate).  The
 // scale is the byte e + 127; 255 makes the block NaN (one that held an infinity or NaN).
 //
 // 16 rows of a page are a group of 2176 bytes, 17 lines of 128, laid out so that a wave of 64
